@@ -165,6 +165,20 @@ int dtf_head_f32_fused_fwd_bwd(const void* part, int S, const void* bias1, float
                                void* da, int B, int H, float grad_scale, float inv_keep, int backward, hipStream_t s);
 int dtf_head_f32_wgrad(const void* h1, const void* dlogits, const void* da, void* part, int B, int H, int KS,
                        hipStream_t s);
+// ---- global norm of a list of gradient tensors and clipping by it (clip.hip); mirrored in ops/clip.py ----
+struct DtfClipSpan {
+  const void* in;
+  void* out;              // may be `in`; not read by dtf_global_norm
+  long n;                 // elements
+  long in_pitch, out_pitch;   // elements between the starts of two rows (cols != 0)
+  int cols;               // elements of a row; 0: all n elements are contiguous
+  int dtype;              // 0 fp32, 1 bf16, 2 fp16
+};
+long dtf_clip_partials(int count, const DtfClipSpan* spans);
+int dtf_global_norm(int count, const DtfClipSpan* spans, void* partials, long slots, double scale, const void* hyper,
+                    void* hyper_out, int n_hyper, double limit, void* norm_out, hipStream_t s);
+int dtf_clip_by_global_norm(int count, const DtfClipSpan* spans, void* partials, long slots, double scale, double limit,
+                            void* norm_out, hipStream_t s);
 // asynchronous parameter server over peer-to-peer mailboxes (ps.hip)
 int dtf_ps_blocks();
 int dtf_ps_max_workers();

@@ -64,6 +64,22 @@ def accuracy(logits: torch.Tensor, labels: torch.Tensor) -> torch.Tensor:
     return (logits.argmax(-1) == labels.long()).float().mean()
 
 
+def global_norm(tensors, scale: float = 1.0) -> torch.Tensor:
+    """tf.global_norm: scale * sqrt(sum of all squares), in 64 bits."""
+    return scale * torch.stack([t.double().square().sum() for t in tensors]).sum().sqrt()
+
+
+def clip_by_global_norm(tensors, clip_norm: float, scale: float = 1.0):
+    """tf.clip_by_global_norm of scale * tensors: (clipped copies, norm before clipping).  A norm that is not finite
+    makes every value NaN."""
+    norm = global_norm(tensors, scale)
+    if not bool(torch.isfinite(norm)):
+        factor = torch.full_like(norm, float("nan"))
+    else:
+        factor = scale * clip_norm / torch.clamp(norm, min=clip_norm)
+    return [(t.double() * factor).to(t.dtype) for t in tensors], norm
+
+
 def truncated_normal(shape, stddev: float, generator=None, device="cpu") -> torch.Tensor:
     """tf.truncated_normal: N(0, stddev) with |z| > 2 sigma redrawn  (reference M:42-44)."""
     out = torch.empty(shape, device=device)
