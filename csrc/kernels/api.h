@@ -165,6 +165,14 @@ int dtf_head_f32_fused_fwd_bwd(const void* part, int S, const void* bias1, float
                                void* da, int B, int H, float grad_scale, float inv_keep, int backward, hipStream_t s);
 int dtf_head_f32_wgrad(const void* h1, const void* dlogits, const void* da, void* part, int B, int H, int KS,
                        hipStream_t s);
+// ---- classifier head with many classes (vocab_head.hip) ----
+long dtf_vocab_head_workspace(int dtype, int backward_pass, const void* h, long ldh, const void* w, long ldw, int n, int H, int V,
+                              int bias, int piece);
+int dtf_vocab_head_fwd(int dtype, const void* h, long ldh, const void* w, long ldw, const void* bias, const void* labels, int n,
+                       int H, int V, int ignore, void* loss, void* lse, void* ws, long ws_bytes, hipStream_t s);
+int dtf_vocab_head_bwd(int dtype, const void* h, long ldh, const void* w, long ldw, const void* bias, const void* labels,
+                       const void* lse, const void* row_scale, float grad_scale, int n, int H, int V, int ignore, int piece, void* dh,
+                       void* dw, int dw_f32, void* db, void* ws, long ws_bytes, hipStream_t s);
 // ---- global norm of a list of gradient tensors and clipping by it (clip.hip); mirrored in ops/clip.py ----
 struct DtfClipSpan {
   const void* in;

@@ -139,6 +139,12 @@ _SIGS = {
                                    c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int,
                                    c_float, c_float, c_int, c_void_p],
     "dtf_head_f32_wgrad": [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_void_p],
+    # ---- classifier head with many classes (csrc/kernels/vocab_head.hip) ----
+    "dtf_vocab_head_workspace": [c_int, c_int, c_void_p, c_long, c_void_p, c_long, c_int, c_int, c_int, c_int, c_int],
+    "dtf_vocab_head_fwd": [c_int, c_void_p, c_long, c_void_p, c_long, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_void_p,
+                           c_void_p, c_void_p, c_long, c_void_p],
+    "dtf_vocab_head_bwd": [c_int, c_void_p, c_long, c_void_p, c_long, c_void_p, c_void_p, c_void_p, c_void_p, c_float, c_int, c_int,
+                           c_int, c_int, c_int, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_long, c_void_p],
     # ---- global norm and clipping (csrc/kernels/clip.hip; spans: ops/clip.py ClipSpan) ----
     "dtf_clip_partials": [c_int, c_void_p],
     "dtf_global_norm": [c_int, c_void_p, c_void_p, c_long, c_double, c_void_p, c_void_p, c_int, c_double, c_void_p, c_void_p],
@@ -217,7 +223,7 @@ def load() -> ctypes.CDLL:
         fn = getattr(lib, name)
         fn.argtypes = argtypes
         fn.restype = (c_long if name in ("dtf_p2p_bytes", "dtf_p2p2_bytes", "dtf_dp_fabric_layout", "dtf_ps_ctl_bytes",
-                                         "dtf_gemm_f32_sk_workspace_bytes", "dtf_clip_partials")
+                                         "dtf_gemm_f32_sk_workspace_bytes", "dtf_clip_partials", "dtf_vocab_head_workspace")
                       else c_void_p if name == "dtf_gemm_f32_sk_workspace_alloc"
                       else None if name == "dtf_gemm_f32_sk_workspace_free" else c_int)
     lib.dtf_build_flavour.restype = c_char_p

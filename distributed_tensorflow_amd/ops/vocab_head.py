@@ -1,0 +1,156 @@
+"""Classifier head with many classes: softmax cross-entropy of ``h @ wT.T (+ bias)`` and its gradient, without logits.
+
+    loss_rows, lse = vocab_head_fwd(h, wT, labels, bias)
+    dh, dwT, dbias = vocab_head_bwd(h, wT, labels, lse, bias, grad_scale=1.0 / n)
+
+The ten-class head of the engine keeps a row's logits in registers; here the classes may be a vocabulary.  Conventions are
+the engine's: rows of hidden units ``h`` [n, hidden], the weight transposed ``wT`` [classes, hidden], int32 labels, the
+per-row loss and everything that is summed in fp32; both operands bf16 (gradients of them bf16 as well, ``dwT`` on request
+fp32) or both fp32 (exact-fp32 matrix cores).  Rows of ``h`` and ``wT`` may be further apart than they are long; rows that
+do not start on 16 bytes are copied once per call.
+
+A row whose label is ``ignore_label`` has loss 0 and takes no part in any gradient, whatever its hidden units hold
+(padding); any other label outside the classes makes its loss, and with it every gradient it enters, NaN, as
+``tf.nn.sparse_softmax_cross_entropy_with_logits`` does on a GPU.  A class can be masked by a bias of -inf.
+
+The backward pass computes the logits again, one piece of the classes at a time: its workspace holds two copies of the
+piece's bf16 / fp32 gradient of the logits and one of its weights.  Calls launch on the current stream of the operands'
+device, take their workspace from PyTorch's allocator on that stream and keep nothing, so they can be captured into HIP
+graphs and run on several streams at once.  Kernels: csrc/kernels/vocab_head.hip.
+"""
+from __future__ import annotations
+
+from typing import Optional, Tuple
+
+import torch
+
+from . import native
+from .native import check, ptr
+
+_DTYPES = {torch.float32: 0, torch.bfloat16: 1}
+_MAX_ROW = 1 << 20          # rows, hidden units and row strides of one call
+
+
+def _rows(t: torch.Tensor, name: str) -> int:
+    """Row stride (elements) of a matrix with contiguous rows."""
+    if t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1):
+        raise ValueError(f"{name} must be a matrix with contiguous rows, got shape {tuple(t.shape)}, strides {t.stride()}")
+    ld = max(t.stride(0), t.shape[1]) if t.shape[0] <= 1 else t.stride(0)
+    if ld < t.shape[1]:
+        raise ValueError(f"rows of {name} share memory (strides {t.stride()})")
+    if ld > _MAX_ROW or t.shape[1] > _MAX_ROW:
+        raise ValueError(f"rows of {name} may be at most {_MAX_ROW} elements long and apart, got {max(ld, t.shape[1])}")
+    return ld
+
+
+def _vector(t: Optional[torch.Tensor], name: str, n: int, dtype: torch.dtype, device: torch.device):
+    if t is None:
+        return
+    if t.dtype != dtype or t.shape != (n,) or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous {dtype} vector of {n} elements, got {t.dtype} {tuple(t.shape)}")
+    if t.device != device:
+        raise ValueError(f"{name} is on {t.device}, the hidden rows on {device}")
+
+
+def _check(h, wT, labels, bias, ignore_label) -> Tuple[int, int, int, int, int]:
+    if h.dtype not in _DTYPES or wT.dtype != h.dtype:
+        raise TypeError(f"h and wT must both be bf16 or both fp32, got {h.dtype} and {wT.dtype}")
+    ldh, ldw = _rows(h, "h"), _rows(wT, "wT")
+    n, hidden = h.shape
+    classes = wT.shape[0]
+    if wT.shape[1] != hidden:
+        raise ValueError(f"h has {hidden} hidden units, wT {wT.shape[1]}")
+    if hidden < 1 or not 1 <= classes < 1 << 30:
+        raise ValueError(f"at least one hidden unit and 1 to 2^30 - 1 classes expected, got wT {tuple(wT.shape)}")
+    if n > _MAX_ROW:
+        raise ValueError(f"at most {_MAX_ROW} rows per call, got {n}")
+    if wT.device != h.device:
+        raise ValueError(f"wT is on {wT.device}, the hidden rows on {h.device}")
+    _vector(labels, "labels", n, torch.int32, h.device)
+    _vector(bias, "bias", classes, torch.float32, h.device)
+    if not -(1 << 31) <= ignore_label < 1 << 31:
+        raise ValueError(f"ignore_label must be an int32, got {ignore_label}")
+    if h.device.type != "cuda":
+        raise ValueError(f"GPU tensors expected, got {h.device} (ops.reference.softmax_cross_entropy_with_logits runs on the CPU)")
+    return n, hidden, classes, ldh, ldw
+
+
+def vocab_head_fwd(h: torch.Tensor, wT: torch.Tensor, labels: torch.Tensor, bias: Optional[torch.Tensor] = None, *,
+                   ignore_label: int = -1) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(loss_rows, lse), fp32 [n]: per-row cross-entropy and the logarithm of the sum of exponentials of the logits (what the
+    backward pass needs)."""
+    n, hidden, classes, ldh, ldw = _check(h, wT, labels, bias, ignore_label)
+    loss = torch.empty(n, dtype=torch.float32, device=h.device)
+    lse = torch.empty(n, dtype=torch.float32, device=h.device)
+    if n == 0:
+        return loss, lse
+    lib, dt = native.load(), _DTYPES[h.dtype]
+    with torch.cuda.device(h.device):
+        stream = torch.cuda.current_stream(h.device).cuda_stream
+        need = lib.dtf_vocab_head_workspace(dt, 0, ptr(h), ldh, ptr(wT), ldw, n, hidden, classes, int(bias is not None), 0)
+        check(min(need, 0), "vocab_head_workspace")
+        ws = torch.empty(need, dtype=torch.uint8, device=h.device)
+        check(lib.dtf_vocab_head_fwd(dt, ptr(h), ldh, ptr(wT), ldw, ptr(bias), ptr(labels), n, hidden, classes, ignore_label,
+                                     ptr(loss), ptr(lse), ptr(ws), need, stream), "vocab_head_fwd")
+    return loss, lse
+
+
+def _span(t: torch.Tensor) -> Tuple[int, int]:
+    last = sum((s - 1) * st for s, st in zip(t.shape, t.stride())) if t.numel() else -1
+    return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
+
+
+def vocab_head_bwd(h: torch.Tensor, wT: torch.Tensor, labels: torch.Tensor, lse: torch.Tensor,
+                   bias: Optional[torch.Tensor] = None, *, grad_scale: float = 1.0, row_scale: Optional[torch.Tensor] = None,
+                   ignore_label: int = -1, need_dh: bool = True, need_dwT: bool = True, dh: Optional[torch.Tensor] = None,
+                   dwT: Optional[torch.Tensor] = None, dbias: Optional[torch.Tensor] = None, piece: int = 0):
+    """(dh, dwT, dbias) of sum_i grad_scale * row_scale[i] * loss_rows[i]; dbias is None without a bias, dh / dwT where they
+    are not wanted.  ``row_scale``: fp32 [n], the upstream gradient of the loss rows (default: ones).  ``dh`` / ``dwT`` /
+    ``dbias``: where to write (contiguous, 16-byte aligned; ``dwT`` in the operands' type or fp32), e.g. views of a gradient
+    arena.  ``piece``: classes per piece (rounded up to 256; 0: chosen from n)."""
+    n, hidden, classes, ldh, ldw = _check(h, wT, labels, bias, ignore_label)
+    _vector(lse, "lse", n, torch.float32, h.device)
+    _vector(row_scale, "row_scale", n, torch.float32, h.device)
+    if lse is None:
+        raise ValueError("lse is missing: it is the second result of vocab_head_fwd")
+    if not 0 <= piece <= _MAX_ROW:
+        raise ValueError(f"piece must lie between 0 and {_MAX_ROW}, got {piece}")
+    if dbias is not None and bias is None:
+        raise ValueError("dbias without a bias")
+    reads = [t for t in (h, wT, labels, lse, bias, row_scale) if t is not None]
+    for t, name, shape, types in ((dh, "dh", (n, hidden), (h.dtype,)), (dwT, "dwT", (classes, hidden), (h.dtype, torch.float32)),
+                                  (dbias, "dbias", (classes,), (torch.float32,))):
+        if t is None:
+            continue
+        if t.shape != shape or t.dtype not in types or not t.is_contiguous() or t.device != h.device or t.data_ptr() % 16:
+            raise ValueError(f"{name} must be a contiguous, 16-byte aligned {' or '.join(map(str, types))} tensor of shape {shape} "
+                             f"on {h.device}")
+        a, b = _span(t)
+        for other in reads:
+            c, d = _span(other)
+            if a < d and c < b:
+                raise ValueError(f"{name} shares memory with an operand or another output")
+        reads.append(t)
+    dev = h.device
+    if dh is None and need_dh:
+        dh = torch.empty((n, hidden), dtype=h.dtype, device=dev)
+    if dwT is None and need_dwT:
+        dwT = torch.empty((classes, hidden), dtype=h.dtype, device=dev)
+    if dbias is None and bias is not None:
+        dbias = torch.empty(classes, dtype=torch.float32, device=dev)
+    if n == 0:
+        for t in (dwT, dbias):
+            if t is not None:
+                t.zero_()
+        return dh, dwT, dbias
+    lib, dt = native.load(), _DTYPES[h.dtype]
+    with torch.cuda.device(dev):
+        stream = torch.cuda.current_stream(dev).cuda_stream
+        need = lib.dtf_vocab_head_workspace(dt, 1, ptr(h), ldh, ptr(wT), ldw, n, hidden, classes, int(dbias is not None), piece)
+        check(min(need, 0), "vocab_head_workspace")
+        ws = torch.empty(need, dtype=torch.uint8, device=dev)
+        check(lib.dtf_vocab_head_bwd(dt, ptr(h), ldh, ptr(wT), ldw, ptr(bias), ptr(labels), ptr(lse), ptr(row_scale),
+                                     float(grad_scale), n, hidden, classes, ignore_label, piece, ptr(dh), ptr(dwT),
+                                     int(dwT is not None and dwT.dtype == torch.float32), ptr(dbias), ptr(ws), need, stream),
+              "vocab_head_bwd")
+    return dh, dwT, dbias
