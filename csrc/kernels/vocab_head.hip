@@ -9,7 +9,8 @@
 // instead of the 6 n H V of a program that keeps n V logits), d of that piece is stored in the operand type, and two more
 // products make dw of the piece and add to dh, which is summed over the pieces in fp32.
 //
-// All products run through one kernel, vh_gemm: out[j][i] = sum_k A[i][k] B[j][k], both operands with contiguous k.
+// All products run through one kernel template, vh_gemm: out[j][i] = sum_k A(i, k) B(j, k), where an operand lies in memory
+// with k contiguous (fast) or with its rows contiguous (slow); nothing is transposed in memory.
 #include "common.hpp"
 #include "api.h"
 
@@ -21,15 +22,11 @@ typedef f32x4 f32x4_any __attribute__((aligned(4)));
 
 template <typename T> struct VhType;
 template <> struct VhType<bf16> {
-  static constexpr int KE = 32;     // elements of a 64-byte K tile row
-  typedef bf16x8 Vec;               // 16 bytes
   static __device__ __forceinline__ f32x4 mma(const u32x4& a, const u32x4& b, f32x4 c) {
     return mfma16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c);
   }
 };
 template <> struct VhType<float> {
-  static constexpr int KE = 16;
-  typedef f32x4 Vec;
   // lane group g holds k = 4 g .. 4 g + 3 of both operands; step s multiplies k = 4 g + s, so that the four steps cover
   // all sixteen
   static __device__ __forceinline__ f32x4 mma(const u32x4& a, const u32x4& b, f32x4 c) {
@@ -63,14 +60,14 @@ __device__ __forceinline__ void vh_barrier() {
   asm volatile("" ::: "memory");
 }
 
-struct VhTrue { static constexpr bool value = true; };
-struct VhFalse { static constexpr bool value = false; };
-
 struct VhOperands {
-  const void *A, *B;      // rows of K elements, lda / ldb elements apart, 16-byte aligned
+  // Fast operand: [rows][K], ld elements between rows, k contiguous.  Slow operand: [K][rows], ld elements between the K
+  // rows, padded to 16 bytes.  Rows start on 16 bytes.  A fast operand's K is a multiple of 16 bytes.
+  const void *A, *B;
   long lda, ldb;
-  int M, N, K;            // K: a multiple of 16 bytes
+  int M, N, Ka, Kb;       // Ka, Kb: k from there on counts as zero
   int tiles_m, tiles_n;
+  int ktiles, splits;     // K tiles of 128 bytes (of the operand type); workgroups that share a tile's K range
 };
 
 // C tile of a wave: lane l holds rows i = 16 mt + 4 (l >> 4) + r, column j = 16 nt + (l & 15) -- four consecutive i
@@ -82,122 +79,261 @@ struct VhTile {
   f32x4 acc[MT][NTL];
   int m0, n0;             // of the workgroup's tile
   int wm0, wn0;           // of the wave's tile, within the workgroup's
-  int lane, wave;
+  int lane, wave, split;
 };
 
-// Main loop.  K tiles of 64 bytes per row, D buffers in LDS, filled by LDS-DMA; rows of 64 bytes, the 16-byte chunk p of row
-// r holds chunk p ^ ((r >> 1) & 3), so that the fragment reads of 16 rows touch every bank once.
-// Phase t: DMA of tile t + D into the buffer of tile t (whose fragments every wave read before the last barrier) | read the
-// fragments of tile t + 1 | MFMAs on those of tile t | wait until tile t + 2 has landed | barrier.
-template <typename T, int BM, int BN, int NWM, int NWN, int D, class Tile>
-__device__ __forceinline__ void vh_mainloop(const VhOperands& p, Tile& c, char* lds) {
+// LDS-DMA of one operand's K tile (128 bytes of k for ROWS rows) and the fragment reads from it.
+//   fast: LDS rows of 128 bytes; chunk (16 bytes) p of row r holds chunk p ^ (r & 7): a fragment read of 16 rows touches
+//         every bank once.  A half tile is one 16-byte read per lane: group g holds the chunk g (bf16: k = 8 g .. 8 g + 7,
+//         fp32: k = 4 g .. 4 g + 3).
+//   slow: LDS rows are the K rows, ROWS elements long; the 16-element windows of a row are permuted by row.  bf16 fragments
+//         come from transposed reads, two per fragment, which give group g the k = 4 g .. 4 g + 3 and 16 + 4 g .. + 3 of the
+//         half; fp32 ones from four 4-byte reads, k = 4 g .. 4 g + 3 as in a fast operand.
+template <typename T, int ROWS, bool SLOW, int NT>
+struct VhLoader {
+  static constexpr int E = sizeof(T), KT = 128 / E, CH = ROWS * 8 / NT, CPR = ROWS * E / 16, ROWB = ROWS * E;
+  static_assert(ROWS * 8 % NT == 0 && (!SLOW || NT % CPR == 0), "every thread stages whole chunks");
+  const char* base;
+  long ld;
+  uint32_t v0, step;
+  int K, rows, kch;
+
+  __device__ __forceinline__ void init(const void* p, long ld_, int r0, int total, int K_, int tid) {
+    ld = ld_ * E;
+    K = K_;
+    rows = total - r0;
+    if (SLOW) {
+      rows = (rows + 16 / E - 1) & ~(16 / E - 1);      // whole chunks: a slow operand's K rows are padded to them
+      base = (const char*)p + (size_t)r0 * E;
+    } else {
+      base = (const char*)p + (size_t)r0 * ld;
+      kch = ((tid & 7) ^ ((tid >> 3) & 7)) << 4;       // the same for every chunk of a thread: NT is a multiple of 64
+      v0 = (uint32_t)(tid >> 3) * (uint32_t)ld + kch;
+      step = (uint32_t)(NT / 8) * (uint32_t)ld;
+    }
+  }
+  static __device__ __forceinline__ int key(int row) { return E == 2 ? (row & 7) << 1 : ((row >> 2) & 3) << 2; }
+  // lds: start of this operand's part of the buffer
+  __device__ __forceinline__ void dma(int t, char* lds, int wave, int tid) const {
+    char* const dst = lds + wave * 1024;
+    if constexpr (SLOW) {
+      const int left = K - t * KT;
+      const size_t bytes = left > 0 ? (size_t)(left - 1) * ld + (size_t)rows * E : 0;
+      const __amdgpu_buffer_rsrc_t r = make_rsrc(base + (size_t)t * KT * ld, bytes < 0x7ffffff0u ? bytes : 0x7ffffff0u);
+#pragma unroll
+      for (int i = 0; i < CH; ++i) {
+        const int q = tid + i * NT, row = q / CPR, ch = q % CPR;
+        vh_dma16(r, dst + i * NT * 16, (uint32_t)row * (uint32_t)ld + ((ch ^ key(row)) << 4), 0);
+      }
+    } else {
+      const uint32_t so = (uint32_t)t << 7;
+      const int n = rows < ROWS ? rows : ROWS;
+      const __amdgpu_buffer_rsrc_t r = make_rsrc(base, (size_t)(n - 1) * ld + (size_t)K * E);
+      // K may end inside the tile: zeros from there on (an offset behind every descriptor: tiles span less than 2 GB)
+      const uint32_t v = (int)so + kch < K * E ? v0 : 0x80000000u;
+#pragma unroll
+      for (int i = 0; i < CH; ++i) vh_dma16(r, dst + i * NT * 16, v + i * step, so);
+    }
+  }
+};
+
+// fragments of 16 rows r0 .. r0 + 15 (+ 16 i) from an operand's LDS part, half 0 or 1 of the K tile
+template <typename T, int ROWS, bool SLOW, int CNT>
+struct VhFrags {
+  static constexpr int E = sizeof(T), ROWB = ROWS * E;
+  int off;
+  __device__ __forceinline__ void init(int r0, int lane) {
+    const int i16 = lane & 15, g = lane >> 4;
+    if (!SLOW) off = (r0 + i16) * 128 + ((g ^ (i16 & 7)) << 4);
+    else if (E == 2) off = (4 * g + (i16 >> 2)) * ROWB + ((((r0 >> 4) ^ ((4 * g + (i16 >> 2)) & 7))) << 5) + 8 * (i16 & 3);
+    else off = 4 * g * ROWB + (((r0 >> 4) ^ g) << 6) + 4 * i16;
+  }
+  __device__ __forceinline__ void read(u32x4 (&f)[CNT], const char* lds, int half) const {
+    static_assert(!SLOW || E == 4, "bf16 slow operands are read by read_tr");
+    if constexpr (!SLOW) {
+      const char* p = lds + (off ^ (half << 6));
+#pragma unroll
+      for (int i = 0; i < CNT; ++i) f[i] = *reinterpret_cast<const u32x4*>(p + i * 2048);
+    } else {
+      const char* p = lds + half * 16 * ROWB;
+#pragma unroll
+      for (int i = 0; i < CNT; ++i)
+#pragma unroll
+        for (int s = 0; s < 4; ++s) f[i][s] = *reinterpret_cast<const unsigned*>(p + (off ^ (i << 6)) + s * ROWB);
+    }
+  }
+  // Two fragments i, i + 1 of a bf16 slow operand.  The reads and the wait for them are one block: nothing between them can
+  // use, move or reuse a register that is still being written.
+  __device__ __forceinline__ void read_tr2(u32x4& f0, u32x4& f1, const char* lds, int half, int i) const {
+    const uint32_t p = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void*)(const void*)(lds + half * 32 * ROWB);
+    const uint32_t a0 = p + (off ^ (i << 5)), a1 = p + (off ^ ((i + 1) << 5));
+    u32x2 x0, x1, y0, y1;
+    asm volatile(
+        "ds_read_b64_tr_b16 %0, %4\n\t"
+        "ds_read_b64_tr_b16 %1, %4 offset:%6\n\t"
+        "ds_read_b64_tr_b16 %2, %5\n\t"
+        "ds_read_b64_tr_b16 %3, %5 offset:%6\n\t"
+        "s_waitcnt lgkmcnt(0)"
+        : "=&v"(x0), "=&v"(x1), "=&v"(y0), "=&v"(y1)
+        : "v"(a0), "v"(a1), "n"(16 * ROWB)
+        : "memory");
+    f0 = (u32x4){x0[0], x0[1], x1[0], x1[1]};
+    f1 = (u32x4){y0[0], y0[1], y1[0], y1[1]};
+  }
+};
+
+// Main loop: K tiles t0 .. t1 - 1 in two LDS buffers.
+//
+// Both operands fast (or fp32): a tile is multiplied in two halves, and the fragments of a half are read during the MFMAs of
+// the half before it, one barrier per tile:
+//   read the second half of tile t | MFMAs on the first | wait until tile t + 1 has landed, barrier
+//   DMA of tile t + 2 into the buffer of tile t | read the first half of tile t + 1 | MFMAs on the second half of tile t
+// A bf16 slow operand (its fragments are read right before their MFMAs; the other wave of the SIMD covers the wait):
+//   wait until tile t has landed, barrier | DMA of tile t + 1 into the buffer of tile t - 1 | both halves of tile t
+template <typename T, int BM, int BN, int NWM, int NWN, bool AS, bool BS, class Tile>
+__device__ __forceinline__ void vh_mainloop(const VhOperands& p, Tile& c, char* lds, int t0, int t1) {
   constexpr int NT = Tile::NT, MT = Tile::MT, NTL = Tile::NTL;
-  constexpr int ACH = BM * 4 / NT, BCH = BN * 4 / NT, NDMA = ACH + BCH;
-  static_assert(BM * 4 % NT == 0 && BN * 4 % NT == 0, "every thread stages whole chunks");
-  constexpr int ABYTES = BM * 64, STAGE = (BM + BN) * 64;
-  const int tid = threadIdx.x, lane = c.lane, i16 = lane & 15, g = lane >> 4;
-  const int E = (int)sizeof(T);
-  const int rows_a = min(BM, p.M - c.m0), rows_b = min(BN, p.N - c.n0);
-  const __amdgpu_buffer_rsrc_t ra = make_rsrc((const char*)p.A + (size_t)c.m0 * p.lda * E, ((size_t)(rows_a - 1) * p.lda + p.K) * E);
-  const __amdgpu_buffer_rsrc_t rb = make_rsrc((const char*)p.B + (size_t)c.n0 * p.ldb * E, ((size_t)(rows_b - 1) * p.ldb + p.K) * E);
-  uint32_t va[ACH], vb[BCH];
-#pragma unroll
-  for (int i = 0; i < ACH; ++i) {
-    const int q = tid + i * NT, row = q >> 2;
-    va[i] = (uint32_t)row * (uint32_t)(p.lda * E) + (((q & 3) ^ ((row >> 1) & 3)) << 4);
-  }
-#pragma unroll
-  for (int i = 0; i < BCH; ++i) {
-    const int q = tid + i * NT, row = q >> 2;
-    vb[i] = (uint32_t)row * (uint32_t)(p.ldb * E) + (((q & 3) ^ ((row >> 1) & 3)) << 4);
-  }
-  const int kbytes = p.K * E, T_ = (kbytes + 63) >> 6;
-  // chunks of a lane: byte offset of its chunk within the 64-byte row (the same for every i: NT is a multiple of 8 rows)
-  const int kch = (((tid & 3) ^ ((tid >> 3) & 3)) << 4);
-  auto dma = [&](int t, int buf) {
-    const uint32_t so = (uint32_t)t << 6;
-    const bool in = (int)so + kch < kbytes;          // the last K tile may end inside the row: zeros from there on
-    char* const base = lds + buf * STAGE + c.wave * 1024;
-#pragma unroll
-    for (int i = 0; i < ACH; ++i) vh_dma16(ra, base + i * NT * 16, in ? va[i] : 0xfffffff0u, so);
-#pragma unroll
-    for (int i = 0; i < BCH; ++i) vh_dma16(rb, base + ABYTES + i * NT * 16, in ? vb[i] : 0xfffffff0u, so);
-  };
-  u32x4 fa[2][MT], fb[2][NTL];
-  const int sw = (g ^ ((i16 >> 1) & 3)) << 4;
-  const int oa = (c.wm0 + i16) * 64 + sw, ob = ABYTES + (c.wn0 + i16) * 64 + sw;
-  auto frags = [&](u32x4 (&a)[MT], u32x4 (&b)[NTL], int buf) {
-    const char* base = lds + buf * STAGE;
-#pragma unroll
-    for (int i = 0; i < MT; ++i) a[i] = *reinterpret_cast<const u32x4*>(base + oa + i * 1024);
-#pragma unroll
-    for (int j = 0; j < NTL; ++j) b[j] = *reinterpret_cast<const u32x4*>(base + ob + j * 1024);
-  };
-  auto mma = [&](const u32x4 (&a)[MT], const u32x4 (&b)[NTL]) {
-#pragma unroll
-    for (int i = 0; i < MT; ++i)
-#pragma unroll
-      for (int j = 0; j < NTL; ++j) c.acc[i][j] = VhType<T>::mma(a[i], b[j], c.acc[i][j]);
+  constexpr int ABYTES = BM * 128, STAGE = (BM + BN) * 128;
+  typedef VhLoader<T, BM, AS, NT> LA;
+  typedef VhLoader<T, BN, BS, NT> LB;
+  constexpr int NDMA = LA::CH + LB::CH;
+  const int tid = threadIdx.x;
+  LA la;
+  LB lb;
+  la.init(p.A, p.lda, c.m0, p.M, p.Ka, tid);
+  lb.init(p.B, p.ldb, c.n0, p.N, p.Kb, tid);
+  VhFrags<T, BM, AS, MT> ra;
+  VhFrags<T, BN, BS, NTL> rb;
+  ra.init(c.wm0, c.lane);
+  rb.init(c.wn0, c.lane);
+  auto dma = [&](int t) {
+    char* const buf = lds + ((t - t0) & 1) * STAGE;
+    la.dma(t, buf, c.wave, tid);
+    lb.dma(t, buf + ABYTES, c.wave, tid);
   };
 #pragma unroll
   for (int i = 0; i < MT; ++i)
 #pragma unroll
     for (int j = 0; j < NTL; ++j) c.acc[i][j] = (f32x4){0.f, 0.f, 0.f, 0.f};
+  if (t0 >= t1) return;
+  u32x4 fb[2][NTL];
 
+  if constexpr (sizeof(T) == 2 && (AS || BS)) {
+    static_assert(AS && MT % 2 == 0 && (!BS || NTL % 2 == 0), "slow products: dh (A) and dw (A and B)");
+    dma(t0);
+#pragma unroll 1
+    for (int t = t0; t < t1; ++t) {
+      const char* buf = lds + ((t - t0) & 1) * STAGE;
+      vh_wait<0>();
+      vh_barrier();
+      if constexpr (!BS) rb.read(fb[0], buf + ABYTES, 0);
+      if (t + 1 < t1) dma(t + 1);
 #pragma unroll
-  for (int d = 0; d < D; ++d)
-    if (d < T_) dma(d, d);
-  if (T_ >= D) vh_wait<(D - 2) * NDMA>();
-  else vh_wait<0>();
-  vh_barrier();
-  frags(fa[0], fb[0], 0);
-  vh_wait<63>();
-  vh_barrier();
-  int buf = 0;
-  // steady: tiles t + 1 and t + D exist
-  auto phase = [&](auto steady, int t, u32x4 (&a)[MT], u32x4 (&b)[NTL], u32x4 (&na)[MT], u32x4 (&nb)[NTL]) {
-    constexpr bool kSteady = decltype(steady)::value;
-    const bool more = kSteady || t + D < T_;
-    if (more) dma(t + D, buf);
-    buf = buf + 1 == D ? 0 : buf + 1;
-    if (kSteady || t + 1 < T_) frags(na, nb, buf);
-    mma(a, b);
-    if (kSteady) {
-      vh_wait<(D - 2) * NDMA>();
+      for (int h = 0; h < 2; ++h) {
+        if constexpr (BS) {
+#pragma unroll
+          for (int j = 0; j < NTL; j += 2) rb.read_tr2(fb[h][j], fb[h][j + 1], buf + ABYTES, h, j);
+        } else if (h == 0) {
+          rb.read(fb[1], buf + ABYTES, 1);
+        }
+#pragma unroll
+        for (int i = 0; i < MT; i += 2) {
+          u32x4 a0, a1;
+          ra.read_tr2(a0, a1, buf, h, i);
+#pragma unroll
+          for (int j = 0; j < NTL; ++j) c.acc[i][j] = VhType<T>::mma(a0, fb[h][j], c.acc[i][j]);
+#pragma unroll
+          for (int j = 0; j < NTL; ++j) c.acc[i + 1][j] = VhType<T>::mma(a1, fb[h][j], c.acc[i + 1][j]);
+        }
+      }
+    }
+  } else {
+    u32x4 fa[2][MT];
+    auto frags = [&](int x, int t, int half) {
+      const char* buf = lds + ((t - t0) & 1) * STAGE;
+      ra.read(fa[x], buf, half);
+      rb.read(fb[x], buf + ABYTES, half);
+    };
+    auto mma = [&](int x) {
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < NTL; ++j) c.acc[i][j] = VhType<T>::mma(fa[x][i], fb[x][j], c.acc[i][j]);
+    };
+    // the schedule of a half: the DMAs one MFMA apart, then the fragment reads spread over the others
+    constexpr int R = (AS ? 4 * MT : MT) + (BS ? 4 * NTL : NTL), X = MT * NTL * (sizeof(T) == 2 ? 1 : 4);
+    constexpr int PER = (X - NDMA) / R > 0 ? (X - NDMA) / R : 1;
+    auto spread = [&](bool dmas) {
+      if (dmas) {
+#pragma unroll
+        for (int i = 0; i < NDMA; ++i) {
+          __builtin_amdgcn_sched_group_barrier(0x010, 1, 0);
+          __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < R; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x008, PER, 0);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    dma(t0);
+    if (t0 + 1 < t1) {
+      dma(t0 + 1);
+      vh_wait<NDMA>();
     } else {
-      vh_wait<63>();                      // the LDS reads, on every path
-      if (!more) vh_wait<0>();
-      else vh_wait<(D - 2) * NDMA>();
+      vh_wait<0>();
     }
     vh_barrier();
-  };
-  int t = 0;
+    frags(0, t0, 0);
+    vh_wait<63>();
+    int t = t0;
 #pragma unroll 1
-  for (; t + 1 + D < T_; t += 2) {
-    phase(VhTrue{}, t, fa[0], fb[0], fa[1], fb[1]);
-    phase(VhTrue{}, t + 1, fa[1], fb[1], fa[0], fb[0]);
-  }
+    for (; t + 2 < t1; ++t) {
+      frags(1, t, 1);
+      mma(0);
+      spread(false);
+      vh_wait<0>();
+      vh_barrier();
+      dma(t + 2);
+      frags(0, t + 1, 0);
+      mma(1);
+      spread(true);
+      vh_wait<63>();
+    }
 #pragma unroll 1
-  for (; t < T_; t += 2) {
-    phase(VhFalse{}, t, fa[0], fb[0], fa[1], fb[1]);
-    if (t + 1 < T_) phase(VhFalse{}, t + 1, fa[1], fb[1], fa[0], fb[0]);
+    for (; t < t1; ++t) {
+      frags(1, t, 1);
+      mma(0);
+      vh_wait<0>();
+      vh_barrier();
+      frags(0, t + 1 < t1 ? t + 1 : t, 0);      // (behind the last tile: read, not used)
+      mma(1);
+      vh_wait<63>();
+    }
   }
+  vh_wait<0>();
+  vh_barrier();
 }
 
-template <typename T, int BM, int BN, int NWM, int NWN, int D, class Epi>
+template <typename T, int BM, int BN, int NWM, int NWN, bool AS, bool BS, class Epi>
 __global__ __launch_bounds__(NWM * NWN * 64, 1) void vh_gemm(VhOperands p, Epi e) {
   typedef VhTile<T, BM, BN, NWM, NWN> Tile;
-  __shared__ __attribute__((aligned(16))) char lds[D * (BM + BN) * 64];
+  __shared__ __attribute__((aligned(16))) char lds[2 * (BM + BN) * 128];
   Tile c;
   c.lane = threadIdx.x & 63;
   c.wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   c.wm0 = (c.wave / NWN) * Tile::WM;
   c.wn0 = (c.wave % NWN) * Tile::WN;
+  const int tiles = p.tiles_m * p.tiles_n;
   int tx, ty;
-  xcd_tile_linear(blockIdx.x, p.tiles_m, p.tiles_n, tx, ty);
+  xcd_tile_linear(blockIdx.x % tiles, p.tiles_m, p.tiles_n, tx, ty);
+  c.split = blockIdx.x / tiles;
   c.m0 = tx * BM;
   c.n0 = ty * BN;
-  vh_mainloop<T, BM, BN, NWM, NWN, D>(p, c, lds);
+  const int per = (p.ktiles + p.splits - 1) / p.splits, t0 = c.split * per;
+  vh_mainloop<T, BM, BN, NWM, NWN, AS, BS>(p, c, lds, t0, min(p.ktiles, t0 + per));
   e.template run<T, BM, BN, NWM, NWN>(p, c, tx, ty, lds);
 }
 
@@ -215,6 +351,11 @@ __device__ __forceinline__ f32x4 vh_bias4(const float* bias, int m, int M) {
   for (int r = 0; r < 4; ++r) b[r] = m + r < M ? b[r] : -INFINITY;
   return b;
 }
+
+// Place of class k (0 .. 31) among the 32 of its group in a row of d: bf16 products read d with contiguous k next to a slow
+// operand whose transposed reads deliver k = 4 g .. 4 g + 3 and 16 + 4 g .. + 3 to lane group g, so those eight lie together.
+__device__ __forceinline__ int vh_place(int k) { return (k & ~31) | ((k & 12) << 1) | ((k & 16) >> 2) | (k & 3); }
+__device__ __forceinline__ int vh_class(int at) { return (at & ~31) | ((at & 24) >> 1) | ((at & 4) << 2) | (at & 3); }
 
 // (a.m, a.s) stands for a.s * exp2(a.m): the sum of exponentials relative to the largest.  An empty sum is (-inf, 0).
 struct MaxSum {
@@ -283,8 +424,8 @@ struct VhForward {
   }
 };
 
-// Backward, first product: i = class (relative to the piece), j = row.  d[row][class] in the operand type, columns up to
-// ldd (a multiple of the K tile) written as zeros; dbias partial sums per row tile from the values before rounding.
+// Backward, first product: i = class (relative to the piece), j = row.  d[row][vh_place(class)] in the operand
+// type, places up to ldd (a multiple of the K tile) written as zeros; dbias partial sums per row tile from the values before rounding.
 struct VhGradLogits {
   const float* bias;        // of the piece
   const int* labels;
@@ -331,7 +472,7 @@ struct VhGradLogits {
         if (live && m < ldd) {
           typedef __attribute__((ext_vector_type(4))) T T4;
           const T4 o = {(T)v[0], (T)v[1], (T)v[2], (T)v[3]};
-          *reinterpret_cast<T4*>((T*)d + (long)row * ldd + m) = o;
+          *reinterpret_cast<T4*>((T*)d + (long)row * ldd + (sizeof(T) == 2 ? vh_place(m) : m)) = o;
         }
       }
     }
@@ -356,13 +497,16 @@ struct VhGradLogits {
   }
 };
 
-// Plain product: out[j][i] in type O; acc: fp32 [N][M] running sum over the pieces of the classes (read unless `first`,
-// written unless `last`, in which case the result goes to out).
+// Plain product: out[j][i], j < rows, in the operand type or fp32; the product's j is a place of d where by_place is set
+// (its N is then the number of places).  With sum: fp32 [split][rows][M] running sums over the pieces of the classes, read unless `first` and written unless `last` (a single split:
+// the last piece's result goes to out).
 struct VhStore {
   void* out;
   long ldo;
-  int out_f32;              // out holds fp32, else the operand type
-  float* sum;               // nullptr: a single piece
+  int out_f32;
+  int by_place;
+  int rows;
+  float* sum;
   int first, last;
   template <typename T, int BM, int BN, int NWM, int NWN, class Tile>
   __device__ void run(const VhOperands& p, Tile& c, int, int, char*) const {
@@ -371,28 +515,31 @@ struct VhStore {
     const bool vec = !(p.M & 3);
 #pragma unroll
     for (int j = 0; j < NTL; ++j) {
-      const int row = c.n0 + c.wn0 + 16 * j + i16;
-      if (row >= p.N) continue;
+      int row = c.n0 + c.wn0 + 16 * j + i16;
+      if (sizeof(T) == 2 && by_place) row = vh_class(row);
+      if (row >= rows) continue;
 #pragma unroll
       for (int i = 0; i < MT; ++i) {
         const int m = c.m0 + c.wm0 + 16 * i + 4 * g;
         if (m >= p.M) continue;
         f32x4 v = c.acc[i][j];
         const int left = p.M - m;
-        float* s = sum ? sum + (long)row * p.M + m : nullptr;
-        if (s && !first) {
-          if (vec) v += *reinterpret_cast<const f32x4*>(s);
-          else
+        if (sum) {
+          float* s = sum + ((long)c.split * rows + row) * p.M + m;
+          if (!first) {
+            if (vec) v += *reinterpret_cast<const f32x4*>(s);
+            else
 #pragma unroll
-            for (int r = 0; r < 4; ++r) v[r] += r < left ? s[r] : 0.f;
-        }
-        if (s && !last) {
-          if (vec) *reinterpret_cast<f32x4*>(s) = v;
-          else
+              for (int r = 0; r < 4; ++r) v[r] += r < left ? s[r] : 0.f;
+          }
+          if (!last) {
+            if (vec) *reinterpret_cast<f32x4*>(s) = v;
+            else
 #pragma unroll
-            for (int r = 0; r < 4; ++r)
-              if (r < left) s[r] = v[r];
-          continue;
+              for (int r = 0; r < 4; ++r)
+                if (r < left) s[r] = v[r];
+            continue;
+          }
         }
         if (out_f32 || sizeof(T) == 4) {
           float* o = (float*)out + (long)row * ldo + m;
@@ -451,36 +598,55 @@ __global__ __launch_bounds__(256) void vh_dbias(const float* __restrict__ part, 
   db[v] = s;
 }
 
-// dst[c][r] = src[r][c] for r < R, c < C; columns R .. ldd - 1 of dst are zero.  Rows of src for which live(r) is false
-// count as zero (labels given: the ignored ones -- whatever lies there, 0 * NaN must not reach a gradient).
-// 64 x 64 tiles through LDS.
-template <typename T>
-__global__ __launch_bounds__(256) void vh_transpose(const T* __restrict__ src, long lds_, int R, int C, T* __restrict__ dst, long ldd,
-                                                    const int* __restrict__ labels, int ignore) {
-  __shared__ T tile[64][64 + 4 / sizeof(T) * 2];
-  const int nr = (int)((ldd + 63) >> 6);
-  const int r0 = (blockIdx.x % nr) * 64, c0 = (blockIdx.x / nr) * 64, x = threadIdx.x & 63, y = threadIdx.x >> 6;
-  for (int i = y; i < 64; i += 4) {
-    const int r = r0 + i, c = c0 + x;
-    T v = (T)0.f;
-    if (r < R && c < C && !(labels && labels[r] == ignore)) v = src[(long)r * lds_ + c];
-    tile[i][x] = v;
-  }
-  __syncthreads();
-  for (int i = y; i < 64; i += 4) {
-    const int c = c0 + i, r = r0 + x;
-    if (c < C && r < ldd) dst[(long)c * ldd + r] = tile[x][i];
+// dst[r][c] = src[r][c] with rows ldd apart (16-byte multiples), columns C .. ldd - 1 zero.  labels given: the rows of
+// ignored labels are zero as well -- whatever lies there, 0 * NaN must not reach a gradient.  V elements per access.
+template <typename T, int V>
+__global__ __launch_bounds__(256) void vh_copy(const T* __restrict__ src, long lds_, int R, int C, T* __restrict__ dst, long ldd,
+                                               const int* __restrict__ labels, int ignore) {
+  typedef __attribute__((ext_vector_type(V))) T vec;
+  const int per = (int)(ldd / V);
+  for (int r = blockIdx.y; r < R; r += gridDim.y) {
+    const bool keep = !(labels && labels[r] == ignore);
+    for (int i = blockIdx.x * 256 + threadIdx.x; i < per; i += gridDim.x * 256) {
+      vec v;
+#pragma unroll
+      for (int e = 0; e < V; ++e) v[e] = (T)0.f;
+      if (keep) {
+        if constexpr (V == 1) {
+          if (i < C) v[0] = src[r * lds_ + i];
+        } else {
+          v = *reinterpret_cast<const vec*>(src + r * lds_ + (long)i * V);      // (C is a multiple of V)
+        }
+      }
+      *reinterpret_cast<vec*>(dst + r * ldd + (long)i * V) = v;
+    }
   }
 }
 
-// dst[r][c] = src[r][c] with rows ldd apart, columns C .. ldd - 1 zero: a copy whose rows start on 16 bytes
-template <typename T>
-__global__ __launch_bounds__(256) void vh_pad(const T* __restrict__ src, long lds_, int R, int C, T* __restrict__ dst, long ldd) {
-  const long n = (long)R * ldd;
-  for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long)gridDim.x * 256) {
-    const long r = i / ldd;
-    const int c = (int)(i - r * ldd);
-    dst[i] = c < C ? src[r * lds_ + c] : (T)0.f;
+// out[i] = sum of the splits' slabs, in order
+template <typename O>
+__global__ __launch_bounds__(256) void vh_sum(const float* __restrict__ part, long n, int splits, O* __restrict__ out) {
+  const long i = ((long)blockIdx.x * 256 + threadIdx.x) * 4;
+  if (i >= n) return;
+  if (!(n & 3)) {
+    f32x4 s = *reinterpret_cast<const f32x4*>(part + i);
+    int k = 1;
+    for (; k + 4 <= splits; k += 4) {
+      f32x4 v[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) v[u] = *reinterpret_cast<const f32x4*>(part + (k + u) * n + i);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) s += v[u];
+    }
+    for (; k < splits; ++k) s += *reinterpret_cast<const f32x4*>(part + k * n + i);
+    typedef __attribute__((ext_vector_type(4))) O O4;
+    *reinterpret_cast<O4*>(out + i) = (O4){(O)s[0], (O)s[1], (O)s[2], (O)s[3]};
+  } else {
+    for (long j = i; j < n && j < i + 4; ++j) {
+      float s = part[j];
+      for (int k = 1; k < splits; ++k) s += part[k * n + j];
+      out[j] = (O)s;
+    }
   }
 }
 
@@ -492,68 +658,118 @@ namespace {
 
 constexpr long up(long a, long b) { return (a + b - 1) / b * b; }
 constexpr int cdiv(long a, long b) { return (int)((a + b - 1) / b); }
-constexpr int kTile = 256;            // classes per tile of the logits products: the partials are laid out by it
-constexpr long kMaxRow = 1L << 20;    // longest row of an operand: a tile's 256 rows are addressed with 32-bit byte offsets
-template <typename T> constexpr int kRows = sizeof(T) == 2 ? 256 : 128;      // rows of h per tile
+constexpr long kMaxRow = 1L << 20;    // longest row of an operand: a tile's rows are addressed with 32-bit byte offsets
+constexpr int kPiece = 256;           // pieces are multiples of this many classes
 
-template <typename T, class Epi>
-int run_gemm(VhOperands p, const Epi& e, hipStream_t s) {
-  constexpr int BM = kTile, BN = kRows<T>;
+// Tile configurations, chosen by the number of rows.
+//   kSmall: up to 64 rows -- every product streams the weight or its gradient once and is bound by memory: small tiles of the
+//           classes / hidden units, several workgroups per CU.
+//   kMid:   up to 128 rows.
+//   kLarge: 256 x 256 tiles (fp32: 256 x 128), one workgroup of eight (four) waves per CU.
+enum { kSmall, kMid, kLarge };
+int config_for(int E, long n) { return n <= 64 ? kSmall : (E == 4 || n <= 128 ? kMid : kLarge); }
+constexpr int logits_bm(int cfg) { return cfg == kSmall ? 64 : 256; }
+constexpr int rows_bn(int cfg) { return cfg == kSmall ? 64 : (cfg == kMid ? 128 : 256); }
+
+template <typename T, int BM, int BN, int NWM, int NWN, bool AS, bool BS, class Epi>
+int launch(VhOperands p, int splits, const Epi& e, hipStream_t s) {
   p.tiles_m = cdiv(p.M, BM);
   p.tiles_n = cdiv(p.N, BN);
-  hipLaunchKernelGGL((vh_gemm<T, BM, BN, 2, sizeof(T) == 2 ? 4 : 2, 4, Epi>), dim3(p.tiles_m * p.tiles_n),
-                     dim3(sizeof(T) == 2 ? 512 : 256), 0, s, p, e);
+  p.ktiles = cdiv(p.Ka > p.Kb ? p.Ka : p.Kb, 128 / sizeof(T));
+  p.splits = splits;
+  const long grid = (long)p.tiles_m * p.tiles_n * splits;
+  if (grid > 0x7fffffff) return -1;
+  hipLaunchKernelGGL((vh_gemm<T, BM, BN, NWM, NWN, AS, BS, Epi>), dim3((unsigned)grid), dim3(NWM * NWN * 64), 0, s, p, e);
   return (int)hipGetLastError();
+}
+
+// logits^T [classes][rows] = w . h^T
+template <typename T, class Epi>
+int logits(int cfg, const VhOperands& p, const Epi& e, hipStream_t s) {
+  if (cfg == kSmall) return launch<T, 64, 64, 4, 1, false, false>(p, 1, e, s);
+  if (cfg == kMid) return launch<T, 256, 128, 2, 2, false, false>(p, 1, e, s);
+  if constexpr (sizeof(T) == 2) return launch<T, 256, 256, 2, 4, false, false>(p, 1, e, s);
+  return -1;
+}
+// dh^T [hidden][rows] = w^T . d^T: the hidden units' side is slow
+template <typename T>
+int product_dh(int cfg, const VhOperands& p, int splits, const VhStore& e, hipStream_t s) {
+  if (cfg == kSmall) return launch<T, 128, 64, 4, 1, true, false>(p, splits, e, s);
+  if (cfg == kMid) return launch<T, 256, 128, 2, 2, true, false>(p, splits, e, s);
+  if constexpr (sizeof(T) == 2) return launch<T, 256, 256, 2, 4, true, false>(p, splits, e, s);
+  return -1;
+}
+// dw^T [hidden][classes] = h^T . d: both sides slow
+template <typename T>
+int product_dw(int cfg, const VhOperands& p, int splits, const VhStore& e, hipStream_t s) {
+  if (cfg == kLarge) {
+    if constexpr (sizeof(T) == 2) return launch<T, 256, 256, 2, 4, true, true>(p, splits, e, s);
+    return -1;
+  }
+  return launch<T, 256, 128, 2, 2, true, true>(p, splits, e, s);
+}
+
+// Workgroups that share a tile's K range: where the tiles alone leave CUs idle, the range is cut so that about `want`
+// workgroups run, each with at least eight K tiles; their fp32 results are added by vh_sum.
+int splits_for(long tiles, int ktiles, int want) {
+  long s = want / (tiles < 1 ? 1 : tiles);
+  if (s > ktiles / 8) s = ktiles / 8;
+  if (s > 64) s = 64;
+  if (s < 2) return 1;
+  const int per = cdiv(ktiles, s);      // no split without a K tile
+  return cdiv(ktiles, per);
 }
 
 // Layout of one call's workspace (bytes).  Everything a call needs besides its inputs and outputs.
 struct Plan {
-  long h_pad, w_pad;        // 16-byte aligned copies of h / of a piece of w (0: used as they are)
+  long h_copy, w_copy;      // aligned copies of h (backward: ignored rows zero) and of a piece of w; 0: used as they are
   long part, zlab;          // forward
-  long hT, wT, d, dT, sum, dbpart;
+  long d, sum_h, sum_w, dbpart;
   long total;
-  long ldk, ldn, ldv;       // padded hidden, rows, classes of a piece
-  int piece, pieces, row_tiles;
+  long ldk, ldv;            // padded hidden units, classes of a piece
+  int cfg, piece, pieces, row_tiles, class_tiles, splits_h, splits_w;
 };
 
 int esize(int dtype) { return dtype == 1 ? 2 : 4; }
 
-// Classes per piece: d and its transpose take piece * n values each.  2^27 values (256 MB in bf16) leave few, long pieces --
-// every piece reads and writes the fp32 sum of dh once.
+// Classes per piece: d takes piece * n values.  2^27 of them (256 MB in bf16) leave few, long pieces -- every piece reads and
+// writes the fp32 sum of dh once.
 int piece_for(long n, int classes) {
-  long v = (1L << 27) / (n < 1 ? 1 : n) / kTile * kTile;
-  if (v < 4 * kTile) v = 4 * kTile;
+  long v = (1L << 27) / (n < 1 ? 1 : n) / kPiece * kPiece;
+  if (v < 4 * kPiece) v = 4 * kPiece;
   if (v > kMaxRow) v = kMaxRow;
   return v >= classes ? classes : (int)v;
 }
 
 Plan plan_for(int dtype, int backward, long n, int H, int V, bool h_ok, bool w_ok, bool bias, int piece) {
   Plan q{};
-  const int E = esize(dtype), KE = 64 / E;
+  const int E = esize(dtype);
   long at = 0;
   auto take = [&](long bytes) {
     const long o = at;
     at += up(bytes, 256);
     return o + 1;           // 0 stands for "none"
   };
+  q.cfg = config_for(E, n);
   q.ldk = up(H, 16 / E);
-  q.ldn = up(n, KE);
-  if (!h_ok) q.h_pad = take(n * q.ldk * E);
-  q.piece = backward ? (piece > 0 ? (int)up(piece, kTile) : piece_for(n, V)) : V;
+  if (!h_ok || backward) q.h_copy = take(n * q.ldk * E);
+  q.piece = backward ? (piece > 0 ? (int)up(piece, kPiece) : piece_for(n, V)) : V;
   if (q.piece > V) q.piece = V;
   q.pieces = cdiv(V, q.piece);
-  if (!w_ok) q.w_pad = take((long)q.piece * q.ldk * E);
+  if (!w_ok) q.w_copy = take((long)q.piece * q.ldk * E);
+  q.class_tiles = cdiv(V, logits_bm(q.cfg));
+  q.row_tiles = cdiv(n, rows_bn(q.cfg));
   if (!backward) {
-    q.part = take((long)cdiv(V, kTile) * n * 8);
+    q.part = take((long)q.class_tiles * n * 8);
     q.zlab = take(n * 4);
   } else {
-    q.ldv = up(q.piece, KE);
-    q.row_tiles = cdiv(n, E == 2 ? kRows<bf16> : kRows<float>);
-    q.hT = take(H * q.ldn * E);
-    q.wT = take(H * q.ldv * E);
+    const int KT = 128 / E, want = q.cfg == kSmall ? 768 : 256;
+    q.ldv = up(q.piece, KT);
     q.d = take(n * q.ldv * E);
-    q.dT = take(q.piece * q.ldn * E);
-    if (q.pieces > 1) q.sum = take(n * H * 4);
+    q.splits_h = splits_for((long)cdiv(H, q.cfg == kSmall ? 128 : 256) * q.row_tiles, cdiv(q.ldv, KT), want);
+    q.splits_w = splits_for((long)cdiv(H, 256) * cdiv(q.piece, q.cfg == kLarge ? 256 : 128), cdiv(n, KT), 256);
+    if (q.pieces > 1 || q.splits_h > 1) q.sum_h = take(q.splits_h * n * H * 4);
+    if (q.splits_w > 1) q.sum_w = take(q.splits_w * (long)q.piece * H * 4);
     if (bias) q.dbpart = take((long)q.row_tiles * q.ldv * 4);
   }
   q.total = at ? at : 256;
@@ -566,14 +782,18 @@ T* at(void* ws, long o) { return (T*)((char*)ws + o - 1); }
 bool rows_ok(const void* p, long ld, int H, int E) { return !((uintptr_t)p & 15) && !(ld * E & 15) && !((long)H * E & 15); }
 
 template <typename T>
-int launch_transpose(const T* src, long lds, int R, int C, T* dst, long ldd, const int* labels, int ignore, hipStream_t s) {
-  hipLaunchKernelGGL(vh_transpose<T>, dim3(cdiv(C, 64) * cdiv(ldd, 64)), dim3(256), 0, s, src, lds, R, C, dst, ldd, labels, ignore);
+int launch_copy(const T* src, long lds, int R, int C, T* dst, long ldd, const int* labels, int ignore, hipStream_t s) {
+  constexpr int V = 16 / sizeof(T);
+  const bool ok = rows_ok(src, lds, C, sizeof(T));
+  const int x = cdiv(ok ? ldd / V : ldd, 256);
+  const dim3 grid(x > 64 ? 64 : x, R > 16384 ? 16384 : R);
+  if (ok) hipLaunchKernelGGL((vh_copy<T, V>), grid, dim3(256), 0, s, src, lds, R, C, dst, ldd, labels, ignore);
+  else hipLaunchKernelGGL((vh_copy<T, 1>), grid, dim3(256), 0, s, src, lds, R, C, dst, ldd, labels, ignore);
   return (int)hipGetLastError();
 }
-template <typename T>
-int launch_pad(const T* src, long lds, int R, int C, T* dst, long ldd, hipStream_t s) {
-  const long blocks = cdiv((long)R * ldd, 1024);
-  hipLaunchKernelGGL(vh_pad<T>, dim3(blocks > 8192 ? 8192 : (int)blocks), dim3(256), 0, s, src, lds, R, C, dst, ldd);
+template <typename O>
+int launch_sum(const float* part, long n, int splits, O* out, hipStream_t s) {
+  hipLaunchKernelGGL(vh_sum<O>, dim3(cdiv(n, 1024)), dim3(256), 0, s, part, n, splits, out);
   return (int)hipGetLastError();
 }
 
@@ -589,21 +809,20 @@ int forward(const void* h, long ldh, const void* w, long ldw, const float* bias,
   const int E = sizeof(T);
   const bool h_ok = rows_ok(h, ldh, H, E), w_ok = rows_ok(w, ldw, H, E);
   const Plan q = plan_for(E == 2 ? 1 : 0, 0, n, H, V, h_ok, w_ok, bias != nullptr, 0);
-  VhOperands p{w, h, ldw, ldh, V, n, H, 0, 0};
+  VhOperands p{w, h, ldw, ldh, V, n, (int)q.ldk, (int)q.ldk, 0, 0, 0, 0};
   if (!h_ok) {
-    VH_TRY(launch_pad((const T*)h, ldh, n, H, at<T>(ws, q.h_pad), q.ldk, s));
-    p.B = at<T>(ws, q.h_pad);
+    VH_TRY(launch_copy((const T*)h, ldh, n, H, at<T>(ws, q.h_copy), q.ldk, nullptr, 0, s));
+    p.B = at<T>(ws, q.h_copy);
     p.ldb = q.ldk;
   }
   if (!w_ok) {
-    VH_TRY(launch_pad((const T*)w, ldw, V, H, at<T>(ws, q.w_pad), q.ldk, s));
-    p.A = at<T>(ws, q.w_pad);
+    VH_TRY(launch_copy((const T*)w, ldw, V, H, at<T>(ws, q.w_copy), q.ldk, nullptr, 0, s));
+    p.A = at<T>(ws, q.w_copy);
     p.lda = q.ldk;
   }
-  p.K = (int)q.ldk;
   VhForward e{bias, labels, at<float2>(ws, q.part), at<float>(ws, q.zlab), n};
-  VH_TRY((run_gemm<T>(p, e, s)));
-  hipLaunchKernelGGL(vh_join, dim3(cdiv(n, 16)), dim3(256), 0, s, at<float2>(ws, q.part), (long)n, cdiv(V, kTile),
+  VH_TRY((logits<T>(q.cfg, p, e, s)));
+  hipLaunchKernelGGL(vh_join, dim3(cdiv(n, 16)), dim3(256), 0, s, at<float2>(ws, q.part), (long)n, q.class_tiles,
                      at<float>(ws, q.zlab), labels, n, V, ignore, (float*)loss, (float*)lse);
   return (int)hipGetLastError();
 }
@@ -612,43 +831,42 @@ template <typename T>
 int backward(const void* h, long ldh, const void* w, long ldw, const float* bias, const int* labels, const float* lse,
              const float* row_scale, float grad_scale, int n, int H, int V, int ignore, int piece, void* dh, void* dw, int dw_f32,
              void* db, void* ws, hipStream_t s) {
-  const int E = sizeof(T);
-  const bool h_ok = rows_ok(h, ldh, H, E), w_ok = rows_ok(w, ldw, H, E);
-  const Plan q = plan_for(E == 2 ? 1 : 0, 1, n, H, V, h_ok, w_ok, db != nullptr, piece);
-  const void* hp = h;
-  long ldhp = ldh;
-  if (!h_ok) {
-    VH_TRY(launch_pad((const T*)h, ldh, n, H, at<T>(ws, q.h_pad), q.ldk, s));
-    hp = at<T>(ws, q.h_pad);
-    ldhp = q.ldk;
-  }
-  VH_TRY(launch_transpose((const T*)h, ldh, n, H, at<T>(ws, q.hT), q.ldn, labels, ignore, s));
+  const int E = sizeof(T), KT = 128 / E;
+  const Plan q = plan_for(E == 2 ? 1 : 0, 1, n, H, V, rows_ok(h, ldh, H, E), rows_ok(w, ldw, H, E), db != nullptr, piece);
+  const T* hp = at<T>(ws, q.h_copy);
+  VH_TRY(launch_copy((const T*)h, ldh, n, H, at<T>(ws, q.h_copy), q.ldk, labels, ignore, s));
   for (int k = 0; k < q.pieces; ++k) {
     const int v0 = k * q.piece, vn = V - v0 < q.piece ? V - v0 : q.piece;
-    const long ldv = up(vn, 64 / E);
+    const long ldv = up(vn, KT);
     const T* wp = (const T*)w + (long)v0 * ldw;
-    VhOperands p{wp, hp, ldw, ldhp, vn, n, (int)q.ldk, 0, 0};
-    if (!w_ok) {
-      VH_TRY(launch_pad(wp, ldw, vn, H, at<T>(ws, q.w_pad), q.ldk, s));
-      p.A = at<T>(ws, q.w_pad);
-      p.lda = q.ldk;
+    long ldwp = ldw;
+    if (q.w_copy) {
+      VH_TRY(launch_copy(wp, ldw, vn, H, at<T>(ws, q.w_copy), q.ldk, nullptr, 0, s));
+      wp = at<T>(ws, q.w_copy);
+      ldwp = q.ldk;
     }
-    VhGradLogits e{bias ? bias + v0 : nullptr, labels, lse, row_scale, grad_scale, v0, V, ignore, at<T>(ws, q.d), ldv,
+    T* d = at<T>(ws, q.d);
+    VhGradLogits e{bias ? bias + v0 : nullptr, labels, lse, row_scale, grad_scale, v0, V, ignore, d, ldv,
                    db ? at<float>(ws, q.dbpart) : nullptr};
-    VH_TRY((run_gemm<T>(p, e, s)));
+    VH_TRY((logits<T>(q.cfg, VhOperands{wp, hp, ldwp, q.ldk, vn, n, (int)q.ldk, (int)q.ldk, 0, 0, 0, 0}, e, s)));
     if (db) {
       hipLaunchKernelGGL(vh_dbias, dim3(cdiv(vn, 256)), dim3(256), 0, s, at<float>(ws, q.dbpart), ldv, q.row_tiles, (float*)db + v0, vn);
       VH_TRY((int)hipGetLastError());
     }
     if (dw) {
-      VH_TRY(launch_transpose((const T*)at<T>(ws, q.d), ldv, n, vn, at<T>(ws, q.dT), q.ldn, nullptr, 0, s));
-      VhStore st{(char*)dw + (long)v0 * H * (dw_f32 ? 4 : E), H, dw_f32, nullptr, 1, 1};
-      VH_TRY((run_gemm<T>(VhOperands{at<T>(ws, q.hT), at<T>(ws, q.dT), q.ldn, q.ldn, H, vn, (int)q.ldn, 0, 0}, st, s)));
+      void* out = (char*)dw + (long)v0 * H * (dw_f32 ? 4 : E);
+      const bool split = q.splits_w > 1;
+      VhStore st{out, H, dw_f32, 1, vn, split ? at<float>(ws, q.sum_w) : nullptr, 1, !split};
+      VH_TRY((product_dw<T>(q.cfg, VhOperands{hp, d, q.ldk, ldv, H, (int)ldv, n, n, 0, 0, 0, 0}, q.splits_w, st, s)));
+      if (split)
+        VH_TRY(dw_f32 ? launch_sum(at<float>(ws, q.sum_w), (long)vn * H, q.splits_w, (float*)out, s)
+                      : launch_sum(at<float>(ws, q.sum_w), (long)vn * H, q.splits_w, (T*)out, s));
     }
     if (dh) {
-      VH_TRY(launch_transpose(wp, ldw, vn, H, at<T>(ws, q.wT), ldv, nullptr, 0, s));
-      VhStore st{dh, H, 0, q.sum ? at<float>(ws, q.sum) : nullptr, k == 0, k == q.pieces - 1};
-      VH_TRY((run_gemm<T>(VhOperands{at<T>(ws, q.wT), at<T>(ws, q.d), ldv, ldv, H, n, (int)ldv, 0, 0}, st, s)));
+      const bool last = k == q.pieces - 1, split = q.splits_h > 1;
+      VhStore st{dh, H, 0, 0, n, q.sum_h ? at<float>(ws, q.sum_h) : nullptr, k == 0, last && !split};
+      VH_TRY((product_dh<T>(q.cfg, VhOperands{wp, d, ldwp, ldv, H, n, vn, (int)ldv, 0, 0, 0, 0}, q.splits_h, st, s)));
+      if (last && split) VH_TRY(launch_sum(at<float>(ws, q.sum_h), (long)n * H, q.splits_h, (T*)dh, s));
     }
   }
   return 0;
