@@ -60,6 +60,15 @@ __device__ __forceinline__ void vh_barrier() {
   asm volatile("" ::: "memory");
 }
 
+// Buffer descriptor from values that are the same in every lane, said so: 64-bit address arithmetic is done on the vector
+// units, and a descriptor that comes from there is otherwise taken lane by lane in a loop around every load.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t vh_rsrc(const char* p, size_t bytes) {
+  const uint64_t a = (uint64_t)p;
+  const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)a), hi = __builtin_amdgcn_readfirstlane((uint32_t)(a >> 32));
+  const uint32_t n = __builtin_amdgcn_readfirstlane((uint32_t)(bytes < 0x7ffffff0u ? bytes : 0x7ffffff0u));
+  return make_rsrc((const void*)(((uint64_t)hi << 32) | lo), n);
+}
+
 struct VhOperands {
   // Fast operand: [rows][K], ld elements between rows, k contiguous.  Slow operand: [K][rows], ld elements between the K
   // rows, padded to 16 bytes.  Rows start on 16 bytes.  A fast operand's K is a multiple of 16 bytes.
@@ -119,7 +128,7 @@ struct VhLoader {
     if constexpr (SLOW) {
       const int left = K - t * KT;
       const size_t bytes = left > 0 ? (size_t)(left - 1) * ld + (size_t)rows * E : 0;
-      const __amdgpu_buffer_rsrc_t r = make_rsrc(base + (size_t)t * KT * ld, bytes < 0x7ffffff0u ? bytes : 0x7ffffff0u);
+      const __amdgpu_buffer_rsrc_t r = vh_rsrc(base + (size_t)t * KT * ld, bytes);
 #pragma unroll
       for (int i = 0; i < CH; ++i) {
         const int q = tid + i * NT, row = q / CPR, ch = q % CPR;
@@ -128,7 +137,7 @@ struct VhLoader {
     } else {
       const uint32_t so = (uint32_t)t << 7;
       const int n = rows < ROWS ? rows : ROWS;
-      const __amdgpu_buffer_rsrc_t r = make_rsrc(base, (size_t)(n - 1) * ld + (size_t)K * E);
+      const __amdgpu_buffer_rsrc_t r = vh_rsrc(base, (size_t)(n - 1) * ld + (size_t)K * E);
       // K may end inside the tile: zeros from there on (an offset behind every descriptor: tiles span less than 2 GB)
       const uint32_t v = (int)so + kch < K * E ? v0 : 0x80000000u;
 #pragma unroll
@@ -468,11 +477,26 @@ struct VhGradLogits {
           v[r] = dead ? 0.f : sc * (y == 16 * i + r ? e - 1.f : e);
         }
         c.acc[i][j] = v;
-        const int m = mw + 16 * i;
-        if (live && m < ldd) {
+      }
+      if (live) {
+        T* const o = (T*)d + (long)row * ldd;
+        if constexpr (sizeof(T) == 2 && MT % 2 == 0) {      // eight neighbouring places: classes 4 g .. and 16 + 4 g ..
+#pragma unroll
+          for (int i = 0; i < MT; i += 2) {
+            const int m = mw + 16 * i;
+            const f32x4 v = c.acc[i][j], x = c.acc[i + 1][j];
+            const bf16x8 y = {(T)v[0], (T)v[1], (T)v[2], (T)v[3], (T)x[0], (T)x[1], (T)x[2], (T)x[3]};
+            if (m < ldd) *reinterpret_cast<bf16x8*>(o + vh_place(m)) = y;
+          }
+        } else {
           typedef __attribute__((ext_vector_type(4))) T T4;
-          const T4 o = {(T)v[0], (T)v[1], (T)v[2], (T)v[3]};
-          *reinterpret_cast<T4*>((T*)d + (long)row * ldd + (sizeof(T) == 2 ? vh_place(m) : m)) = o;
+#pragma unroll
+          for (int i = 0; i < MT; ++i) {
+            const int m = mw + 16 * i;
+            const f32x4 v = c.acc[i][j];
+            const T4 y = {(T)v[0], (T)v[1], (T)v[2], (T)v[3]};
+            if (m < ldd) *reinterpret_cast<T4*>(o + (sizeof(T) == 2 ? vh_place(m) : m)) = y;
+          }
         }
       }
     }
@@ -508,58 +532,85 @@ struct VhStore {
   int rows;
   float* sum;
   int first, last;
-  template <typename T, int BM, int BN, int NWM, int NWN, class Tile>
-  __device__ void run(const VhOperands& p, Tile& c, int, int, char*) const {
-    constexpr int MT = Tile::MT, NTL = Tile::NTL;
-    const int i16 = c.lane & 15, g = c.lane >> 4;
-    const bool vec = !(p.M & 3);
+  // V values of a row, from the wave's staging rows to where they belong
+  template <typename T, int V>
+  __device__ __forceinline__ void put(const float* src, long row, int m, int M, int split) const {
+    float v[V];
 #pragma unroll
-    for (int j = 0; j < NTL; ++j) {
-      int row = c.n0 + c.wn0 + 16 * j + i16;
-      if (sizeof(T) == 2 && by_place) row = vh_class(row);
-      if (row >= rows) continue;
+    for (int q = 0; q < V; q += 4) {
+      const f32x4 x = *reinterpret_cast<const f32x4*>(src + q);
 #pragma unroll
-      for (int i = 0; i < MT; ++i) {
-        const int m = c.m0 + c.wm0 + 16 * i + 4 * g;
-        if (m >= p.M) continue;
-        f32x4 v = c.acc[i][j];
-        const int left = p.M - m;
-        if (sum) {
-          float* s = sum + ((long)c.split * rows + row) * p.M + m;
-          if (!first) {
-            if (vec) v += *reinterpret_cast<const f32x4*>(s);
-            else
+      for (int r = 0; r < 4; ++r) v[q + r] = x[r];
+    }
+    const bool whole = m + V <= M;
+    if (sum) {
+      float* s = sum + ((long)split * rows + row) * M + m;
+      if (!first) {
 #pragma unroll
-              for (int r = 0; r < 4; ++r) v[r] += r < left ? s[r] : 0.f;
-          }
-          if (!last) {
-            if (vec) *reinterpret_cast<f32x4*>(s) = v;
-            else
+        for (int q = 0; q < V; q += 4) {
+          if (whole) {
+            const f32x4 x = *reinterpret_cast<const f32x4_any*>(s + q);
 #pragma unroll
-              for (int r = 0; r < 4; ++r)
-                if (r < left) s[r] = v[r];
-            continue;
-          }
-        }
-        if (out_f32 || sizeof(T) == 4) {
-          float* o = (float*)out + (long)row * ldo + m;
-          if (vec) *reinterpret_cast<f32x4_any*>(o) = v;
-          else
+            for (int r = 0; r < 4; ++r) v[q + r] += x[r];
+          } else {
 #pragma unroll
             for (int r = 0; r < 4; ++r)
-              if (r < left) o[r] = v[r];
-        } else {
-          T* o = (T*)out + (long)row * ldo + m;
-          typedef __attribute__((ext_vector_type(4))) T T4;
-          typedef T4 T4_any __attribute__((aligned(2)));
-          const T4 x = {(T)v[0], (T)v[1], (T)v[2], (T)v[3]};
-          if (vec) *reinterpret_cast<T4_any*>(o) = x;
-          else
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-              if (r < left) o[r] = x[r];
+              if (m + q + r < M) v[q + r] += s[q + r];
+          }
         }
       }
+      if (!last) {
+        store<float, V>(s, v, M - m);
+        return;
+      }
+    }
+    if (out_f32 || sizeof(T) == 4) store<float, V>((float*)out + row * ldo + m, v, M - m);
+    else store<T, V>((T*)out + row * ldo + m, v, M - m);
+  }
+  template <typename O, int V>
+  static __device__ __forceinline__ void store(O* o, const float (&v)[V], int left) {
+    constexpr int W = 16 / sizeof(O) < V ? 16 / sizeof(O) : V;
+    typedef __attribute__((ext_vector_type(W))) O vec;
+    typedef vec vec_any __attribute__((aligned(sizeof(O))));
+    if (left >= V) {
+#pragma unroll
+      for (int q = 0; q < V; q += W) {
+        vec x;
+#pragma unroll
+        for (int r = 0; r < W; ++r) x[r] = (O)v[q + r];
+        *reinterpret_cast<vec_any*>(o + q) = x;
+      }
+    } else {
+#pragma unroll
+      for (int r = 0; r < V; ++r)
+        if (r < left) o[r] = (O)v[r];
+    }
+  }
+  // A lane of the product holds four values of a row, sixteen rows side by side: stores of it would touch sixteen lines for
+  // 32 or 64 bytes each.  Sixteen rows at a time go through a part of LDS of the wave's own and leave as whole runs of WM
+  // values (16 rows x 132 floats: the 16-byte writes of a column group spread over all banks).
+  template <typename T, int BM, int BN, int NWM, int NWN, class Tile>
+  __device__ void run(const VhOperands& p, Tile& c, int, int, char* lds) const {
+    constexpr int MT = Tile::MT, NTL = Tile::NTL, WM = Tile::WM, PITCH = WM + 4;
+    constexpr int V = sizeof(T) == 2 ? 8 : 4, LPR = WM / V, RPP = 64 / LPR;       // lanes per row, rows per pass
+    static_assert(NWM * NWN * 16 * PITCH * 4 <= 2 * (BM + BN) * 128, "staging rows fit in the tile buffers");
+    float* const st = reinterpret_cast<float*>(lds) + c.wave * 16 * PITCH;
+    const int i16 = c.lane & 15, g = c.lane >> 4;
+    const int rl = c.lane / LPR, cl = (c.lane % LPR) * V, m = c.m0 + c.wm0 + cl;
+#pragma unroll
+    for (int j = 0; j < NTL; ++j) {
+#pragma unroll
+      for (int i = 0; i < MT; ++i) *reinterpret_cast<f32x4*>(st + i16 * PITCH + 16 * i + 4 * g) = c.acc[i][j];
+      asm volatile("" ::: "memory");        // other lanes' values are read: LDS accesses of a wave stay in this order
+      __builtin_amdgcn_wave_barrier();
+#pragma unroll
+      for (int r = 0; r < 16; r += RPP) {
+        int row = c.n0 + c.wn0 + 16 * j + r + rl;
+        if (sizeof(T) == 2 && by_place) row = vh_class(row);
+        if (row < rows && m < p.M) put<T, V>(st + (r + rl) * PITCH + cl, row, m, p.M, c.split);
+      }
+      asm volatile("" ::: "memory");
+      __builtin_amdgcn_wave_barrier();
     }
   }
 };
@@ -664,12 +715,14 @@ constexpr int kPiece = 256;           // pieces are multiples of this many class
 // Tile configurations, chosen by the number of rows.
 //   kSmall: up to 64 rows -- every product streams the weight or its gradient once and is bound by memory: small tiles of the
 //           classes / hidden units, several workgroups per CU.
-//   kMid:   up to 128 rows.
-//   kLarge: 256 x 256 tiles (fp32: 256 x 128), one workgroup of eight (four) waves per CU.
+//   kMid:   up to 128 rows, and fp32: 128 x 128 tiles of four waves, two workgroups per CU.
+//   kLarge: 256 x 256 tiles of eight waves, one workgroup per CU.
 enum { kSmall, kMid, kLarge };
 int config_for(int E, long n) { return n <= 64 ? kSmall : (E == 4 || n <= 128 ? kMid : kLarge); }
-constexpr int logits_bm(int cfg) { return cfg == kSmall ? 64 : 256; }
+constexpr int logits_bm(int cfg) { return cfg == kSmall ? 64 : (cfg == kMid ? 128 : 256); }
 constexpr int rows_bn(int cfg) { return cfg == kSmall ? 64 : (cfg == kMid ? 128 : 256); }
+constexpr int hidden_bm(int cfg) { return cfg == kLarge ? 256 : 128; }      // of dh and dw
+constexpr int classes_bn(int cfg) { return cfg == kLarge ? 256 : 128; }     // of dw
 
 template <typename T, int BM, int BN, int NWM, int NWN, bool AS, bool BS, class Epi>
 int launch(VhOperands p, int splits, const Epi& e, hipStream_t s) {
@@ -687,7 +740,7 @@ int launch(VhOperands p, int splits, const Epi& e, hipStream_t s) {
 template <typename T, class Epi>
 int logits(int cfg, const VhOperands& p, const Epi& e, hipStream_t s) {
   if (cfg == kSmall) return launch<T, 64, 64, 4, 1, false, false>(p, 1, e, s);
-  if (cfg == kMid) return launch<T, 256, 128, 2, 2, false, false>(p, 1, e, s);
+  if (cfg == kMid) return launch<T, 128, 128, 2, 2, false, false>(p, 1, e, s);
   if constexpr (sizeof(T) == 2) return launch<T, 256, 256, 2, 4, false, false>(p, 1, e, s);
   return -1;
 }
@@ -695,7 +748,7 @@ int logits(int cfg, const VhOperands& p, const Epi& e, hipStream_t s) {
 template <typename T>
 int product_dh(int cfg, const VhOperands& p, int splits, const VhStore& e, hipStream_t s) {
   if (cfg == kSmall) return launch<T, 128, 64, 4, 1, true, false>(p, splits, e, s);
-  if (cfg == kMid) return launch<T, 256, 128, 2, 2, true, false>(p, splits, e, s);
+  if (cfg == kMid) return launch<T, 128, 128, 2, 2, true, false>(p, splits, e, s);
   if constexpr (sizeof(T) == 2) return launch<T, 256, 256, 2, 4, true, false>(p, splits, e, s);
   return -1;
 }
@@ -706,7 +759,7 @@ int product_dw(int cfg, const VhOperands& p, int splits, const VhStore& e, hipSt
     if constexpr (sizeof(T) == 2) return launch<T, 256, 256, 2, 4, true, true>(p, splits, e, s);
     return -1;
   }
-  return launch<T, 256, 128, 2, 2, true, true>(p, splits, e, s);
+  return launch<T, 128, 128, 2, 2, true, true>(p, splits, e, s);
 }
 
 // Workgroups that share a tile's K range: where the tiles alone leave CUs idle, the range is cut so that about `want`
@@ -763,11 +816,11 @@ Plan plan_for(int dtype, int backward, long n, int H, int V, bool h_ok, bool w_o
     q.part = take((long)q.class_tiles * n * 8);
     q.zlab = take(n * 4);
   } else {
-    const int KT = 128 / E, want = q.cfg == kSmall ? 768 : 256;
+    const int KT = 128 / E, want = q.cfg == kSmall ? 768 : (q.cfg == kMid ? 512 : 256);
     q.ldv = up(q.piece, KT);
     q.d = take(n * q.ldv * E);
-    q.splits_h = splits_for((long)cdiv(H, q.cfg == kSmall ? 128 : 256) * q.row_tiles, cdiv(q.ldv, KT), want);
-    q.splits_w = splits_for((long)cdiv(H, 256) * cdiv(q.piece, q.cfg == kLarge ? 256 : 128), cdiv(n, KT), 256);
+    q.splits_h = splits_for((long)cdiv(H, hidden_bm(q.cfg)) * q.row_tiles, cdiv(q.ldv, KT), want);
+    q.splits_w = splits_for((long)cdiv(H, hidden_bm(q.cfg)) * cdiv(q.piece, classes_bn(q.cfg)), cdiv(n, KT), want);
     if (q.pieces > 1 || q.splits_h > 1) q.sum_h = take(q.splits_h * n * H * 4);
     if (q.splits_w > 1) q.sum_w = take(q.splits_w * (long)q.piece * H * 4);
     if (bias) q.dbpart = take((long)q.row_tiles * q.ldv * 4);
