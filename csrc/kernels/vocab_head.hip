@@ -98,6 +98,12 @@ struct VhTile {
 //   slow: LDS rows are the K rows, ROWS elements long; the 16-element windows of a row are permuted by row.  bf16 fragments
 //         come from transposed reads, two per fragment, which give group g the k = 4 g .. 4 g + 3 and 16 + 4 g .. + 3 of the
 //         half; fp32 ones from four 4-byte reads, k = 4 g .. 4 g + 3 as in a fast operand.
+// What a slow operand's window numbers are XORed with (bf16: eight rows of a transposed read in eight windows, or two rows to
+// the 256 bytes of all banks where a row is 128 bytes; fp32: the four groups of a read).
+template <int E, int ROWB>
+__device__ __forceinline__ int vh_window_key(int row) {
+  return E == 2 ? (ROWB >= 256 ? row & 7 : (row >> 1) & 3) : (row >> 2) & 3;
+}
 template <typename T, int ROWS, bool SLOW, int NT>
 struct VhLoader {
   static constexpr int E = sizeof(T), KT = 128 / E, CH = ROWS * 8 / NT, CPR = ROWS * E / 16, ROWB = ROWS * E;
@@ -121,7 +127,7 @@ struct VhLoader {
       step = (uint32_t)(NT / 8) * (uint32_t)ld;
     }
   }
-  static __device__ __forceinline__ int key(int row) { return E == 2 ? (row & 7) << 1 : ((row >> 2) & 3) << 2; }
+  static __device__ __forceinline__ int key(int row) { return vh_window_key<E, ROWB>(row) * (E == 2 ? 2 : 4); }
   // lds: start of this operand's part of the buffer
   __device__ __forceinline__ void dma(int t, char* lds, int wave, int tid) const {
     char* const dst = lds + wave * 1024;
@@ -154,8 +160,8 @@ struct VhFrags {
   __device__ __forceinline__ void init(int r0, int lane) {
     const int i16 = lane & 15, g = lane >> 4;
     if (!SLOW) off = (r0 + i16) * 128 + ((g ^ (i16 & 7)) << 4);
-    else if (E == 2) off = (4 * g + (i16 >> 2)) * ROWB + ((((r0 >> 4) ^ ((4 * g + (i16 >> 2)) & 7))) << 5) + 8 * (i16 & 3);
-    else off = 4 * g * ROWB + (((r0 >> 4) ^ g) << 6) + 4 * i16;
+    else if (E == 2) off = (4 * g + (i16 >> 2)) * ROWB + (((r0 >> 4) ^ vh_window_key<E, ROWB>(4 * g + (i16 >> 2))) << 5) + 8 * (i16 & 3);
+    else off = 4 * g * ROWB + (((r0 >> 4) ^ vh_window_key<E, ROWB>(4 * g)) << 6) + 4 * i16;
   }
   __device__ __forceinline__ void read(u32x4 (&f)[CNT], const char* lds, int half) const {
     static_assert(!SLOW || E == 4, "bf16 slow operands are read by read_tr");
@@ -171,23 +177,44 @@ struct VhFrags {
         for (int s = 0; s < 4; ++s) f[i][s] = *reinterpret_cast<const unsigned*>(p + (off ^ (i << 6)) + s * ROWB);
     }
   }
-  // Two fragments i, i + 1 of a bf16 slow operand.  The reads and the wait for them are one block: nothing between them can
-  // use, move or reuse a register that is still being written.
-  __device__ __forceinline__ void read_tr2(u32x4& f0, u32x4& f1, const char* lds, int half, int i) const {
+  // Fragments i .. i + 3 (or both of CNT == 2) of a bf16 slow operand.  The reads and the wait for them are one block: nothing
+  // between them can use, move or reuse a register that is still being written.
+  static constexpr int TR = CNT < 4 ? CNT : 4;
+  __device__ __forceinline__ void read_tr(u32x4* f, const char* lds, int half, int i) const {
     const uint32_t p = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void*)(const void*)(lds + half * 32 * ROWB);
     const uint32_t a0 = p + (off ^ (i << 5)), a1 = p + (off ^ ((i + 1) << 5));
-    u32x2 x0, x1, y0, y1;
-    asm volatile(
-        "ds_read_b64_tr_b16 %0, %4\n\t"
-        "ds_read_b64_tr_b16 %1, %4 offset:%6\n\t"
-        "ds_read_b64_tr_b16 %2, %5\n\t"
-        "ds_read_b64_tr_b16 %3, %5 offset:%6\n\t"
-        "s_waitcnt lgkmcnt(0)"
-        : "=&v"(x0), "=&v"(x1), "=&v"(y0), "=&v"(y1)
-        : "v"(a0), "v"(a1), "n"(16 * ROWB)
-        : "memory");
-    f0 = (u32x4){x0[0], x0[1], x1[0], x1[1]};
-    f1 = (u32x4){y0[0], y0[1], y1[0], y1[1]};
+    u32x2 w0, w1, x0, x1;
+    if constexpr (TR == 4) {
+      const uint32_t a2 = p + (off ^ ((i + 2) << 5)), a3 = p + (off ^ ((i + 3) << 5));
+      u32x2 y0, y1, z0, z1;
+      asm volatile(
+          "ds_read_b64_tr_b16 %0, %8\n\t"
+          "ds_read_b64_tr_b16 %1, %8 offset:%12\n\t"
+          "ds_read_b64_tr_b16 %2, %9\n\t"
+          "ds_read_b64_tr_b16 %3, %9 offset:%12\n\t"
+          "ds_read_b64_tr_b16 %4, %10\n\t"
+          "ds_read_b64_tr_b16 %5, %10 offset:%12\n\t"
+          "ds_read_b64_tr_b16 %6, %11\n\t"
+          "ds_read_b64_tr_b16 %7, %11 offset:%12\n\t"
+          "s_waitcnt lgkmcnt(0)"
+          : "=&v"(w0), "=&v"(w1), "=&v"(x0), "=&v"(x1), "=&v"(y0), "=&v"(y1), "=&v"(z0), "=&v"(z1)
+          : "v"(a0), "v"(a1), "v"(a2), "v"(a3), "n"(16 * ROWB)
+          : "memory");
+      f[2] = (u32x4){y0[0], y0[1], y1[0], y1[1]};
+      f[3] = (u32x4){z0[0], z0[1], z1[0], z1[1]};
+    } else {
+      asm volatile(
+          "ds_read_b64_tr_b16 %0, %4\n\t"
+          "ds_read_b64_tr_b16 %1, %4 offset:%6\n\t"
+          "ds_read_b64_tr_b16 %2, %5\n\t"
+          "ds_read_b64_tr_b16 %3, %5 offset:%6\n\t"
+          "s_waitcnt lgkmcnt(0)"
+          : "=&v"(w0), "=&v"(w1), "=&v"(x0), "=&v"(x1)
+          : "v"(a0), "v"(a1), "n"(16 * ROWB)
+          : "memory");
+    }
+    f[0] = (u32x4){w0[0], w0[1], w1[0], w1[1]};
+    f[1] = (u32x4){x0[0], x0[1], x1[0], x1[1]};
   }
 };
 
@@ -199,8 +226,12 @@ struct VhFrags {
 //   DMA of tile t + 2 into the buffer of tile t | read the first half of tile t + 1 | MFMAs on the second half of tile t
 // A bf16 slow operand (its fragments are read right before their MFMAs; the other wave of the SIMD covers the wait):
 //   wait until tile t has landed, barrier | DMA of tile t + 1 into the buffer of tile t - 1 | both halves of tile t
-template <typename T, int BM, int BN, int NWM, int NWN, bool AS, bool BS, class Tile>
-__device__ __forceinline__ void vh_mainloop(const VhOperands& p, Tile& c, char* lds, int t0, int t1) {
+//
+// The epilogue's inputs (labels, log-sum-exps, biases of the tile) are requested before the first operand tile and put into
+// LDS behind it, where they cost no latency at the end.
+template <typename T, int BM, int BN, int NWM, int NWN, bool AS, bool BS, class Epi, class Tile>
+__device__ __forceinline__ void vh_mainloop(const VhOperands& p, Tile& c, char* lds, int t0, int t1, const Epi& e,
+                                            typename Epi::template Inputs<BM, BN>* in) {
   constexpr int NT = Tile::NT, MT = Tile::MT, NTL = Tile::NTL;
   constexpr int ABYTES = BM * 128, STAGE = (BM + BN) * 128;
   typedef VhLoader<T, BM, AS, NT> LA;
@@ -225,11 +256,15 @@ __device__ __forceinline__ void vh_mainloop(const VhOperands& p, Tile& c, char* 
 #pragma unroll
     for (int j = 0; j < NTL; ++j) c.acc[i][j] = (f32x4){0.f, 0.f, 0.f, 0.f};
   if (t0 >= t1) return;
+  const auto early = e.template request<BM, BN, NT>(p, c.m0, c.n0, tid);
   u32x4 fb[2][NTL];
 
   if constexpr (sizeof(T) == 2 && (AS || BS)) {
-    static_assert(AS && MT % 2 == 0 && (!BS || NTL % 2 == 0), "slow products: dh (A) and dw (A and B)");
+    typedef VhFrags<T, BM, AS, MT> RA;
+    typedef VhFrags<T, BN, BS, NTL> RB;
+    static_assert(AS && MT % RA::TR == 0 && (!BS || NTL % RB::TR == 0), "slow products: dh (A) and dw (A and B)");
     dma(t0);
+    e.template keep<BM, BN, NT>(early, in, tid);
 #pragma unroll 1
     for (int t = t0; t < t1; ++t) {
       const char* buf = lds + ((t - t0) & 1) * STAGE;
@@ -241,18 +276,18 @@ __device__ __forceinline__ void vh_mainloop(const VhOperands& p, Tile& c, char* 
       for (int h = 0; h < 2; ++h) {
         if constexpr (BS) {
 #pragma unroll
-          for (int j = 0; j < NTL; j += 2) rb.read_tr2(fb[h][j], fb[h][j + 1], buf + ABYTES, h, j);
+          for (int j = 0; j < NTL; j += RB::TR) rb.read_tr(&fb[0][j], buf + ABYTES, h, j);
         } else if (h == 0) {
           rb.read(fb[1], buf + ABYTES, 1);
         }
 #pragma unroll
-        for (int i = 0; i < MT; i += 2) {
-          u32x4 a0, a1;
-          ra.read_tr2(a0, a1, buf, h, i);
+        for (int i = 0; i < MT; i += RA::TR) {
+          u32x4 a[RA::TR];
+          ra.read_tr(a, buf, h, i);
 #pragma unroll
-          for (int j = 0; j < NTL; ++j) c.acc[i][j] = VhType<T>::mma(a0, fb[h][j], c.acc[i][j]);
+          for (int k = 0; k < RA::TR; ++k)
 #pragma unroll
-          for (int j = 0; j < NTL; ++j) c.acc[i + 1][j] = VhType<T>::mma(a1, fb[h][j], c.acc[i + 1][j]);
+            for (int j = 0; j < NTL; ++j) c.acc[i + k][j] = VhType<T>::mma(a[k], fb[BS ? 0 : h][j], c.acc[i + k][j]);
         }
       }
     }
@@ -290,8 +325,10 @@ __device__ __forceinline__ void vh_mainloop(const VhOperands& p, Tile& c, char* 
     dma(t0);
     if (t0 + 1 < t1) {
       dma(t0 + 1);
+      e.template keep<BM, BN, NT>(early, in, tid);
       vh_wait<NDMA>();
     } else {
+      e.template keep<BM, BN, NT>(early, in, tid);
       vh_wait<0>();
     }
     vh_barrier();
@@ -329,7 +366,11 @@ __device__ __forceinline__ void vh_mainloop(const VhOperands& p, Tile& c, char* 
 template <typename T, int BM, int BN, int NWM, int NWN, bool AS, bool BS, class Epi>
 __global__ __launch_bounds__(NWM * NWN * 64, 1) void vh_gemm(VhOperands p, Epi e) {
   typedef VhTile<T, BM, BN, NWM, NWN> Tile;
-  __shared__ __attribute__((aligned(16))) char lds[2 * (BM + BN) * 128];
+  // one LDS object: with two of them the compiler orders every fragment read behind all LDS-DMAs in flight (s_waitcnt
+  // vmcnt(0) in the middle of the loop, forward 15 % slower)
+  typedef typename Epi::template Inputs<BM, BN> Inputs;
+  __shared__ __attribute__((aligned(16))) char lds[2 * (BM + BN) * 128 + sizeof(Inputs)];
+  Inputs& in = *reinterpret_cast<Inputs*>(lds + 2 * (BM + BN) * 128);
   Tile c;
   c.lane = threadIdx.x & 63;
   c.wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -342,23 +383,60 @@ __global__ __launch_bounds__(NWM * NWN * 64, 1) void vh_gemm(VhOperands p, Epi e
   c.m0 = tx * BM;
   c.n0 = ty * BN;
   const int per = (p.ktiles + p.splits - 1) / p.splits, t0 = c.split * per;
-  vh_mainloop<T, BM, BN, NWM, NWN, AS, BS>(p, c, lds, t0, min(p.ktiles, t0 + per));
-  e.template run<T, BM, BN, NWM, NWN>(p, c, tx, ty, lds);
+  vh_mainloop<T, BM, BN, NWM, NWN, AS, BS>(p, c, lds, t0, min(p.ktiles, t0 + per), e, &in);
+  e.template run<T, BM, BN, NWM, NWN>(p, c, tx, ty, lds, in);
 }
 
 // ---- epilogues ------------------------------------------------------------------------------------------------------
-// Logits of a lane's four consecutive classes: bias added, classes beyond the last one -inf.
-__device__ __forceinline__ f32x4 vh_bias4(const float* bias, int m, int M) {
-  f32x4 b = {0.f, 0.f, 0.f, 0.f};
-  if (bias) {
-    if (m + 4 <= M) b = *reinterpret_cast<const f32x4_any*>(bias + m);
-    else
+// Inputs of the logits' epilogues, per row and per class of the tile
+struct VhRowInputs {
+  int label;          // relative to the tile's first class; never a class of the tile where the row has none there
+  float l2, sc;       // base-2 log-sum-exp and upstream gradient (backward)
+};
+template <int BM, int BN>
+struct VhLogitsInputs {
+  VhRowInputs row[BN];
+  float bias[BM];     // -inf for classes beyond the last one
+};
+template <int BM, int BN, int NT>
+struct VhEarly {
+  VhRowInputs row[(BN + NT - 1) / NT];
+  float bias[(BM + NT - 1) / NT];
+};
+template <class Epi, int BM, int BN, int NT>
+__device__ __forceinline__ VhEarly<BM, BN, NT> vh_request(const Epi& e, const VhOperands& p, int m0, int n0, int tid) {
+  VhEarly<BM, BN, NT> x;
 #pragma unroll
-      for (int r = 0; r < 4; ++r) b[r] = m + r < M ? bias[m + r] : 0.f;
+  for (int k = 0; k < (BN + NT - 1) / NT; ++k) {
+    const int j = tid + k * NT;
+    x.row[k] = j < BN && n0 + j < p.N ? e.row_inputs(n0 + j, m0) : VhRowInputs{-1, 0.f, 0.f};
   }
 #pragma unroll
-  for (int r = 0; r < 4; ++r) b[r] = m + r < M ? b[r] : -INFINITY;
-  return b;
+  for (int k = 0; k < (BM + NT - 1) / NT; ++k) {
+    const int i = tid + k * NT;
+    x.bias[k] = i < BM && m0 + i < p.M ? (e.bias ? e.bias[m0 + i] : 0.f) : -INFINITY;
+  }
+  return x;
+}
+template <int BM, int BN, int NT>
+__device__ __forceinline__ void vh_keep(const VhEarly<BM, BN, NT>& x, VhLogitsInputs<BM, BN>* in, int tid) {
+#pragma unroll
+  for (int k = 0; k < (BN + NT - 1) / NT; ++k)
+    if (tid + k * NT < BN) in->row[tid + k * NT] = x.row[k];
+#pragma unroll
+  for (int k = 0; k < (BM + NT - 1) / NT; ++k)
+    if (tid + k * NT < BM) in->bias[tid + k * NT] = x.bias[k];
+}
+// acc += bias, and -inf beyond the last class; nothing to do inside a product without a bias
+template <class Tile, int BM, int BN>
+__device__ __forceinline__ void vh_add_bias(Tile& c, const VhLogitsInputs<BM, BN>& in, bool any, int M) {
+  if (!any && c.m0 + BM <= M) return;
+#pragma unroll
+  for (int i = 0; i < Tile::MT; ++i) {
+    const f32x4 b = *reinterpret_cast<const f32x4*>(&in.bias[c.wm0 + 16 * i + 4 * (c.lane >> 4)]);
+#pragma unroll
+    for (int j = 0; j < Tile::NTL; ++j) c.acc[i][j] += b;
+  }
 }
 
 // Place of class k (0 .. 31) among the 32 of its group in a row of d: bf16 products read d with contiguous k next to a slow
@@ -383,28 +461,35 @@ struct VhForward {
   float2* part;
   float* zlab;
   long ldpart;
+  template <int BM, int BN> using Inputs = VhLogitsInputs<BM, BN>;
+  __device__ __forceinline__ VhRowInputs row_inputs(int row, int m0) const {
+    const int y = labels[row];
+    return {y < 0 ? -1 : y - m0, 0.f, 0.f};
+  }
+  template <int BM, int BN, int NT>
+  __device__ __forceinline__ VhEarly<BM, BN, NT> request(const VhOperands& p, int m0, int n0, int tid) const {
+    return vh_request<VhForward, BM, BN, NT>(*this, p, m0, n0, tid);
+  }
+  template <int BM, int BN, int NT>
+  __device__ __forceinline__ void keep(const VhEarly<BM, BN, NT>& x, VhLogitsInputs<BM, BN>* in, int tid) const {
+    vh_keep<BM, BN, NT>(x, in, tid);
+  }
   template <typename T, int BM, int BN, int NWM, int NWN, class Tile>
-  __device__ void run(const VhOperands& p, Tile& c, int tx, int, char* lds) const {
+  __device__ __forceinline__ void run(const VhOperands& p, Tile& c, int tx, int, char* lds, const Inputs<BM, BN>& in) const {
     constexpr int MT = Tile::MT, NTL = Tile::NTL;
     const int i16 = c.lane & 15, g = c.lane >> 4;
-    const int mw = c.m0 + c.wm0 + 4 * g;
     MaxSum (*red)[BN] = reinterpret_cast<MaxSum(*)[BN]>(lds);
-#pragma unroll
-    for (int i = 0; i < MT; ++i) {
-      const f32x4 b = vh_bias4(bias, mw + 16 * i, p.M);
-#pragma unroll
-      for (int j = 0; j < NTL; ++j) c.acc[i][j] += b;
-    }
+    vh_add_bias(c, in, bias != nullptr, p.M);
 #pragma unroll
     for (int j = 0; j < NTL; ++j) {
-      const int row = c.n0 + c.wn0 + 16 * j + i16;
-      const int y = row < p.N ? labels[row] - mw : -1;      // label relative to this lane's first class
+      const int jl = c.wn0 + 16 * j + i16;
+      const int y = in.row[jl].label - (c.wm0 + 4 * g);      // label relative to this lane's first class
       if (__any(y >= 0 && y < Tile::WM)) {
 #pragma unroll
         for (int i = 0; i < MT; ++i)
 #pragma unroll
           for (int r = 0; r < 4; ++r)
-            if (y == 16 * i + r) zlab[row] = c.acc[i][j][r];
+            if (y == 16 * i + r) zlab[c.n0 + jl] = c.acc[i][j][r];
       }
       float m = -INFINITY;
 #pragma unroll
@@ -414,14 +499,18 @@ struct VhForward {
       m = fmaxf(m, __shfl_xor(m, 16, 64));
       m = fmaxf(m, __shfl_xor(m, 32, 64));
       const float m2 = m * kLog2e, off = m == -INFINITY ? 0.f : m2;
-      float s = 0.f;
+      float s0 = 0.f, s1 = 0.f;
 #pragma unroll
       for (int i = 0; i < MT; ++i)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) s += __builtin_amdgcn_exp2f(fmaf(c.acc[i][j][r], kLog2e, -off));
+        for (int r = 0; r < 4; r += 2) {
+          s0 += __builtin_amdgcn_exp2f(fmaf(c.acc[i][j][r], kLog2e, -off));
+          s1 += __builtin_amdgcn_exp2f(fmaf(c.acc[i][j][r + 1], kLog2e, -off));
+        }
+      float s = s0 + s1;
       s += __shfl_xor(s, 16, 64);
       s += __shfl_xor(s, 32, 64);
-      if (g == 0) red[c.wave / NWN][c.wn0 + 16 * j + i16] = {m2, s};
+      if (g == 0) red[c.wave / NWN][jl] = {m2, s};
     }
     __syncthreads();
     for (int j = threadIdx.x; j < BN; j += Tile::NT) {
@@ -445,38 +534,51 @@ struct VhGradLogits {
   void* d;
   long ldd;
   float* dbpart;            // [row tile][ldd] or nullptr
+  template <int BM, int BN> using Inputs = VhLogitsInputs<BM, BN>;
+  __device__ __forceinline__ VhRowInputs row_inputs(int row, int m0) const {
+    const int y = labels[row];
+    if (y == ignore) return {-1, 0.f, 0.f};
+    const bool known = y >= 0 && y < classes;
+    const float sc = row_scale ? grad_scale * row_scale[row] : grad_scale;
+    // (a label that is no class: the whole row says so)
+    return {known && y >= v0 ? y - v0 - m0 : -1, lse[row] * kLog2e, known ? sc : __builtin_nanf("")};
+  }
+  template <int BM, int BN, int NT>
+  __device__ __forceinline__ VhEarly<BM, BN, NT> request(const VhOperands& p, int m0, int n0, int tid) const {
+    return vh_request<VhGradLogits, BM, BN, NT>(*this, p, m0, n0, tid);
+  }
+  template <int BM, int BN, int NT>
+  __device__ __forceinline__ void keep(const VhEarly<BM, BN, NT>& x, VhLogitsInputs<BM, BN>* in, int tid) const {
+    vh_keep<BM, BN, NT>(x, in, tid);
+  }
   template <typename T, int BM, int BN, int NWM, int NWN, class Tile>
-  __device__ void run(const VhOperands& p, Tile& c, int, int ty, char* lds) const {
+  __device__ __forceinline__ void run(const VhOperands& p, Tile& c, int, int ty, char* lds, const Inputs<BM, BN>& in) const {
     constexpr int MT = Tile::MT, NTL = Tile::NTL;
     const int i16 = c.lane & 15, g = c.lane >> 4;
     const int mw = c.m0 + c.wm0 + 4 * g;
-#pragma unroll
-    for (int i = 0; i < MT; ++i) {
-      const f32x4 b = vh_bias4(bias, mw + 16 * i, p.M);
-#pragma unroll
-      for (int j = 0; j < NTL; ++j) c.acc[i][j] += b;
-    }
+    vh_add_bias(c, in, bias != nullptr, p.M);
 #pragma unroll
     for (int j = 0; j < NTL; ++j) {
-      const int row = c.n0 + c.wn0 + 16 * j + i16;
+      const int jl = c.wn0 + 16 * j + i16, row = c.n0 + jl;
       const bool live = row < p.N;
-      const int label = live ? labels[row] : ignore;
-      float sc = label == ignore ? 0.f : (row_scale ? grad_scale * row_scale[row] : grad_scale);
-      const float l2 = live ? lse[row] * kLog2e : 0.f;
-      const bool known = label >= 0 && label < classes;
-      if (label != ignore && !known) sc = __builtin_nanf("");       // a label that is no class: the whole row says so
-      const int y = known ? label - v0 - mw : -1;
-      const bool dead = label == ignore;
+      const VhRowInputs x = in.row[jl];
+      const int y = x.label - (c.wm0 + 4 * g);
+      const bool hit = y >= 0 && y < Tile::WM, dead = x.sc == 0.f;
 #pragma unroll
-      for (int i = 0; i < MT; ++i) {
-        f32x4 v;
+      for (int i = 0; i < MT; ++i)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          // (an ignored row is zero whatever its logits are)
-          const float e = __builtin_amdgcn_exp2f(fmaf(c.acc[i][j][r], kLog2e, -l2));
-          v[r] = dead ? 0.f : sc * (y == 16 * i + r ? e - 1.f : e);
-        }
-        c.acc[i][j] = v;
+        for (int r = 0; r < 4; ++r) c.acc[i][j][r] = x.sc * __builtin_amdgcn_exp2f(fmaf(c.acc[i][j][r], kLog2e, -x.l2));
+      if (__any(hit)) {
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) c.acc[i][j][r] -= y == 16 * i + r ? x.sc : 0.f;
+      }
+      if (__any(dead)) {        // an ignored row is zero whatever its logits are (0 * inf and 0 * NaN are not)
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) c.acc[i][j][r] = dead ? 0.f : c.acc[i][j][r];
       }
       if (live) {
         T* const o = (T*)d + (long)row * ldd;
@@ -589,8 +691,14 @@ struct VhStore {
   // A lane of the product holds four values of a row, sixteen rows side by side: stores of it would touch sixteen lines for
   // 32 or 64 bytes each.  Sixteen rows at a time go through a part of LDS of the wave's own and leave as whole runs of WM
   // values (16 rows x 132 floats: the 16-byte writes of a column group spread over all banks).
+  struct None {};
+  template <int BM, int BN> using Inputs = None;
+  template <int BM, int BN, int NT>
+  __device__ __forceinline__ None request(const VhOperands&, int, int, int) const { return {}; }
+  template <int BM, int BN, int NT>
+  __device__ __forceinline__ void keep(None, None*, int) const {}
   template <typename T, int BM, int BN, int NWM, int NWN, class Tile>
-  __device__ void run(const VhOperands& p, Tile& c, int, int, char* lds) const {
+  __device__ __forceinline__ void run(const VhOperands& p, Tile& c, int, int, char* lds, const None&) const {
     constexpr int MT = Tile::MT, NTL = Tile::NTL, WM = Tile::WM, PITCH = WM + 4;
     constexpr int V = sizeof(T) == 2 ? 8 : 4, LPR = WM / V, RPP = 64 / LPR;       // lanes per row, rows per pass
     static_assert(NWM * NWN * 16 * PITCH * 4 <= 2 * (BM + BN) * 128, "staging rows fit in the tile buffers");
@@ -616,24 +724,41 @@ struct VhStore {
 };
 
 // ---- small kernels --------------------------------------------------------------------------------------------------
-// lse and loss of a row from its (maximum, sum) pairs, joined in class order: 16 rows x 16 slices per workgroup.
+// lse and loss of a row from its (maximum, sum) pairs, joined in a fixed order.  One workgroup takes ROWS rows, 256 / ROWS
+// slices of the class tiles each, four pairs in flight per thread: with few rows every row gets a workgroup of its own
+// (500 class tiles, one row: 9.8 us with 16 rows per workgroup).
+template <int ROWS>
 __global__ __launch_bounds__(256) void vh_join(const float2* __restrict__ part, long ldpart, int tiles, const float* __restrict__ zlab,
                                                const int* __restrict__ labels, int n, int classes, int ignore,
                                                float* __restrict__ loss, float* __restrict__ lse) {
-  __shared__ MaxSum red[16][17];
-  const int rl = threadIdx.x & 15, sl = threadIdx.x >> 4, row = blockIdx.x * 16 + rl;
+  constexpr int SL = 256 / ROWS;
+  __shared__ MaxSum red[SL][ROWS];
+  const int rl = threadIdx.x % ROWS, sl = threadIdx.x / ROWS, row = blockIdx.x * ROWS + rl;
   MaxSum a = {-INFINITY, 0.f};
   if (row < n) {
-    const int per = (tiles + 15) / 16, t1 = min(tiles, (sl + 1) * per);
-    for (int t = sl * per; t < t1; ++t) {
-      const float2 v = part[(long)t * ldpart + row];
+    const float2* p = part + row;
+    int t = sl;
+    for (; t + 3 * SL < tiles; t += 4 * SL) {
+      float2 v[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) v[u] = p[(long)(t + u * SL) * ldpart];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) a = join(a, {v[u].x, v[u].y});
+    }
+    for (; t < tiles; t += SL) {
+      const float2 v = p[(long)t * ldpart];
       a = join(a, {v.x, v.y});
     }
   }
   red[sl][rl] = a;
   __syncthreads();
+#pragma unroll
+  for (int w = SL / 2; w > 0; w >>= 1) {
+    if (sl < w) red[sl][rl] = join(red[sl][rl], red[sl + w][rl]);
+    __syncthreads();
+  }
   if (sl || row >= n) return;
-  for (int w = 1; w < 16; ++w) a = join(a, red[w][rl]);
+  a = red[0][rl];
   const float l = kLn2 * (a.m + __builtin_amdgcn_logf(a.s));     // (the hardware's base-2 logarithm, one step of error)
   lse[row] = l;
   const int y = labels[row];
@@ -715,14 +840,16 @@ constexpr int kPiece = 256;           // pieces are multiples of this many class
 // Tile configurations, chosen by the number of rows.
 //   kSmall: up to 64 rows -- every product streams the weight or its gradient once and is bound by memory: small tiles of the
 //           classes / hidden units, several workgroups per CU.
-//   kMid:   up to 128 rows, and fp32: 128 x 128 tiles of four waves, two workgroups per CU.
+//   kMid:   up to 128 rows, and fp32: 128 x 64 tiles of four waves, three workgroups per CU (fp32, 1024 x 1024 x 10000: forward
+//           198 us with 128 x 128 tiles, whose 640 do not divide evenly over the CUs, 174 us with these; 4096 x 1024 x 16000: 969
+//           and 976).
 //   kLarge: 256 x 256 tiles of eight waves, one workgroup per CU.
 enum { kSmall, kMid, kLarge };
 int config_for(int E, long n) { return n <= 64 ? kSmall : (E == 4 || n <= 128 ? kMid : kLarge); }
 constexpr int logits_bm(int cfg) { return cfg == kSmall ? 64 : (cfg == kMid ? 128 : 256); }
-constexpr int rows_bn(int cfg) { return cfg == kSmall ? 64 : (cfg == kMid ? 128 : 256); }
+constexpr int rows_bn(int cfg) { return cfg == kSmall ? 64 : (cfg == kMid ? 64 : 256); }
 constexpr int hidden_bm(int cfg) { return cfg == kLarge ? 256 : 128; }      // of dh and dw
-constexpr int classes_bn(int cfg) { return cfg == kLarge ? 256 : 128; }     // of dw
+constexpr int classes_bn(int cfg) { return cfg == kLarge ? 256 : 64; }     // of dw
 
 template <typename T, int BM, int BN, int NWM, int NWN, bool AS, bool BS, class Epi>
 int launch(VhOperands p, int splits, const Epi& e, hipStream_t s) {
@@ -740,7 +867,7 @@ int launch(VhOperands p, int splits, const Epi& e, hipStream_t s) {
 template <typename T, class Epi>
 int logits(int cfg, const VhOperands& p, const Epi& e, hipStream_t s) {
   if (cfg == kSmall) return launch<T, 64, 64, 4, 1, false, false>(p, 1, e, s);
-  if (cfg == kMid) return launch<T, 128, 128, 2, 2, false, false>(p, 1, e, s);
+  if (cfg == kMid) return launch<T, 128, 64, 2, 2, false, false>(p, 1, e, s);
   if constexpr (sizeof(T) == 2) return launch<T, 256, 256, 2, 4, false, false>(p, 1, e, s);
   return -1;
 }
@@ -748,7 +875,7 @@ int logits(int cfg, const VhOperands& p, const Epi& e, hipStream_t s) {
 template <typename T>
 int product_dh(int cfg, const VhOperands& p, int splits, const VhStore& e, hipStream_t s) {
   if (cfg == kSmall) return launch<T, 128, 64, 4, 1, true, false>(p, splits, e, s);
-  if (cfg == kMid) return launch<T, 128, 128, 2, 2, true, false>(p, splits, e, s);
+  if (cfg == kMid) return launch<T, 128, 64, 2, 2, true, false>(p, splits, e, s);
   if constexpr (sizeof(T) == 2) return launch<T, 256, 256, 2, 4, true, false>(p, splits, e, s);
   return -1;
 }
@@ -759,7 +886,7 @@ int product_dw(int cfg, const VhOperands& p, int splits, const VhStore& e, hipSt
     if constexpr (sizeof(T) == 2) return launch<T, 256, 256, 2, 4, true, true>(p, splits, e, s);
     return -1;
   }
-  return launch<T, 128, 128, 2, 2, true, true>(p, splits, e, s);
+  return launch<T, 128, 64, 2, 2, true, true>(p, splits, e, s);
 }
 
 // Workgroups that share a tile's K range: where the tiles alone leave CUs idle, the range is cut so that about `want`
@@ -816,7 +943,7 @@ Plan plan_for(int dtype, int backward, long n, int H, int V, bool h_ok, bool w_o
     q.part = take((long)q.class_tiles * n * 8);
     q.zlab = take(n * 4);
   } else {
-    const int KT = 128 / E, want = q.cfg == kSmall ? 768 : (q.cfg == kMid ? 512 : 256);
+    const int KT = 128 / E, want = q.cfg == kSmall ? 768 : (q.cfg == kMid ? 768 : 256);
     q.ldv = up(q.piece, KT);
     q.d = take(n * q.ldv * E);
     q.splits_h = splits_for((long)cdiv(H, hidden_bm(q.cfg)) * q.row_tiles, cdiv(q.ldv, KT), want);
@@ -875,8 +1002,9 @@ int forward(const void* h, long ldh, const void* w, long ldw, const float* bias,
   }
   VhForward e{bias, labels, at<float2>(ws, q.part), at<float>(ws, q.zlab), n};
   VH_TRY((logits<T>(q.cfg, p, e, s)));
-  hipLaunchKernelGGL(vh_join, dim3(cdiv(n, 16)), dim3(256), 0, s, at<float2>(ws, q.part), (long)n, q.class_tiles,
-                     at<float>(ws, q.zlab), labels, n, V, ignore, (float*)loss, (float*)lse);
+  const int per = n >= 2048 ? 16 : 1;
+  hipLaunchKernelGGL((per == 16 ? vh_join<16> : vh_join<1>), dim3(cdiv(n, per)), dim3(256), 0, s, at<float2>(ws, q.part), (long)n,
+                     q.class_tiles, at<float>(ws, q.zlab), labels, n, V, ignore, (float*)loss, (float*)lse);
   return (int)hipGetLastError();
 }
 
