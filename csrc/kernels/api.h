@@ -176,16 +176,17 @@ int dtf_vocab_head_bwd(int dtype, const void* h, long ldh, const void* w, long l
 // ---- global norm of a list of gradient tensors and clipping by it (clip.hip); mirrored in ops/clip.py ----
 struct DtfClipSpan {
   const void* in;
-  void* out;              // may be `in`; not read by dtf_global_norm
-  long n;                 // elements
+  void* out;                  // may be `in`
+  long n;                     // elements
   long in_pitch, out_pitch;   // elements between the starts of two rows (cols != 0)
-  int cols;               // elements of a row; 0: all n elements are contiguous
-  int dtype;              // 0 fp32, 1 bf16, 2 fp16
+  int cols;                   // elements of a row; 0: all n elements are contiguous
+  int dtype;                  // 0 fp32, 1 bf16, 2 fp16
 };
-long dtf_clip_partials(int count, const DtfClipSpan* spans);
-int dtf_global_norm(int count, const DtfClipSpan* spans, void* partials, long slots, double scale, const void* hyper,
-                    void* hyper_out, int n_hyper, double limit, void* norm_out, hipStream_t s);
-int dtf_clip_by_global_norm(int count, const DtfClipSpan* spans, void* partials, long slots, double scale, double limit,
+long dtf_clip_table(int count, const DtfClipSpan* spans, void* table, long table_chunks, int* in_place);
+long dtf_clip_partials(long chunks);
+int dtf_global_norm(const void* table, long chunks, void* partials, long slots, double scale, const void* hyper, void* hyper_out,
+                    int n_hyper, double limit, void* norm_out, hipStream_t s);
+int dtf_clip_by_global_norm(const void* table, long chunks, int in_place, void* partials, long slots, double scale, double limit,
                             void* norm_out, hipStream_t s);
 // asynchronous parameter server over peer-to-peer mailboxes (ps.hip)
 int dtf_ps_blocks();

@@ -16,19 +16,23 @@
 
 namespace dtf {
 
-constexpr int kSpans = 72;          // spans per launch: the table travels as a kernel argument (4 KB limit), so a captured
-                                    // launch carries it and no upload or device table exists
 constexpr int kClipThreads = 256;
 constexpr int kClipVec = kClipThreads * 16;   // bytes one workgroup reads per load instruction
 
-struct ClipBatch {
-  DtfClipSpan s[kSpans];
-  int chunk_end[kSpans];            // running number of chunks up to and including span k
-  int count;
-  int chunks;                       // == chunk_end[count - 1]
-  int chunk_bytes;                  // of the input, a multiple of kClipVec
+// One chunk of one tensor, built on the host once per list (dtf_clip_table) and kept in device memory: a workgroup finds its
+// work with a single 64-byte load, and a call over any number of tensors is two launches.  (The list as kernel arguments, 72
+// tensors to a launch: 400 small tensors took 57 us, all of it launches.)
+struct ClipChunk {
+  const void* in;             // contiguous: of the chunk's first element; rows: of the tensor
+  void* out;
+  long lo;                    // rows: the chunk's first element
+  long in_pitch, out_pitch;   // rows: elements between two of them
+  int n;                      // elements
+  int cols;                   // elements of a row; 0: contiguous
+  int dtype;
+  int pad[3];
 };
-static_assert(sizeof(ClipBatch) + 64 <= 4096, "kernel arguments");
+static_assert(sizeof(ClipChunk) == 64, "one scalar load");
 
 // 16 bytes at any element alignment (global memory takes unaligned vector accesses; a tensor of an arena may start at
 // any element)
@@ -69,40 +73,20 @@ __device__ __forceinline__ u32x4 pack(const float (&f)[VE]) {
   return __builtin_bit_cast(u32x4, v);
 }
 
-// span and element range [lo, hi) of a chunk; chunk < batch.chunks
-struct ClipRange {
-  int k;
-  long lo, hi;
-};
-__device__ __forceinline__ ClipRange find_chunk(const ClipBatch& b, int chunk) {
-  int a = 0, z = b.count - 1;
-  while (a < z) {                    // first span whose chunk_end is beyond the chunk (uniform: scalar loads)
-    const int m = (a + z) >> 1;
-    if (b.chunk_end[m] > chunk) z = m;
-    else a = m + 1;
-  }
-  const int first = a ? b.chunk_end[a - 1] : 0;
-  const long per = b.chunk_bytes / (b.s[a].dtype == 0 ? 4 : 2);
-  const long lo = (long)(chunk - first) * per;
-  const long n = b.s[a].n;
-  return {a, lo, lo + per < n ? lo + per : n};
-}
-
-// element index -> element offset of a span with rows of `cols` elements, `pitch` apart (cols == 0: contiguous)
+// element index -> element offset of a tensor with rows of `cols` elements, `pitch` apart (cols == 0: contiguous)
 __device__ __forceinline__ long span_at(long e, int cols, long pitch) {
   if (cols == 0) return e;
   const long r = (e >> 32) ? e / cols : (long)((unsigned)e / (unsigned)cols);
   return r * pitch + (e - r * cols);
 }
 
+// Walks the 16-byte vectors of a contiguous chunk, kDeep of them in flight per thread, then its last elements.
+constexpr int kDeep = 8;
 template <typename T>
-__device__ __forceinline__ double chunk_sumsq(const DtfClipSpan& s, long lo, long hi) {
+__device__ __forceinline__ double chunk_sumsq(const ClipChunk& s) {
   constexpr int VE = 16 / sizeof(T);
   const T* p = (const T*)s.in;
   double a0 = 0.0, a1 = 0.0, a2 = 0.0, a3 = 0.0;
-  long v = lo / VE + threadIdx.x;                     // lo is a multiple of VE
-  const bool whole = s.cols == 0 || s.cols % VE == 0; // no vector of elements crosses a row
-  const long vend = whole ? hi / VE : 0;
   auto add = [&](const u32x4& x) {
     float f[VE];
     unpack(p, x, f);
@@ -114,19 +98,23 @@ __device__ __forceinline__ double chunk_sumsq(const DtfClipSpan& s, long lo, lon
       a3 = fma((double)f[i + 3], (double)f[i + 3], a3);
     }
   };
+  auto one = [&](float x) { a0 = fma((double)x, (double)x, a0); };
   if (s.cols == 0) {
-    for (; v + 3 * kClipThreads < vend; v += 4 * kClipThreads) {   // four loads in flight
-      u32x4 x[4];
+    const int vend = s.n / VE;
+    int v = threadIdx.x;
+    for (; v + (kDeep - 1) * kClipThreads < vend; v += kDeep * kClipThreads) {
+      u32x4 x[kDeep];
 #pragma unroll
-      for (int u = 0; u < 4; ++u) x[u] = load_any(p + (v + u * kClipThreads) * VE);
+      for (int u = 0; u < kDeep; ++u) x[u] = load_any(p + (v + u * kClipThreads) * VE);
 #pragma unroll
-      for (int u = 0; u < 4; ++u) add(x[u]);
+      for (int u = 0; u < kDeep; ++u) add(x[u]);
     }
-  }
-  for (; v < vend; v += kClipThreads) add(load_any(p + span_at(v * VE, s.cols, s.in_pitch)));
-  for (long e = (whole ? (hi / VE) * VE : lo) + threadIdx.x; e < hi; e += kClipThreads) {
-    const double f = (double)(float)p[span_at(e, s.cols, s.in_pitch)];
-    a0 = fma(f, f, a0);
+    for (; v < vend; v += kClipThreads) add(load_any(p + v * VE));
+    for (int e = vend * VE + threadIdx.x; e < s.n; e += kClipThreads) one((float)p[e]);
+  } else if (s.cols % VE == 0) {       // no vector crosses a row (lo is a multiple of VE)
+    for (int e = threadIdx.x * VE; e + VE <= s.n; e += kClipThreads * VE) add(load_any(p + span_at(s.lo + e, s.cols, s.in_pitch)));
+  } else {
+    for (int e = threadIdx.x; e < s.n; e += kClipThreads) one((float)p[span_at(s.lo + e, s.cols, s.in_pitch)]);
   }
   return (a0 + a1) + (a2 + a3);
 }
@@ -141,14 +129,12 @@ __device__ __forceinline__ double block_sum(double v, double* red) {
   return (red[0] + red[1]) + (red[2] + red[3]);
 }
 
-__global__ __launch_bounds__(kClipThreads) void norm_partials(ClipBatch b, double* __restrict__ part) {
+__global__ __launch_bounds__(kClipThreads) void norm_partials(const ClipChunk* __restrict__ table, int chunks, double* __restrict__ part) {
   __shared__ double red[4];
   double acc = 0.0;
-  for (int c = blockIdx.x; c < b.chunks; c += gridDim.x) {
-    const ClipRange r = find_chunk(b, c);
-    const DtfClipSpan& s = b.s[r.k];
-    acc += s.dtype == 0 ? chunk_sumsq<float>(s, r.lo, r.hi)
-                        : s.dtype == 1 ? chunk_sumsq<bf16>(s, r.lo, r.hi) : chunk_sumsq<_Float16>(s, r.lo, r.hi);
+  for (int c = blockIdx.x; c < chunks; c += gridDim.x) {
+    const ClipChunk s = table[c];
+    acc += s.dtype == 0 ? chunk_sumsq<float>(s) : s.dtype == 1 ? chunk_sumsq<bf16>(s) : chunk_sumsq<_Float16>(s);
   }
   acc = block_sum(acc, red);
   if (threadIdx.x == 0) part[blockIdx.x] = acc;
@@ -167,13 +153,10 @@ __device__ __forceinline__ float clip_factor(double norm, double scale, double l
 }
 
 template <typename T>
-__device__ __forceinline__ void chunk_scale(const DtfClipSpan& s, long lo, long hi, float f) {
+__device__ __forceinline__ void chunk_scale(const ClipChunk& s, float f) {
   constexpr int VE = 16 / sizeof(T);
   const T* p = (const T*)s.in;
   T* o = (T*)s.out;
-  const bool whole = s.cols == 0 || s.cols % VE == 0;
-  const long vend = whole ? hi / VE : 0;
-  long v = lo / VE + threadIdx.x;
   auto scaled = [&](const u32x4& x) {
     float y[VE];
     unpack(p, x, y);
@@ -182,34 +165,40 @@ __device__ __forceinline__ void chunk_scale(const DtfClipSpan& s, long lo, long 
     return pack<T, VE>(y);
   };
   if (s.cols == 0) {
-    for (; v + 3 * kClipThreads < vend; v += 4 * kClipThreads) {
-      u32x4 x[4];
+    const int vend = s.n / VE;
+    int v = threadIdx.x;
+    for (; v + (kDeep - 1) * kClipThreads < vend; v += kDeep * kClipThreads) {
+      u32x4 x[kDeep];
 #pragma unroll
-      for (int u = 0; u < 4; ++u) x[u] = load_any(p + (v + u * kClipThreads) * VE);
+      for (int u = 0; u < kDeep; ++u) x[u] = load_any(p + (v + u * kClipThreads) * VE);
 #pragma unroll
-      for (int u = 0; u < 4; ++u) store_any(o + (v + u * kClipThreads) * VE, scaled(x[u]));
+      for (int u = 0; u < kDeep; ++u) store_any(o + (v + u * kClipThreads) * VE, scaled(x[u]));
     }
+    for (; v < vend; v += kClipThreads) store_any(o + v * VE, scaled(load_any(p + v * VE)));
+    for (int e = vend * VE + threadIdx.x; e < s.n; e += kClipThreads) o[e] = (T)((float)p[e] * f);
+  } else if (s.cols % VE == 0) {
+    for (int e = threadIdx.x * VE; e + VE <= s.n; e += kClipThreads * VE)
+      store_any(o + span_at(s.lo + e, s.cols, s.out_pitch), scaled(load_any(p + span_at(s.lo + e, s.cols, s.in_pitch))));
+  } else {
+    for (int e = threadIdx.x; e < s.n; e += kClipThreads)
+      o[span_at(s.lo + e, s.cols, s.out_pitch)] = (T)((float)p[span_at(s.lo + e, s.cols, s.in_pitch)] * f);
   }
-  for (; v < vend; v += kClipThreads)
-    store_any(o + span_at(v * VE, s.cols, s.out_pitch), scaled(load_any(p + span_at(v * VE, s.cols, s.in_pitch))));
-  for (long e = (whole ? (hi / VE) * VE : lo) + threadIdx.x; e < hi; e += kClipThreads)
-    o[span_at(e, s.cols, s.out_pitch)] = (T)((float)p[span_at(e, s.cols, s.in_pitch)] * f);
 }
 
 // in_place: the outputs are the inputs, and a factor of one leaves nothing to do
-__global__ __launch_bounds__(kClipThreads) void clip_scale(ClipBatch b, const double* __restrict__ part, int np, double scale,
-                                                           double limit, int in_place, float* __restrict__ norm_out) {
+__global__ __launch_bounds__(kClipThreads) void clip_scale(const ClipChunk* __restrict__ table, int chunks,
+                                                           const double* __restrict__ part, int np, double scale, double limit,
+                                                           int in_place, float* __restrict__ norm_out) {
   __shared__ double red[4];
   const double norm = norm_of(part, np, scale, red);
   const float f = clip_factor(norm, scale, limit);
-  if (norm_out && blockIdx.x == 0 && threadIdx.x == 0) *norm_out = (float)norm;
+  if (blockIdx.x == 0 && threadIdx.x == 0) *norm_out = (float)norm;
   if (in_place && f == 1.0f) return;
-  for (int c = b.chunks - 1 - (int)blockIdx.x; c >= 0; c -= gridDim.x) {
-    const ClipRange r = find_chunk(b, c);
-    const DtfClipSpan& s = b.s[r.k];
-    if (s.dtype == 0) chunk_scale<float>(s, r.lo, r.hi, f);
-    else if (s.dtype == 1) chunk_scale<bf16>(s, r.lo, r.hi, f);
-    else chunk_scale<_Float16>(s, r.lo, r.hi, f);
+  for (int c = chunks - 1 - (int)blockIdx.x; c >= 0; c -= gridDim.x) {
+    const ClipChunk s = table[c];
+    if (s.dtype == 0) chunk_scale<float>(s, f);
+    else if (s.dtype == 1) chunk_scale<bf16>(s, f);
+    else chunk_scale<_Float16>(s, f);
   }
 }
 
@@ -231,116 +220,77 @@ __global__ __launch_bounds__(kClipThreads) void norm_finish(const double* __rest
 
 using namespace dtf;
 
-static bool span_ok(const DtfClipSpan& s, bool need_out) {
-  if (s.n < 0 || s.dtype < 0 || s.dtype > 2) return false;
-  if (s.n == 0) return true;
-  const uintptr_t align = s.dtype == 0 ? 3 : 1;
-  if (!s.in || ((uintptr_t)s.in & align)) return false;
-  if (need_out && (!s.out || ((uintptr_t)s.out & align))) return false;
-  if (s.cols < 0 || (s.cols > 0 && (s.in_pitch < s.cols || (need_out && s.out_pitch < s.cols)))) return false;
-  return true;
-}
-
-// Chunk size for all launches of one call: small totals are cut finer so that they spread over the chip.
-static int chunk_bytes_for(int count, const DtfClipSpan* sp) {
-  long bytes = 0;
-  for (int k = 0; k < count; ++k) bytes += sp[k].n * (sp[k].dtype == 0 ? 4 : 2);
-  long c = bytes / 2048 / kClipVec;         // about 2048 workgroups' worth
-  c = c < 1 ? 1 : (c > 16 ? 16 : c);
-  return (int)c * kClipVec;
-}
-
-// Walks the spans in batches of kSpans with at least one value each: fn(batch, grid).
-template <class F>
-static int for_batches(int count, const DtfClipSpan* sp, F&& fn) {
-  ClipBatch b;
-  b.chunk_bytes = chunk_bytes_for(count, sp);
-  b.count = 0;
-  b.chunks = 0;
-  auto flush = [&]() -> int {
-    if (!b.count) return 0;
-    const int rc = fn(b, b.chunks < 2048 ? b.chunks : 2048);
-    b.count = b.chunks = 0;
-    return rc;
-  };
-  for (int k = 0; k < count; ++k) {
-    if (!sp[k].n) continue;
-    const long per = b.chunk_bytes / (sp[k].dtype == 0 ? 4 : 2);
-    const long need = (sp[k].n + per - 1) / per;
-    if (need > 0x3fffffff) return -3;        // 64 TB in one tensor
-    if (b.count == kSpans || b.chunks > 0x3fffffff) {
-      const int rc = flush();
-      if (rc) return rc;
-    }
-    b.s[b.count] = sp[k];
-    b.chunks += (int)need;
-    b.chunk_end[b.count++] = b.chunks;
-  }
-  return flush();
-}
+static int clip_grid(long chunks) { return (int)(chunks < 2048 ? (chunks < 1 ? 1 : chunks) : 2048); }
 
 extern "C" {
 
-// fp64 slots of the partial-sum workspace that a call on these spans needs (at least 1); < 0: bad argument
-long dtf_clip_partials(int count, const DtfClipSpan* spans) {
+// Number of chunks of a list of tensors (< 0: bad argument).  table != NULL: 64 bytes per chunk are written there (host memory),
+// to be copied to the device; *in_place = whether every output is its input.
+long dtf_clip_table(int count, const DtfClipSpan* spans, void* table, long table_chunks, int* in_place) {
   if (count < 0 || (count && !spans)) return -3;
-  for (int k = 0; k < count; ++k)
-    if (!span_ok(spans[k], false)) return -3;
-  long slots = 0;
-  const int rc = for_batches(count, spans, [&](const ClipBatch&, int grid) { slots += grid; return 0; });
-  return rc ? rc : (slots ? slots : 1);
+  long bytes = 0;
+  int same = 1;
+  for (int k = 0; k < count; ++k) {
+    const DtfClipSpan& s = spans[k];
+    if (s.n < 0 || s.dtype < 0 || s.dtype > 2) return -3;
+    if (s.n == 0) continue;
+    const int E = s.dtype == 0 ? 4 : 2;
+    if (!s.in || ((uintptr_t)s.in & (E - 1)) || !s.out || ((uintptr_t)s.out & (E - 1))) return -3;
+    if (s.cols < 0 || (s.cols > 0 && (s.in_pitch < s.cols || s.out_pitch < s.cols || s.n % s.cols))) return -3;
+    if (s.in != s.out || (s.cols && s.in_pitch != s.out_pitch)) same = 0;
+    bytes += s.n * E;
+  }
+  if (in_place) *in_place = same;
+  // About 2048 chunks, one workgroup each; small lists are cut into 4 KB, large ones into 64 KB.
+  long per = bytes / 2048 / kClipVec;
+  per = (per < 1 ? 1 : (per > 16 ? 16 : per)) * kClipVec;
+  long chunks = 0;
+  ClipChunk* t = (ClipChunk*)table;
+  for (int k = 0; k < count; ++k) {
+    const DtfClipSpan& s = spans[k];
+    const int E = s.dtype == 0 ? 4 : 2;
+    const long step = per / E;
+    for (long lo = 0; lo < s.n; lo += step, ++chunks) {
+      if (chunks >= 0x7fffffff) return -1;
+      if (!t) continue;
+      if (chunks >= table_chunks) return -2;
+      const int n = (int)(s.n - lo < step ? s.n - lo : step);
+      const long at = s.cols ? 0 : lo * E;
+      t[chunks] = ClipChunk{(const char*)s.in + at, (char*)s.out + at, s.cols ? lo : 0, s.in_pitch, s.out_pitch, n, s.cols, s.dtype, {0, 0, 0}};
+    }
+  }
+  return chunks;
 }
 
-static int partial_sums(int count, const DtfClipSpan* spans, double* part, long slots, long* used, hipStream_t s) {
-  *used = 0;
-  return for_batches(count, spans, [&](const ClipBatch& b, int grid) {
-    if (*used + grid > slots) return -2;
-    hipLaunchKernelGGL(norm_partials, dim3(grid), dim3(kClipThreads), 0, s, b, part + *used);
-    *used += grid;
-    return (int)hipGetLastError();
-  });
+// fp64 words of a call's workspace
+long dtf_clip_partials(long chunks) { return chunks < 0 ? -3 : clip_grid(chunks); }
+
+static bool table_ok(const void* table, long chunks, const void* partials, long slots) {
+  return chunks >= 0 && chunks <= 0x7fffffff && (table || !chunks) && !((uintptr_t)table & 63) && partials && !((uintptr_t)partials & 7) &&
+         slots >= clip_grid(chunks);
 }
 
-// norm_out (fp32) = scale * norm of all spans.  With hyper / hyper_out (n_hyper floats, hyper[4] = the gradient scale, in
-// place of `scale`) also hyper_out = hyper with [4] multiplied by limit / max(norm, limit); norm_out may then be NULL.
-int dtf_global_norm(int count, const DtfClipSpan* spans, void* partials, long slots, double scale, const void* hyper,
-                    void* hyper_out, int n_hyper, double limit, void* norm_out, hipStream_t s) {
-  if (count < 0 || (count && !spans) || !partials || ((uintptr_t)partials & 7) || slots < 1) return -3;
+// norm_out (fp32) = scale * norm of the table's tensors.  With hyper / hyper_out (n_hyper floats, hyper[4] = the gradient scale,
+// in place of `scale`) also hyper_out = hyper with [4] multiplied by limit / max(norm, limit); norm_out may then be NULL.
+int dtf_global_norm(const void* table, long chunks, void* partials, long slots, double scale, const void* hyper, void* hyper_out,
+                    int n_hyper, double limit, void* norm_out, hipStream_t s) {
+  if (!table_ok(table, chunks, partials, slots)) return -3;
   if (hyper ? (!hyper_out || n_hyper < 5 || n_hyper > kClipThreads || !(limit > 0.0)) : !norm_out) return -3;
-  for (int k = 0; k < count; ++k)
-    if (!span_ok(spans[k], false)) return -3;
-  long used = 0;
-  const int rc = partial_sums(count, spans, (double*)partials, slots, &used, s);
-  if (rc) return rc;
-  hipLaunchKernelGGL(norm_finish, dim3(1), dim3(kClipThreads), 0, s, (const double*)partials, (int)used, scale,
-                     (const float*)hyper, (float*)hyper_out, n_hyper, limit, (float*)norm_out);
+  const int grid = clip_grid(chunks);
+  hipLaunchKernelGGL(norm_partials, dim3(grid), dim3(kClipThreads), 0, s, (const ClipChunk*)table, (int)chunks, (double*)partials);
+  hipLaunchKernelGGL(norm_finish, dim3(1), dim3(kClipThreads), 0, s, (const double*)partials, grid, scale, (const float*)hyper,
+                     (float*)hyper_out, n_hyper, limit, (float*)norm_out);
   return (int)hipGetLastError();
 }
 
-// out = in * scale * limit / max(norm, limit) for every span (out may be in itself), norm_out (fp32) = norm = scale * |in|
-int dtf_clip_by_global_norm(int count, const DtfClipSpan* spans, void* partials, long slots, double scale, double limit,
+// out = in * scale * limit / max(norm, limit) for every tensor of the table, norm_out (fp32) = norm = scale * |in|
+int dtf_clip_by_global_norm(const void* table, long chunks, int in_place, void* partials, long slots, double scale, double limit,
                             void* norm_out, hipStream_t s) {
-  if (count < 0 || (count && !spans) || !partials || ((uintptr_t)partials & 7) || slots < 1 || !norm_out) return -3;
-  if (!(limit > 0.0) || !(limit <= 1.7976931348623157e308)) return -3;
-  int in_place = 1;
-  for (int k = 0; k < count; ++k) {
-    if (!span_ok(spans[k], true)) return -3;
-    if (spans[k].n && (spans[k].in != spans[k].out || (spans[k].cols && spans[k].in_pitch != spans[k].out_pitch))) in_place = 0;
-  }
-  long used = 0;
-  int rc = partial_sums(count, spans, (double*)partials, slots, &used, s);
-  if (rc) return rc;
-  bool first = true;
-  rc = for_batches(count, spans, [&](const ClipBatch& b, int grid) {
-    hipLaunchKernelGGL(clip_scale, dim3(grid), dim3(kClipThreads), 0, s, b, (const double*)partials, (int)used, scale, limit,
-                       in_place, first ? (float*)norm_out : nullptr);
-    first = false;
-    return (int)hipGetLastError();
-  });
-  if (rc || !first) return rc;
-  // no values at all: the norm of nothing is zero
-  hipLaunchKernelGGL(norm_finish, dim3(1), dim3(kClipThreads), 0, s, (const double*)partials, 0, scale, (const float*)nullptr,
-                     (float*)nullptr, 0, 0.0, (float*)norm_out);
+  if (!table_ok(table, chunks, partials, slots) || !norm_out || !(limit > 0.0) || !(limit <= 1.7976931348623157e308)) return -3;
+  const int grid = clip_grid(chunks);
+  hipLaunchKernelGGL(norm_partials, dim3(grid), dim3(kClipThreads), 0, s, (const ClipChunk*)table, (int)chunks, (double*)partials);
+  hipLaunchKernelGGL(clip_scale, dim3(grid), dim3(kClipThreads), 0, s, (const ClipChunk*)table, (int)chunks, (const double*)partials, grid,
+                     scale, limit, in_place, (float*)norm_out);
   return (int)hipGetLastError();
 }
 

@@ -5,10 +5,10 @@
     grads, norm = plan.clip(clip_norm)             # g * clip_norm / max(norm, clip_norm), norm before clipping
 
 The plan is made once for tensors that stay where they are (gradient arenas, as everywhere in this package) and holds
-nothing but their addresses and shapes; each call computes the norm anew from the values that the tensors then have.
-Launches go to the current stream of the tensors' device and can be captured into a HIP graph: the table of tensors
-travels as kernel arguments, the workspace of a call comes from PyTorch's allocator on that stream, so calls on different
-streams and in different graphs share nothing.  As in TensorFlow, a norm that is not finite makes every clipped value NaN.
+nothing but a table of their addresses and shapes in device memory; each call computes the norm anew from the values that
+the tensors then have.  Launches go to the current stream of the tensors' device and can be captured into a HIP graph (the
+plan has to outlive it): the table is only read, the workspace of a call comes from PyTorch's allocator on that stream, so
+calls on different streams and in different graphs share nothing that is written.  As in TensorFlow, a norm that is not finite makes every clipped value NaN.
 Kernels: csrc/kernels/clip.hip.
 """
 from __future__ import annotations
@@ -141,14 +141,18 @@ class GlobalNormClip:
         if self.device.type != "cuda":
             raise ValueError(f"GPU tensors expected, got {self.device} (ops.reference.clip_by_global_norm runs on the CPU)")
         self.lib = native.load()
-        self._spans, self._count = spans, len(tensors)
         self._keep = ([t.detach() for t in tensors], [o.detach() for o in outs])     # the memory stays allocated
         self.out = list(outs)
-        with torch.cuda.device(self.device):
-            slots = int(self.lib.dtf_clip_partials(self._count, spans))
-        if slots < 1:
-            check(slots, "clip_partials")
-        self.slots = slots              # fp64 words of a call's workspace
+        in_place = ctypes.c_int()
+        chunks = int(self.lib.dtf_clip_table(len(tensors), spans, None, 0, ctypes.byref(in_place)))
+        check(min(chunks, 0), "clip_table")
+        host = torch.empty((max(chunks, 1), 64), dtype=torch.uint8)
+        check(min(int(self.lib.dtf_clip_table(len(tensors), spans, ptr(host), chunks, None)), 0), "clip_table")
+        self.table = host.to(self.device)                # 64 bytes per chunk, the same for every call
+        # every other stream may read the table from here on: the copy is done
+        torch.cuda.current_stream(self.device).synchronize()
+        self.chunks, self._in_place = chunks, in_place.value
+        self.slots = int(self.lib.dtf_clip_partials(chunks))    # fp64 words of a call's workspace
 
     def _call(self):
         dev = self.device
@@ -162,7 +166,7 @@ class GlobalNormClip:
         scale = _scale(scale)
         with torch.cuda.device(self.device):
             stream, part, norm = self._call()
-            check(self.lib.dtf_global_norm(self._count, self._spans, ptr(part), self.slots, scale, None, None, 0, 0.0,
+            check(self.lib.dtf_global_norm(ptr(self.table), self.chunks, ptr(part), self.slots, scale, None, None, 0, 0.0,
                                            ptr(norm), stream), "global_norm")
         return norm
 
@@ -176,18 +180,9 @@ class GlobalNormClip:
             raise ValueError(self._clip_error)
         with torch.cuda.device(self.device):
             stream, part, norm = self._call()
-            check(self.lib.dtf_clip_by_global_norm(self._count, self._spans, ptr(part), self.slots, scale, clip_norm,
-                                                   ptr(norm), stream), "clip_by_global_norm")
+            check(self.lib.dtf_clip_by_global_norm(ptr(self.table), self.chunks, self._in_place, ptr(part), self.slots, scale,
+                                                   clip_norm, ptr(norm), stream), "clip_by_global_norm")
         return self.out, norm
-
-    def norm_into_hyper(self, hyper: torch.Tensor, hyper_out: torch.Tensor, clip_norm: float, norm: torch.Tensor,
-                        partials: torch.Tensor):
-        """The engine's form (HipEngine ``clip_norm``): ``hyper_out`` becomes the update kernels' hyper-parameter vector with
-        the gradient scale hyper[4] multiplied by clip_norm / max(norm, clip_norm), norm = hyper[4] * |tensors|; the
-        update then applies the factor while it reads the gradients.  All buffers are the caller's, nothing is allocated."""
-        check(self.lib.dtf_global_norm(self._count, self._spans, ptr(partials), partials.numel(), 1.0, ptr(hyper),
-                                       ptr(hyper_out), hyper.numel(), float(clip_norm), ptr(norm),
-                                       torch.cuda.current_stream(self.device).cuda_stream), "global_norm")
 
 
 def _scale(scale: float) -> float:

@@ -146,9 +146,10 @@ _SIGS = {
     "dtf_vocab_head_bwd": [c_int, c_void_p, c_long, c_void_p, c_long, c_void_p, c_void_p, c_void_p, c_void_p, c_float, c_int, c_int,
                            c_int, c_int, c_int, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_long, c_void_p],
     # ---- global norm and clipping (csrc/kernels/clip.hip; spans: ops/clip.py ClipSpan) ----
-    "dtf_clip_partials": [c_int, c_void_p],
-    "dtf_global_norm": [c_int, c_void_p, c_void_p, c_long, c_double, c_void_p, c_void_p, c_int, c_double, c_void_p, c_void_p],
-    "dtf_clip_by_global_norm": [c_int, c_void_p, c_void_p, c_long, c_double, c_double, c_void_p, c_void_p],
+    "dtf_clip_table": [c_int, c_void_p, c_void_p, c_long, ctypes.POINTER(c_int)],
+    "dtf_clip_partials": [c_long],
+    "dtf_global_norm": [c_void_p, c_long, c_void_p, c_long, c_double, c_void_p, c_void_p, c_int, c_double, c_void_p, c_void_p],
+    "dtf_clip_by_global_norm": [c_void_p, c_long, c_int, c_void_p, c_long, c_double, c_double, c_void_p, c_void_p],
 }
 
 
@@ -223,7 +224,8 @@ def load() -> ctypes.CDLL:
         fn = getattr(lib, name)
         fn.argtypes = argtypes
         fn.restype = (c_long if name in ("dtf_p2p_bytes", "dtf_p2p2_bytes", "dtf_dp_fabric_layout", "dtf_ps_ctl_bytes",
-                                         "dtf_gemm_f32_sk_workspace_bytes", "dtf_clip_partials", "dtf_vocab_head_workspace")
+                                         "dtf_gemm_f32_sk_workspace_bytes", "dtf_clip_table", "dtf_clip_partials",
+                                         "dtf_vocab_head_workspace")
                       else c_void_p if name == "dtf_gemm_f32_sk_workspace_alloc"
                       else None if name == "dtf_gemm_f32_sk_workspace_free" else c_int)
     lib.dtf_build_flavour.restype = c_char_p

@@ -231,32 +231,48 @@ def test_refused_limits(gpu_lib):
             plan.norm(scale=bad)
 
 
-@gpu
-def test_native_entries_refuse_bad_spans(gpu_lib):
+def test_table_refuses_bad_spans():
+    """dtf_clip_table is host code: no GPU needed."""
     import ctypes
+    from distributed_tensorflow_amd.ops import native
     from distributed_tensorflow_amd.ops.clip import ClipSpan
+    lib = native.load()
+    p = 1 << 20
+
+    def chunks(**kw):
+        s = (ClipSpan * 1)(ClipSpan(**{**dict(inp=p, out=p, n=64, in_pitch=0, out_pitch=0, cols=0, dtype=0), **kw}))
+        return lib.dtf_clip_table(1, s, None, 0, None)
+
+    assert chunks() == 1 and chunks(n=0, inp=None) == 0 and chunks(n=1025) == 2 and chunks(n=1025, dtype=1) == 1
+    assert chunks(n=64, cols=8, in_pitch=9, out_pitch=8) == 1
+    for bad in (dict(inp=None), dict(out=None), dict(inp=p + 2), dict(out=p + 2), dict(inp=p + 1, dtype=1), dict(n=-1), dict(dtype=3),
+                dict(cols=8, in_pitch=7, out_pitch=8), dict(cols=8, in_pitch=8, out_pitch=7), dict(cols=-1), dict(cols=7, in_pitch=7, out_pitch=7)):
+        assert chunks(**bad) == -3, bad
+    many = (ClipSpan * 3)(*[ClipSpan(p, p, 5, 0, 0, 0, 0)] * 3)
+    room = ctypes.create_string_buffer(128)
+    assert lib.dtf_clip_table(3, many, room, 2, None) == -2 and lib.dtf_clip_table(-1, many, None, 0, None) == -3
+    assert lib.dtf_clip_partials(5) == 5 and lib.dtf_clip_partials(1 << 20) == 2048 and lib.dtf_clip_partials(-1) == -3
+
+
+@gpu
+def test_native_entries_refuse(gpu_lib):
     t = torch.zeros(64, device=DEV)
+    plan = GlobalNormClip([t])
     part = torch.zeros(64, dtype=torch.float64, device=DEV)
     p, q, s = t.data_ptr(), part.data_ptr(), torch.cuda.current_stream().cuda_stream
-
-    def span(**kw):
-        return (ClipSpan * 1)(ClipSpan(**{**dict(inp=p, out=p, n=64, in_pitch=0, out_pitch=0, cols=0, dtype=0), **kw}))
-
-    good = span()
-    assert gpu_lib.dtf_clip_partials(1, good) == 1
-    for bad in (span(inp=None), span(inp=p + 2), span(n=-1), span(dtype=3), span(cols=8, in_pitch=7), span(cols=-1)):
-        assert gpu_lib.dtf_clip_partials(1, bad) == -3
-        assert gpu_lib.dtf_global_norm(1, bad, q, 64, 1.0, None, None, 0, 0.0, p, s) == -3
-        assert gpu_lib.dtf_clip_by_global_norm(1, bad, q, 64, 1.0, 1.0, p, s) == -3
-    assert gpu_lib.dtf_clip_by_global_norm(1, span(out=None), q, 64, 1.0, 1.0, p, s) == -3
-    assert gpu_lib.dtf_clip_by_global_norm(1, good, q, 0, 1.0, 1.0, p, s) == -3
-    assert gpu_lib.dtf_clip_by_global_norm(1, good, q, 64, 1.0, 0.0, p, s) == -3
-    assert gpu_lib.dtf_clip_by_global_norm(1, good, q, 64, 1.0, 1.0, None, s) == -3
-    assert gpu_lib.dtf_global_norm(1, good, None, 64, 1.0, None, None, 0, 0.0, p, s) == -3
-    many = (ClipSpan * 200)(*[good[0]] * 200)
-    need = gpu_lib.dtf_clip_partials(200, many)
-    assert need > 64 and gpu_lib.dtf_global_norm(200, many, q, 64, 1.0, None, None, 0, 0.0, p, s) == -2   # too small a workspace
-    del ctypes
+    table = plan.table.data_ptr()
+    assert gpu_lib.dtf_global_norm(None, 1, q, 64, 1.0, None, None, 0, 0.0, p, s) == -3
+    assert gpu_lib.dtf_global_norm(table + 8, 1, q, 64, 1.0, None, None, 0, 0.0, p, s) == -3
+    assert gpu_lib.dtf_global_norm(table, -1, q, 64, 1.0, None, None, 0, 0.0, p, s) == -3
+    assert gpu_lib.dtf_global_norm(table, 1, None, 64, 1.0, None, None, 0, 0.0, p, s) == -3
+    assert gpu_lib.dtf_global_norm(table, 1, q, 0, 1.0, None, None, 0, 0.0, p, s) == -3
+    assert gpu_lib.dtf_global_norm(table, 1, q, 64, 1.0, None, None, 0, 0.0, None, s) == -3
+    assert gpu_lib.dtf_global_norm(table, 1, q, 64, 1.0, p, None, 12, 1.0, None, s) == -3
+    assert gpu_lib.dtf_global_norm(table, 1, q, 64, 1.0, p, p, 4, 1.0, None, s) == -3
+    assert gpu_lib.dtf_global_norm(table, 1, q, 64, 1.0, p, p, 12, 0.0, None, s) == -3
+    assert gpu_lib.dtf_clip_by_global_norm(table, 1, 1, q, 64, 1.0, 0.0, p, s) == -3
+    assert gpu_lib.dtf_clip_by_global_norm(table, 1, 1, q, 64, 1.0, math.inf, p, s) == -3
+    assert gpu_lib.dtf_clip_by_global_norm(table, 1, 1, q, 64, 1.0, 1.0, None, s) == -3
 
 
 # ---------------------------------------------------------------------------------------------- streams and graphs
