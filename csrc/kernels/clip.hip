@@ -10,7 +10,10 @@
 // the result is bitwise reproducible and no third launch is needed between the two passes.
 //
 // Bound by memory: the first pass reads every gradient, the second reads it again and writes it.  The second pass walks
-// the chunks in the opposite order, so that what the first one read last is found in the 256 MB memory-side cache.
+// the chunks in the opposite order and the last 192 MB of the first pass are the only ones it loads to stay, so that they are
+// found in the 256 MB memory-side cache; everything else passes by it (non-temporal).  Measured, rotating over three lists:
+// 0.72 G bf16 values 805 us with plain accesses, 785 with non-temporal stores, 719 with this (1.44 GB read twice and written
+// once: 6.0 TB/s; a copy of that size runs at 5.0); 119 MB of mixed tensors 80 -> 61 us; norm of 209 MB 41.5 -> 36.7 us.
 #include "common.hpp"
 #include "api.h"
 
@@ -41,6 +44,12 @@ __device__ __forceinline__ u32x4 load_any(const void* p) {
   const u32x4 v = *reinterpret_cast<const u32x4_any*>(p);
   return v;
 }
+// the same, not to be kept in the caches
+__device__ __forceinline__ u32x4 load_any_once(const void* p) {
+  const u32x4 v = __builtin_nontemporal_load(reinterpret_cast<const u32x4_any*>(p));
+  return v;
+}
+__device__ __forceinline__ void store_any_once(void* p, u32x4 v) { __builtin_nontemporal_store(v, reinterpret_cast<u32x4_any*>(p)); }
 __device__ __forceinline__ void store_any(void* p, u32x4 v) { *reinterpret_cast<u32x4_any*>(p) = v; }
 
 __device__ __forceinline__ void unpack(const float*, const u32x4& v, float (&f)[4]) {
@@ -80,9 +89,11 @@ __device__ __forceinline__ long span_at(long e, int cols, long pitch) {
   return r * pitch + (e - r * cols);
 }
 
-// Walks the 16-byte vectors of a contiguous chunk, kDeep of them in flight per thread, then its last elements.
-constexpr int kDeep = 8;
-template <typename T>
+// Walks the 16-byte vectors of a contiguous chunk, kDeep of them in flight per thread, then its last elements.  (Two to eight
+// are within 2 % for large lists; four is best for those of 10 to 100 MB, where eight leave chunks to the one-vector loop.)
+constexpr int kDeep = 4;
+constexpr int kKeepChunks = 3072;     // of 64 KB: 192 MB (smaller chunks belong to lists that fit the cache altogether)
+template <typename T, bool PASS_BY>
 __device__ __forceinline__ double chunk_sumsq(const ClipChunk& s) {
   constexpr int VE = 16 / sizeof(T);
   const T* p = (const T*)s.in;
@@ -105,7 +116,10 @@ __device__ __forceinline__ double chunk_sumsq(const ClipChunk& s) {
     for (; v + (kDeep - 1) * kClipThreads < vend; v += kDeep * kClipThreads) {
       u32x4 x[kDeep];
 #pragma unroll
-      for (int u = 0; u < kDeep; ++u) x[u] = load_any(p + (v + u * kClipThreads) * VE);
+      for (int u = 0; u < kDeep; ++u) {
+        const T* q = p + (v + u * kClipThreads) * VE;
+        x[u] = PASS_BY ? load_any_once(q) : load_any(q);
+      }
 #pragma unroll
       for (int u = 0; u < kDeep; ++u) add(x[u]);
     }
@@ -129,12 +143,16 @@ __device__ __forceinline__ double block_sum(double v, double* red) {
   return (red[0] + red[1]) + (red[2] + red[3]);
 }
 
-__global__ __launch_bounds__(kClipThreads) void norm_partials(const ClipChunk* __restrict__ table, int chunks, double* __restrict__ part) {
+__global__ __launch_bounds__(kClipThreads) void norm_partials(const ClipChunk* __restrict__ table, int chunks, int keep,
+                                                              double* __restrict__ part) {
   __shared__ double red[4];
   double acc = 0.0;
   for (int c = blockIdx.x; c < chunks; c += gridDim.x) {
     const ClipChunk s = table[c];
-    acc += s.dtype == 0 ? chunk_sumsq<float>(s) : s.dtype == 1 ? chunk_sumsq<bf16>(s) : chunk_sumsq<_Float16>(s);
+    if (c < chunks - keep)
+      acc += s.dtype == 0 ? chunk_sumsq<float, true>(s) : s.dtype == 1 ? chunk_sumsq<bf16, true>(s) : chunk_sumsq<_Float16, true>(s);
+    else
+      acc += s.dtype == 0 ? chunk_sumsq<float, false>(s) : s.dtype == 1 ? chunk_sumsq<bf16, false>(s) : chunk_sumsq<_Float16, false>(s);
   }
   acc = block_sum(acc, red);
   if (threadIdx.x == 0) part[blockIdx.x] = acc;
@@ -170,9 +188,9 @@ __device__ __forceinline__ void chunk_scale(const ClipChunk& s, float f) {
     for (; v + (kDeep - 1) * kClipThreads < vend; v += kDeep * kClipThreads) {
       u32x4 x[kDeep];
 #pragma unroll
-      for (int u = 0; u < kDeep; ++u) x[u] = load_any(p + (v + u * kClipThreads) * VE);
+      for (int u = 0; u < kDeep; ++u) x[u] = load_any_once(p + (v + u * kClipThreads) * VE);
 #pragma unroll
-      for (int u = 0; u < kDeep; ++u) store_any(o + (v + u * kClipThreads) * VE, scaled(x[u]));
+      for (int u = 0; u < kDeep; ++u) store_any_once(o + (v + u * kClipThreads) * VE, scaled(x[u]));
     }
     for (; v < vend; v += kClipThreads) store_any(o + v * VE, scaled(load_any(p + v * VE)));
     for (int e = vend * VE + threadIdx.x; e < s.n; e += kClipThreads) o[e] = (T)((float)p[e] * f);
@@ -277,7 +295,8 @@ int dtf_global_norm(const void* table, long chunks, void* partials, long slots, 
   if (!table_ok(table, chunks, partials, slots)) return -3;
   if (hyper ? (!hyper_out || n_hyper < 5 || n_hyper > kClipThreads || !(limit > 0.0)) : !norm_out) return -3;
   const int grid = clip_grid(chunks);
-  hipLaunchKernelGGL(norm_partials, dim3(grid), dim3(kClipThreads), 0, s, (const ClipChunk*)table, (int)chunks, (double*)partials);
+  hipLaunchKernelGGL(norm_partials, dim3(grid), dim3(kClipThreads), 0, s, (const ClipChunk*)table, (int)chunks,
+                     hyper ? kKeepChunks : 0, (double*)partials);      // (an update reads the gradients next, a bare norm nothing)
   hipLaunchKernelGGL(norm_finish, dim3(1), dim3(kClipThreads), 0, s, (const double*)partials, grid, scale, (const float*)hyper,
                      (float*)hyper_out, n_hyper, limit, (float*)norm_out);
   return (int)hipGetLastError();
@@ -288,7 +307,8 @@ int dtf_clip_by_global_norm(const void* table, long chunks, int in_place, void* 
                             void* norm_out, hipStream_t s) {
   if (!table_ok(table, chunks, partials, slots) || !norm_out || !(limit > 0.0) || !(limit <= 1.7976931348623157e308)) return -3;
   const int grid = clip_grid(chunks);
-  hipLaunchKernelGGL(norm_partials, dim3(grid), dim3(kClipThreads), 0, s, (const ClipChunk*)table, (int)chunks, (double*)partials);
+  hipLaunchKernelGGL(norm_partials, dim3(grid), dim3(kClipThreads), 0, s, (const ClipChunk*)table, (int)chunks, kKeepChunks,
+                     (double*)partials);
   hipLaunchKernelGGL(clip_scale, dim3(grid), dim3(kClipThreads), 0, s, (const ClipChunk*)table, (int)chunks, (const double*)partials, grid,
                      scale, limit, in_place, (float*)norm_out);
   return (int)hipGetLastError();

@@ -38,6 +38,11 @@ struct DtfEngineDesc {
   hipEvent_t ev_head, ev_fork, ev_join1, ev_join2, ev_dgrad;
   hipEvent_t ev_dense_ready, ev_dense_updated, ev_tail_ready, ev_tail_reduced;  // data-parallel step
   void* sk_ws;   // fp32: uncached stream-K workspace of the fc1 wgrad GEMM (gemm_f32.hip gemm_f32_sk), or NULL
+  // gradient clipping by the global norm (clip.hip); clip_norm == 0: off
+  double clip_norm;
+  const void* clip_table;   // chunks of the eight gradient tensors (no padding, no control block)
+  long clip_chunks, clip_slots;
+  void *clip_part, *hyper_clip, *grad_norm;
 };
 
 #define DTF_TRY(x)            \
@@ -56,6 +61,17 @@ static inline char* bf16at(void* base, long off) { return (char*)base + 2 * off;
 static inline bool is_f32(const DtfEngineDesc* e) { return e->dtype == 1; }
 // the fp32 configuration keeps no bf16 copies: optimizer kernels are told so with shadow == NULL
 static inline void* shadow_of(const DtfEngineDesc* e) { return is_f32(e) ? nullptr : e->shadow; }
+
+// what the update kernels read: with clipping, the copy whose gradient scale carries this step's clipping factor
+static inline const void* hyper_of(const DtfEngineDesc* e) { return e->clip_norm > 0.0 ? e->hyper_clip : e->hyper; }
+
+// Norm of the (final) gradients in the arena and hyper_clip from it: every update that follows on `s` is a clipped one.  No-op
+// without clipping.
+int dtf_engine_clip(const DtfEngineDesc* e, hipStream_t s) {
+  if (!(e->clip_norm > 0.0)) return 0;
+  return dtf_global_norm(e->clip_table, e->clip_chunks, e->clip_part, e->clip_slots, 1.0, e->hyper, e->hyper_clip, 12, e->clip_norm,
+                         e->grad_norm, s);
+}
 
 const char* dtf_build_flavour() { return DTF_DIAG ? "diag" : "release"; }
 
@@ -332,16 +348,16 @@ static int update_range_src(const DtfEngineDesc* e, long lo, long hi, int advanc
   if (g16) {
     if (!gsrc || is_f32(e)) return -3;
     if (e->optimizer == 0)
-      return dtf_sgd_update_g16(f32at(e->params, lo), g, bf16at(e->shadow, lo), e->hyper, n, st, cinc, step_inc, 1, s);
+      return dtf_sgd_update_g16(f32at(e->params, lo), g, bf16at(e->shadow, lo), hyper_of(e), n, st, cinc, step_inc, 1, s);
     return dtf_adam_update_g16(f32at(e->params, lo), g, f32at(e->adam_m, lo), f32at(e->adam_v, lo), bf16at(e->shadow, lo),
-                               e->hyper, n, e->state, adam_slot, st, cinc, step_inc, 1, s);
+                               hyper_of(e), n, e->state, adam_slot, st, cinc, step_inc, 1, s);
   }
   if (e->optimizer == 0)
-    DTF_TRY(dtf_sgd_update(f32at(e->params, lo), g, is_f32(e) ? nullptr : bf16at(e->shadow, lo), e->hyper, n, st, cinc,
+    DTF_TRY(dtf_sgd_update(f32at(e->params, lo), g, is_f32(e) ? nullptr : bf16at(e->shadow, lo), hyper_of(e), n, st, cinc,
                            step_inc, 1, s));
   else
     DTF_TRY(dtf_adam_update(f32at(e->params, lo), g, f32at(e->adam_m, lo), f32at(e->adam_v, lo),
-                            is_f32(e) ? nullptr : bf16at(e->shadow, lo), e->hyper, n, e->state, adam_slot, st, cinc,
+                            is_f32(e) ? nullptr : bf16at(e->shadow, lo), hyper_of(e), n, e->state, adam_slot, st, cinc,
                             step_inc, 1, s));
   // the head kernel reads the output weight transposed: keep that copy current
   if (lo <= e->off_out_w && e->off_out_w < hi)
@@ -399,6 +415,22 @@ int dtf_engine_train_step(const DtfEngineDesc* e, long step_inc, hipStream_t s) 
   // the batch sampler runs inside conv1 forward (rows from the device cursor, published in e->idx)
   DTF_TRY(forward_conv_impl(e, e->ds_images, nullptr, 1, e->B, s));
   DTF_TRY(dtf_engine_forward_dense(e, e->ds_labels, e->idx, 1, e->B, 1, s));
+  if (e->clip_norm > 0.0) {
+    // The norm needs every gradient before the first update: slab sums into the arena, norm, then the fused tail with the arena
+    // itself as a single slab per segment.
+    DTF_TRY(backward_impl(e, e->ds_images, e->idx, 1, s));
+    DTF_TRY(dtf_engine_clip(e, s));
+    const void* part[3] = {f32at(e->grads, e->off_out_w), f32at(e->grads, e->off_wc2), f32at(e->grads, e->off_wc1)};
+    int G[3] = {1, 1, 1}, n[3] = {(int)e->head_stride, (int)e->c2_stride, (int)e->c1_stride};
+    long st[3] = {e->head_stride, e->c2_stride, e->c1_stride};
+    long off[3] = {e->off_out_w, e->off_wc2, e->off_wc1};
+    if (e->optimizer == 0)
+      return dtf_fused_reduce_sgd(3, part, G, n, st, off, e->params, e->grads, shadow_of(e), hyper_of(e), e->off_wd1, e->off_out_w,
+                                  e->wc2T, e->off_wc2, e->c1, e->c2, e->out_wT, e->off_out_w, e->hidden, e->state, e->B, step_inc, 1, s);
+    return dtf_fused_reduce_adam(3, part, G, n, st, off, e->params, e->grads, e->adam_m, e->adam_v, shadow_of(e), hyper_of(e),
+                                 e->off_wd1, e->off_out_w, e->wc2T, e->off_wc2, e->c1, e->c2, e->out_wT, e->off_out_w, e->hidden,
+                                 e->state, 3, e->B, step_inc, 1, s);
+  }
   if (e->optimizer != 0) {
     // Adam: the same fused tail (slab sums + update of the whole arena + shadows + packs + state advance)
     DTF_TRY(backward_impl(e, e->ds_images, e->idx, 0, s));
@@ -440,7 +472,9 @@ int dtf_engine_train_step(const DtfEngineDesc* e, long step_inc, hipStream_t s) 
 //                                                   [Python: all-reduce tail, on s itself by default]
 //   phase3: updates the tail (+ state advance), repacks wc2.  (With a separate tail stream: two event pairs.)
 // ---------------------------------------------------------------------------------------------
+// (Gradient clipping needs the whole reduced gradient before any update and has no place in this schedule: refused.)
 int dtf_engine_dp_phase1(const DtfEngineDesc* e, int wait_dense_updated, hipStream_t s, hipStream_t comm) {
+  if (e->clip_norm > 0.0) return -1;
   DTF_TRY(forward_conv_impl(e, e->ds_images, nullptr, 1, e->B, s));
   if (wait_dense_updated) HIP_TRY(hipStreamWaitEvent(s, e->ev_dense_updated, 0));
   DTF_TRY(dtf_engine_forward_dense(e, e->ds_labels, e->idx, 1, e->B, 1, s));
@@ -523,6 +557,7 @@ int dtf_engine_dp_phase3(const DtfEngineDesc* e, long dense_hi, int tail_adam_sl
 // ---------------------------------------------------------------------------------------------
 int dtf_engine_dp_step(const DtfEngineDesc* e, const DtfDpFabric* f, int collapse_world1, long step_inc, hipStream_t s,
                        hipStream_t comm) {
+  if (e->clip_norm > 0.0) return -1;
   if (!f || f->n_dense != (long)e->flat * e->hidden || f->n_tail != e->n_total - e->off_out_w || e->off_wd1 != 0 ||
       f->ag_bytes != (is_f32(e) ? 4 : 2) || e->dense_g16)
     return -3;

@@ -111,10 +111,10 @@ class CpuBackend(Backend):
     name = "cpu"
 
     def __init__(self, spec: ModelSpec, batch: int, data: Datasets, optimizer="sgd", learning_rate=1e-3,
-                 keep_prob=1.0, seed=0):
+                 keep_prob=1.0, seed=0, clip_norm=0.0):
         self.spec, self.batch, self.data = spec, batch, data
         self.model = OracleModel(spec, device="cpu", seed=seed, optimizer=optimizer, learning_rate=learning_rate,
-                                 keep_prob=keep_prob)
+                                 keep_prob=keep_prob, clip_norm=clip_norm)
         self.layout = self.model.layout
         self._metrics = (float("nan"), float("nan"))
 
@@ -188,7 +188,7 @@ class HipBackend(Backend):
     name = "hip"
 
     def __init__(self, spec: ModelSpec, batch: int, data: Datasets, optimizer="sgd", learning_rate=1e-3,
-                 keep_prob=1.0, seed=0, device="cuda", use_graph=True, dtype="bf16"):
+                 keep_prob=1.0, seed=0, device="cuda", use_graph=True, dtype="bf16", clip_norm=0.0):
         from .engine import DeviceDataset, HipEngine
         self.spec, self.batch, self.data = spec, batch, data
         self.dtype = dtype
@@ -197,7 +197,8 @@ class HipBackend(Backend):
                                                  dtype=dtype)
         self._eval_cache = {}
         self.engine = HipEngine(spec, batch, self.train_ds, optimizer=optimizer, learning_rate=learning_rate,
-                                keep_prob=keep_prob, seed=seed, device=device, fuse_dense_update=True, dtype=dtype)
+                                keep_prob=keep_prob, seed=seed, device=device, fuse_dense_update=True, dtype=dtype,
+                                clip_norm=clip_norm)
         self.layout = self.engine.layout
         # measured on MI355X: eager launches of the 8-kernel step beat graph replay up to 1024 images/step
         self.use_graph = bool(use_graph) and batch > 1024 and dtype == "bf16"

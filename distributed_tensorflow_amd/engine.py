@@ -18,6 +18,7 @@ Memory plan (all resident, sized once for ``batch``):
 from __future__ import annotations
 
 import ctypes
+import math
 import os
 from dataclasses import dataclass
 from typing import Dict, Optional
@@ -26,6 +27,7 @@ import torch
 
 from .models.spec import ArenaLayout, ModelSpec
 from .ops import native
+from .ops.clip import GlobalNormClip
 from .ops.native import check, ptr
 
 
@@ -127,7 +129,13 @@ class HipEngine:
                  optimizer: str = "sgd", learning_rate: float = 1e-3, keep_prob: float = 1.0,
                  seed: int = 0, device="cuda", grad_scale: float = 1.0, shuffle: bool = True,
                  adam_betas=(0.9, 0.999), adam_eps: float = 1e-8, step_inc: int = 1, multi_stream: Optional[bool] = None,
-                 fuse_dense_update: bool = False, dtype: str = "bf16", tuning: Optional[Tuning] = None):
+                 fuse_dense_update: bool = False, dtype: str = "bf16", tuning: Optional[Tuning] = None,
+                 clip_norm: float = 0.0):
+        """clip_norm > 0: every update applies gradients scaled by clip_norm / max(norm, clip_norm), norm = the global norm
+        of the (scaled) gradients of all eight tensors, which ``grad_norm()`` reads back (tf.clip_by_global_norm before
+        apply_gradients); 0: no clipping.  A norm that is not finite makes the parameters NaN."""
+        if not (clip_norm >= 0.0 and math.isfinite(clip_norm)):
+            raise ValueError(f"clip_norm must be finite and not negative, got {clip_norm}")
         if not torch.cuda.is_available():
             raise RuntimeError("HipEngine needs a GPU (use backend='cpu' / models.oracle on CPU)")
         self.lib = native.load()
@@ -259,6 +267,12 @@ class HipEngine:
         self._graph = None
         self._graph_stream = None
         self.dense_g16 = None      # see enable_dense_g16()
+        self.clip_norm = float(clip_norm)
+        if self.clip_norm:
+            self._clip = GlobalNormClip([lay.view(self.grads, name) for name in lay.names()])
+            self._clip_part = torch.empty(self._clip.slots, dtype=torch.float64, device=dev)
+            self._hyper_clip = torch.zeros_like(self.hyper)
+            self._grad_norm = torch.zeros((), **f32)
         self._build_desc()
 
     def _build_desc(self):
@@ -286,6 +300,10 @@ class HipEngine:
             setattr(d, name, getattr(self, name).data_ptr())
         if self.optimizer == "adam":
             d.adam_m, d.adam_v = self.adam_m.data_ptr(), self.adam_v.data_ptr()
+        if self.clip_norm:
+            d.clip_norm, d.clip_table, d.clip_chunks = self.clip_norm, self._clip.table.data_ptr(), self._clip.chunks
+            d.clip_part, d.clip_slots = self._clip_part.data_ptr(), self._clip.slots
+            d.hyper_clip, d.grad_norm = self._hyper_clip.data_ptr(), self._grad_norm.data_ptr()
         self._desc = d
         self._set_dataset(self.dataset)
         check(self.lib.dtf_engine_init(ctypes.byref(d)), "engine_init")
@@ -449,7 +467,18 @@ class HipEngine:
         """K-contiguous copy of the conv2 filter for the forward kernel (wd1 is used in place)."""
         check(self.lib.dtf_engine_transposes(self._d(), int(wc2), self._s()), "transposes")
 
+    def launch_clip(self):
+        """Norm of the gradients in the arena and the clipping factor for the updates that follow (no-op with clip_norm 0)."""
+        check(self.lib.dtf_engine_clip(self._d(), self._s()), "clip")
+
+    def grad_norm(self) -> float:
+        """Global norm of the last clipped step's gradients, before clipping (reads device memory: synchronises)."""
+        if not self.clip_norm:
+            raise RuntimeError("grad_norm() needs an engine with clip_norm > 0")
+        return float(self._grad_norm.item())
+
     def launch_update(self, advance_cursor: bool = True):
+        self.launch_clip()
         self.launch_update_range(0, self.layout.total, True, advance_cursor)
         self.refresh_transposes()
 

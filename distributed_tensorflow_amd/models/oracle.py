@@ -24,7 +24,8 @@ from .spec import ArenaLayout, ModelSpec
 class OracleModel:
     def __init__(self, spec: Optional[ModelSpec] = None, device="cpu", seed: int = 0, optimizer: str = "sgd",
                  learning_rate: float = 1e-3, keep_prob: float = 1.0, adam_betas=(0.9, 0.999),
-                 adam_eps: float = 1e-8):
+                 adam_eps: float = 1e-8, clip_norm: float = 0.0):
+        self.clip_norm = clip_norm      # > 0: gradients clipped by their global norm before the update
         self.spec = spec or ModelSpec()
         self.layout = ArenaLayout(self.spec)
         self.device = torch.device(device)
@@ -92,6 +93,11 @@ class OracleModel:
     def apply_gradients(self, grad_arena: Optional[torch.Tensor] = None, scale: float = 1.0, step_inc: int = 1):
         """ApplyGradientDescent / Adam over the flat arena + global_step increment."""
         g = (self.grad_arena if grad_arena is None else grad_arena.to(self.device)) * scale
+        if self.clip_norm > 0.0:
+            views = [self.layout.view(g, n) for n in self.layout.names()]
+            clipped, self.grad_norm = R.clip_by_global_norm(views, self.clip_norm)
+            for v, c in zip(views, clipped):
+                v.copy_(c)
         if self.optimizer == "sgd":
             self.arena.add_(g, alpha=-self.lr)
         elif self.optimizer == "adam":

@@ -170,6 +170,8 @@ class EngineDesc(ctypes.Structure):
                                    "ds_labels")]
         + [(n, c_void_p) for n in ("side1", "side2", "ev_head", "ev_fork", "ev_join1", "ev_join2", "ev_dgrad",
                                    "ev_dense_ready", "ev_dense_updated", "ev_tail_ready", "ev_tail_reduced", "sk_ws")]
+        + [("clip_norm", c_double), ("clip_table", c_void_p), ("clip_chunks", c_long), ("clip_slots", c_long),
+           ("clip_part", c_void_p), ("hyper_clip", c_void_p), ("grad_norm", c_void_p)]
     )
 
 
@@ -186,6 +188,7 @@ _ENGINE_SIGS = {
     "dtf_engine_backward_dense": [_EP, c_void_p],
     "dtf_engine_backward_conv": [_EP, c_void_p, c_void_p, c_int, c_void_p],
     "dtf_engine_backward": [_EP, c_void_p, c_void_p, c_void_p],
+    "dtf_engine_clip": [_EP, c_void_p],
     "dtf_engine_update_range": [_EP, c_long, c_long, c_int, c_int, c_long, c_int, c_void_p],
     "dtf_engine_transposes": [_EP, c_int, c_void_p],
     "dtf_engine_train_step": [_EP, c_long, c_void_p],

@@ -135,8 +135,14 @@ class SyncAllReduce:
         # The overlapped schedule (parallel/sync_dp.py) needs collectives that run on streams: RCCL, or the
         # peer-to-peer kernels (--p2p_allreduce; these also work between tasks that share one GPU over gloo).
         # (an explicit --dense_update=sharded also selects it over gloo, staged through the host: tests, rehearsals)
-        if backend.name == "hip" and (dist.get_backend(worker_group) != "gloo" or p2p or shard_dense
-                                      or grad_comm == "bf16"):
+        # Gradients that are clipped by their global norm (--clip_norm) need the whole sum before the first update: one
+        # all-reduce of the arena, then norm and update, without overlap.
+        clip = backend.name == "hip" and backend.engine.clip_norm > 0.0
+        if clip and (p2p or shard_dense or grad_comm == "bf16"):
+            raise ValueError("gradient clipping needs the all-reduced fp32 gradient on every worker: no --p2p_allreduce, "
+                             "--dense_update=sharded or --grad_comm=bf16")
+        if backend.name == "hip" and not clip and (dist.get_backend(worker_group) != "gloo" or p2p or shard_dense
+                                                   or grad_comm == "bf16"):
             from .sync_dp import SyncDataParallel
             fabric = None
             if p2p and grad_comm != "bf16":

@@ -96,6 +96,9 @@ class SyncDataParallel:
             raise ValueError("grad_comm=bf16 needs the bf16 configuration (the fp32 configuration is exact end to end)")
         if grad_comm == "bf16" and fabric is not None:
             raise ValueError("grad_comm=bf16 uses the process-group collectives; the exchange fabric sums fp32")
+        if engine.clip_norm:
+            raise ValueError("this schedule updates the dense range before the tail's gradient exists: no gradient clipping "
+                             "(strategies.SyncAllReduce all-reduces the whole arena for an engine that clips)")
         self.grad_comm = grad_comm
         self.eng = engine
         self.group = group

@@ -15,6 +15,7 @@ collective update over the global batch.
 """
 from __future__ import annotations
 
+import math
 import os
 import sys
 import time
@@ -81,6 +82,17 @@ def run(F, log=print) -> dict:
         # every task checks this before the rendezvous, so a refused job ends everywhere at once
         raise SystemExit("--grad_comm=bf16 needs --mode=sync with --backend=hip and --dtype=bf16 (more than one task)")
 
+    clip_norm = float(getattr(F, "clip_norm", 0.0))
+    if not (clip_norm >= 0.0 and math.isfinite(clip_norm)):
+        raise SystemExit(f"--clip_norm must be finite and not negative, got {clip_norm}")
+    if clip_norm and mode == "async":
+        raise SystemExit("--clip_norm needs --mode=sync (or a single task): the parameter server applies every worker's gradient as "
+                         "it arrives, shard by shard, and no task holds a whole gradient's norm")
+    if clip_norm and mode == "sync" and (getattr(F, "p2p_allreduce", False) or grad_comm == "bf16" or
+                                         getattr(F, "dense_update", "auto") == "sharded"):
+        raise SystemExit("--clip_norm clips the summed gradient of all workers, which every worker has to hold: not with "
+                         "--p2p_allreduce, --grad_comm=bf16 or --dense_update=sharded")
+
     if kind == "hip":
         local_rank = int(os.environ.get("LOCAL_RANK", F.local_rank if F.local_rank >= 0 else task.rank))
         local_rank %= max(1, torch.cuda.device_count())
@@ -115,7 +127,7 @@ def run(F, log=print) -> dict:
                           seed=F.seed + 1000 * task.rank)   # every worker shuffles independently (ref. item 9)
     backend = make_backend(kind, spec, F.batch_size, data, optimizer=F.optimizer, learning_rate=F.learning_rate,
                            keep_prob=F.keep_prob, seed=F.seed + task.rank, device=device, use_graph=F.hip_graph,
-                           dtype=getattr(F, "dtype", "bf16"))
+                           dtype=getattr(F, "dtype", "bf16"), clip_norm=clip_norm)
 
     chief_rank = task.cluster.rank_of("worker", 0)
     worker_group = tail_group = None

@@ -75,6 +75,8 @@ flags.DEFINE_string("dense_update", "auto", "sync mode, hip backend over RCCL: a
 flags.DEFINE_string("grad_comm", "fp32", "sync mode, hip backend, bf16 configuration: fp32 (reference arithmetic) | bf16 (opt-in: the "
                     "fc1 weight gradient -- 98 % of the bytes -- is produced, summed across workers and consumed in bf16; "
                     "half the bytes of the dominant collective, not the reference's fp32 gradient sum)")
+flags.DEFINE_float("clip_norm", 0.0, "clip every step's gradient by its global norm (tf.clip_by_global_norm over all eight tensors; "
+                   "sync mode: of the workers' mean gradient); 0 = off")
 flags.DEFINE_boolean("trace", False, "roctx ranges around steps/collectives/checkpoints (rocprofv3 --marker-trace)")
 flags.DEFINE_integer("fault_inject_step", -1, "test hook: crash this worker after N local steps")
 flags.DEFINE_integer("fault_inject_task", -1, "test hook: which worker task crashes (-1 = any)")
