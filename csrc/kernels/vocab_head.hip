@@ -218,18 +218,19 @@ struct VhFrags {
   }
 };
 
-// Main loop: K tiles t0 .. t1 - 1 in two LDS buffers.
+// Main loop: K tiles t0 .. t1 - 1 in D LDS buffers (two for the large tiles, which take all of LDS; four for small ones, whose
+// tiles are over sooner than their operands arrive).
 //
 // Both operands fast (or fp32): a tile is multiplied in two halves, and the fragments of a half are read during the MFMAs of
 // the half before it, one barrier per tile:
 //   read the second half of tile t | MFMAs on the first | wait until tile t + 1 has landed, barrier
-//   DMA of tile t + 2 into the buffer of tile t | read the first half of tile t + 1 | MFMAs on the second half of tile t
+//   DMA of tile t + D into the buffer of tile t | read the first half of tile t + 1 | MFMAs on the second half of tile t
 // A bf16 slow operand (its fragments are read right before their MFMAs; the other wave of the SIMD covers the wait):
-//   wait until tile t has landed, barrier | DMA of tile t + 1 into the buffer of tile t - 1 | both halves of tile t
+//   wait until tile t has landed, barrier | DMA of tile t + D - 1 into the buffer of tile t - 1 | both halves of tile t
 //
 // The epilogue's inputs (labels, log-sum-exps, biases of the tile) are requested before the first operand tile and put into
 // LDS behind it, where they cost no latency at the end.
-template <typename T, int BM, int BN, int NWM, int NWN, bool AS, bool BS, class Epi, class Tile>
+template <typename T, int BM, int BN, int NWM, int NWN, bool AS, bool BS, int D, class Epi, class Tile>
 __device__ __forceinline__ void vh_mainloop(const VhOperands& p, Tile& c, char* lds, int t0, int t1, const Epi& e,
                                             typename Epi::template Inputs<BM, BN>* in) {
   constexpr int NT = Tile::NT, MT = Tile::MT, NTL = Tile::NTL;
@@ -246,11 +247,12 @@ __device__ __forceinline__ void vh_mainloop(const VhOperands& p, Tile& c, char* 
   VhFrags<T, BN, BS, NTL> rb;
   ra.init(c.wm0, c.lane);
   rb.init(c.wn0, c.lane);
-  auto dma = [&](int t) {
-    char* const buf = lds + ((t - t0) & 1) * STAGE;
+  auto dma = [&](int t, char* buf) {
     la.dma(t, buf, c.wave, tid);
     lb.dma(t, buf + ABYTES, c.wave, tid);
   };
+  char* const ring_end = lds + D * STAGE;
+  auto next = [&](char* buf) { return buf + STAGE == ring_end ? lds : buf + STAGE; };
 #pragma unroll
   for (int i = 0; i < MT; ++i)
 #pragma unroll
@@ -263,15 +265,19 @@ __device__ __forceinline__ void vh_mainloop(const VhOperands& p, Tile& c, char* 
     typedef VhFrags<T, BM, AS, MT> RA;
     typedef VhFrags<T, BN, BS, NTL> RB;
     static_assert(AS && MT % RA::TR == 0 && (!BS || NTL % RB::TR == 0), "slow products: dh (A) and dw (A and B)");
-    dma(t0);
+#pragma unroll
+    for (int d = 0; d + 1 < D; ++d)
+      if (t0 + d < t1) dma(t0 + d, lds + d * STAGE);
     e.template keep<BM, BN, NT>(early, in, tid);
+    char* buf = lds;
+    char* last = lds + (D - 1) * STAGE;         // the buffer of tile t - 1
 #pragma unroll 1
     for (int t = t0; t < t1; ++t) {
-      const char* buf = lds + ((t - t0) & 1) * STAGE;
-      vh_wait<0>();
+      if (D > 2 && t + D - 1 <= t1) vh_wait<(D - 2) * NDMA>();
+      else vh_wait<0>();
       vh_barrier();
       if constexpr (!BS) rb.read(fb[0], buf + ABYTES, 0);
-      if (t + 1 < t1) dma(t + 1);
+      if (t + D - 1 < t1) dma(t + D - 1, last);
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         if constexpr (BS) {
@@ -290,11 +296,12 @@ __device__ __forceinline__ void vh_mainloop(const VhOperands& p, Tile& c, char* 
             for (int j = 0; j < NTL; ++j) c.acc[i + k][j] = VhType<T>::mma(a[k], fb[BS ? 0 : h][j], c.acc[i + k][j]);
         }
       }
+      last = buf;
+      buf = next(buf);
     }
   } else {
     u32x4 fa[2][MT];
-    auto frags = [&](int x, int t, int half) {
-      const char* buf = lds + ((t - t0) & 1) * STAGE;
+    auto frags = [&](int x, const char* buf, int half) {
       ra.read(fa[x], buf, half);
       rb.read(fb[x], buf + ABYTES, half);
     };
@@ -322,39 +329,39 @@ __device__ __forceinline__ void vh_mainloop(const VhOperands& p, Tile& c, char* 
       }
       __builtin_amdgcn_sched_barrier(0);
     };
-    dma(t0);
-    if (t0 + 1 < t1) {
-      dma(t0 + 1);
-      e.template keep<BM, BN, NT>(early, in, tid);
-      vh_wait<NDMA>();
-    } else {
-      e.template keep<BM, BN, NT>(early, in, tid);
-      vh_wait<0>();
-    }
+#pragma unroll
+    for (int d = 0; d < D; ++d)
+      if (t0 + d < t1) dma(t0 + d, lds + d * STAGE);
+    e.template keep<BM, BN, NT>(early, in, tid);
+    if (t0 + D <= t1) vh_wait<(D - 1) * NDMA>();
+    else vh_wait<0>();
     vh_barrier();
-    frags(0, t0, 0);
+    frags(0, lds, 0);
     vh_wait<63>();
     int t = t0;
+    char* buf = lds;
 #pragma unroll 1
-    for (; t + 2 < t1; ++t) {
-      frags(1, t, 1);
+    for (; t + D < t1; ++t) {
+      frags(1, buf, 1);
       mma(0);
       spread(false);
-      vh_wait<0>();
+      vh_wait<(D - 2) * NDMA>();
       vh_barrier();
-      dma(t + 2);
-      frags(0, t + 1, 0);
+      dma(t + D, buf);
+      buf = next(buf);
+      frags(0, buf, 0);
       mma(1);
       spread(true);
       vh_wait<63>();
     }
 #pragma unroll 1
     for (; t < t1; ++t) {
-      frags(1, t, 1);
+      frags(1, buf, 1);
       mma(0);
       vh_wait<0>();
       vh_barrier();
-      frags(0, t + 1 < t1 ? t + 1 : t, 0);      // (behind the last tile: read, not used)
+      buf = next(buf);
+      frags(0, buf, 0);      // (behind the last tile: some buffer, read and not used)
       mma(1);
       vh_wait<63>();
     }
@@ -363,14 +370,14 @@ __device__ __forceinline__ void vh_mainloop(const VhOperands& p, Tile& c, char* 
   vh_barrier();
 }
 
-template <typename T, int BM, int BN, int NWM, int NWN, bool AS, bool BS, class Epi>
+template <typename T, int BM, int BN, int NWM, int NWN, bool AS, bool BS, int D, class Epi>
 __global__ __launch_bounds__(NWM * NWN * 64, 1) void vh_gemm(VhOperands p, Epi e) {
   typedef VhTile<T, BM, BN, NWM, NWN> Tile;
   // one LDS object: with two of them the compiler orders every fragment read behind all LDS-DMAs in flight (s_waitcnt
   // vmcnt(0) in the middle of the loop, forward 15 % slower)
   typedef typename Epi::template Inputs<BM, BN> Inputs;
-  __shared__ __attribute__((aligned(16))) char lds[2 * (BM + BN) * 128 + sizeof(Inputs)];
-  Inputs& in = *reinterpret_cast<Inputs*>(lds + 2 * (BM + BN) * 128);
+  __shared__ __attribute__((aligned(16))) char lds[D * (BM + BN) * 128 + sizeof(Inputs)];
+  Inputs& in = *reinterpret_cast<Inputs*>(lds + D * (BM + BN) * 128);
   Tile c;
   c.lane = threadIdx.x & 63;
   c.wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -383,7 +390,7 @@ __global__ __launch_bounds__(NWM * NWN * 64, 1) void vh_gemm(VhOperands p, Epi e
   c.m0 = tx * BM;
   c.n0 = ty * BN;
   const int per = (p.ktiles + p.splits - 1) / p.splits, t0 = c.split * per;
-  vh_mainloop<T, BM, BN, NWM, NWN, AS, BS>(p, c, lds, t0, min(p.ktiles, t0 + per), e, &in);
+  vh_mainloop<T, BM, BN, NWM, NWN, AS, BS, D>(p, c, lds, t0, min(p.ktiles, t0 + per), e, &in);
   e.template run<T, BM, BN, NWM, NWN>(p, c, tx, ty, lds, in);
 }
 
@@ -458,13 +465,14 @@ __device__ __forceinline__ MaxSum join(MaxSum a, MaxSum b) {
 struct VhForward {
   const float* bias;
   const int* labels;
+  int c0;                   // the product's first class
   float2* part;
   float* zlab;
   long ldpart;
   template <int BM, int BN> using Inputs = VhLogitsInputs<BM, BN>;
   __device__ __forceinline__ VhRowInputs row_inputs(int row, int m0) const {
     const int y = labels[row];
-    return {y < 0 ? -1 : y - m0, 0.f, 0.f};
+    return {y < c0 ? -1 : y - c0 - m0, 0.f, 0.f};
   }
   template <int BM, int BN, int NT>
   __device__ __forceinline__ VhEarly<BM, BN, NT> request(const VhOperands& p, int m0, int n0, int tid) const {
@@ -530,9 +538,10 @@ struct VhGradLogits {
   const float* lse;
   const float* row_scale;   // or nullptr
   float grad_scale;
-  int v0, classes, ignore;
+  int v0, classes, ignore;  // the product's first class, all classes
   void* d;
   long ldd;
+  int places;               // of this product's classes: up to there d is written
   float* dbpart;            // [row tile][ldd] or nullptr
   template <int BM, int BN> using Inputs = VhLogitsInputs<BM, BN>;
   __device__ __forceinline__ VhRowInputs row_inputs(int row, int m0) const {
@@ -588,7 +597,7 @@ struct VhGradLogits {
             const int m = mw + 16 * i;
             const f32x4 v = c.acc[i][j], x = c.acc[i + 1][j];
             const bf16x8 y = {(T)v[0], (T)v[1], (T)v[2], (T)v[3], (T)x[0], (T)x[1], (T)x[2], (T)x[3]};
-            if (m < ldd) *reinterpret_cast<bf16x8*>(o + vh_place(m)) = y;
+            if (m < places) *reinterpret_cast<bf16x8*>(o + vh_place(m)) = y;
           }
         } else {
           typedef __attribute__((ext_vector_type(4))) T T4;
@@ -597,7 +606,7 @@ struct VhGradLogits {
             const int m = mw + 16 * i;
             const f32x4 v = c.acc[i][j];
             const T4 y = {(T)v[0], (T)v[1], (T)v[2], (T)v[3]};
-            if (m < ldd) *reinterpret_cast<T4*>(o + (sizeof(T) == 2 ? vh_place(m) : m)) = y;
+            if (m < places) *reinterpret_cast<T4*>(o + (sizeof(T) == 2 ? vh_place(m) : m)) = y;
           }
         }
       }
@@ -618,15 +627,17 @@ struct VhGradLogits {
       float s = red[0][i];
 #pragma unroll
       for (int w = 1; w < NWN; ++w) s += red[w][i];
-      if (c.m0 + i < ldd) dbpart[(long)ty * ldd + c.m0 + i] = s;
+      if (c.m0 + i < places) dbpart[(long)ty * ldd + c.m0 + i] = s;
     }
   }
 };
 
 // Plain product: out[j][i], j < rows, in the operand type or fp32; the product's j is a place of d where by_place is set
 // (its N is then the number of places).  With sum: fp32 [split][rows][M] running sums over the pieces of the classes, read unless `first` and written unless `last` (a single split:
-// the last piece's result goes to out).
-struct VhStore {
+// the last piece's result goes to out).  ONCE: the result is not to be kept in the caches (a template argument: as a value the
+// compiler folds the two kinds of stores into the plain one).
+template <bool ONCE>
+struct VhStoreT {
   void* out;
   long ldo;
   int out_f32;
@@ -662,14 +673,14 @@ struct VhStore {
         }
       }
       if (!last) {
-        store<float, V>(s, v, M - m);
+        store<float, V, false>(s, v, M - m);      // (read again soon)
         return;
       }
     }
-    if (out_f32 || sizeof(T) == 4) store<float, V>((float*)out + row * ldo + m, v, M - m);
-    else store<T, V>((T*)out + row * ldo + m, v, M - m);
+    if (out_f32 || sizeof(T) == 4) store<float, V, ONCE>((float*)out + row * ldo + m, v, M - m);
+    else store<T, V, ONCE>((T*)out + row * ldo + m, v, M - m);
   }
-  template <typename O, int V>
+  template <typename O, int V, bool KEEP_OUT>
   static __device__ __forceinline__ void store(O* o, const float (&v)[V], int left) {
     constexpr int W = 16 / sizeof(O) < V ? 16 / sizeof(O) : V;
     typedef __attribute__((ext_vector_type(W))) O vec;
@@ -680,7 +691,8 @@ struct VhStore {
         vec x;
 #pragma unroll
         for (int r = 0; r < W; ++r) x[r] = (O)v[q + r];
-        *reinterpret_cast<vec_any*>(o + q) = x;
+        if constexpr (KEEP_OUT) __builtin_nontemporal_store(x, reinterpret_cast<vec_any*>(o + q));
+        else *reinterpret_cast<vec_any*>(o + q) = x;
       }
     } else {
 #pragma unroll
@@ -722,6 +734,8 @@ struct VhStore {
     }
   }
 };
+
+typedef VhStoreT<false> VhStore;
 
 // ---- small kernels --------------------------------------------------------------------------------------------------
 // lse and loss of a row from its (maximum, sum) pairs, joined in a fixed order.  One workgroup takes ROWS rows, 256 / ROWS
@@ -846,12 +860,57 @@ constexpr int kPiece = 256;           // pieces are multiples of this many class
 //   kLarge: 256 x 256 tiles of eight waves, one workgroup per CU.
 enum { kSmall, kMid, kLarge };
 int config_for(int E, long n) { return n <= 64 ? kSmall : (E == 4 || n <= 128 ? kMid : kLarge); }
-constexpr int logits_bm(int cfg) { return cfg == kSmall ? 64 : (cfg == kMid ? 128 : 256); }
-constexpr int rows_bn(int cfg) { return cfg == kSmall ? 64 : (cfg == kMid ? 64 : 256); }
+constexpr int rows_bn(int cfg) { return cfg == kLarge ? 256 : 64; }         // of dh
 constexpr int hidden_bm(int cfg) { return cfg == kLarge ? 256 : 128; }      // of dh and dw
-constexpr int classes_bn(int cfg) { return cfg == kLarge ? 256 : 64; }     // of dw
+constexpr int classes_bn(int cfg) { return cfg == kLarge ? 256 : 64; }      // of dw
 
-template <typename T, int BM, int BN, int NWM, int NWN, bool AS, bool BS, class Epi>
+// How the logits product of some classes is tiled: the classes below `first` in tiles of one kind, the others in a second one.
+// The large kinds run one workgroup per CU, so what counts is the number of rounds over the 256 CUs times the length of a round
+// (measured at H = 4096, against 256 x 256: 0.82 for 192 x 256, 0.68 for 256 x 128), and a last round for a few tiles is as long
+// as any other: its classes go to small tiles instead.  777 rows x 50001 classes: 784 tiles are four rounds, 362 us; three
+// rounds and 91 small tiles 299 us.
+struct LogitsTile {
+  int bm, bn;
+};
+struct LogitsTiling {
+  LogitsTile kind[2];
+  int first;              // classes of the first kind (a multiple of its bm, or all)
+  int tiles[2];           // class tiles of either
+};
+LogitsTiling logits_tiling(int cfg, long n, int classes) {
+  LogitsTiling q{{{128, 64}, {128, 64}}, classes, {0, 0}};
+  if (cfg == kSmall) q.kind[0] = {64, 64};
+  if (cfg == kLarge) {
+    const struct { LogitsTile t; double length; } kinds[3] = {{{256, 256}, 1.0}, {{192, 256}, 0.82}, {{256, 128}, 0.68}};
+    // small tiles: three to a CU; the first of a CU costs more than the next two
+    auto small = [&](int rest) {
+      const long t = (long)cdiv(rest, 128) * cdiv(n, 64);
+      return rest ? 0.16 + 0.14 * cdiv(t, 256) : 0.0;
+    };
+    double least = 1e30;
+    for (const auto& k : kinds) {
+      const int rows = cdiv(n, k.t.bn), cols = cdiv(classes, k.t.bm);
+      const int full = (int)((long)rows * cols / 256);
+      const int some = (int)(full * 256L / rows);          // class tiles that fill whole rounds
+      const double whole = cdiv((long)rows * cols, 256) * k.length, split = full * k.length + small(classes - some * k.t.bm);
+      if (whole < least) {
+        least = whole;
+        q.kind[0] = k.t;
+        q.first = classes;
+      }
+      if (some > 0 && some < cols && split < least) {
+        least = split;
+        q.kind[0] = k.t;
+        q.first = some * k.t.bm;
+      }
+    }
+  }
+  q.tiles[0] = cdiv(q.first, q.kind[0].bm);
+  q.tiles[1] = cdiv(classes - q.first, q.kind[1].bm);
+  return q;
+}
+
+template <typename T, int BM, int BN, int NWM, int NWN, bool AS, bool BS, int D, class Epi>
 int launch(VhOperands p, int splits, const Epi& e, hipStream_t s) {
   p.tiles_m = cdiv(p.M, BM);
   p.tiles_n = cdiv(p.N, BN);
@@ -859,34 +918,54 @@ int launch(VhOperands p, int splits, const Epi& e, hipStream_t s) {
   p.splits = splits;
   const long grid = (long)p.tiles_m * p.tiles_n * splits;
   if (grid > 0x7fffffff) return -1;
-  hipLaunchKernelGGL((vh_gemm<T, BM, BN, NWM, NWN, AS, BS, Epi>), dim3((unsigned)grid), dim3(NWM * NWN * 64), 0, s, p, e);
+  hipLaunchKernelGGL((vh_gemm<T, BM, BN, NWM, NWN, AS, BS, D, Epi>), dim3((unsigned)grid), dim3(NWM * NWN * 64), 0, s, p, e);
   return (int)hipGetLastError();
 }
 
-// logits^T [classes][rows] = w . h^T
+// logits^T [classes][rows] = w . h^T with one kind of tiles
 template <typename T, class Epi>
-int logits(int cfg, const VhOperands& p, const Epi& e, hipStream_t s) {
-  if (cfg == kSmall) return launch<T, 64, 64, 4, 1, false, false>(p, 1, e, s);
-  if (cfg == kMid) return launch<T, 128, 64, 2, 2, false, false>(p, 1, e, s);
-  if constexpr (sizeof(T) == 2) return launch<T, 256, 256, 2, 4, false, false>(p, 1, e, s);
+int logits(LogitsTile t, const VhOperands& p, const Epi& e, hipStream_t s) {
+  // buffers: 16 rows, 4096 x 32000 bf16: 65.5 us with two, 63.3 with three, 56.1 with four; 128 x 64 tiles of bf16 alone on their
+  // CUs gain from a third (prompt of 777 rows: 357 -> 344 us), fp32 ones are long enough
+  if (t.bm == 64) return launch<T, 64, 64, 4, 1, false, false, 4>(p, 1, e, s);
+  if (t.bm == 128) return launch<T, 128, 64, 2, 2, false, false, sizeof(T) == 2 ? 3 : 2>(p, 1, e, s);
+  if constexpr (sizeof(T) == 2) {
+    if (t.bm == 192) return launch<T, 192, 256, 2, 4, false, false, 2>(p, 1, e, s);
+    if (t.bn == 128) return launch<T, 256, 128, 4, 2, false, false, 3>(p, 1, e, s);
+    return launch<T, 256, 256, 2, 4, false, false, 2>(p, 1, e, s);
+  }
   return -1;
+}
+// The same for all classes: e(kind, first class, first class tile) is the epilogue of a part
+template <typename T, class Make>
+int logits_all(const LogitsTiling& q, VhOperands p, const Make& make, hipStream_t s) {
+  const int classes = p.M;
+  for (int k = 0; k < 2; ++k) {
+    const int c0 = k ? q.first : 0;
+    p.M = k ? classes - q.first : q.first;
+    if (!p.M) continue;
+    const int rc = logits<T>(q.kind[k], p, make(k, c0, k ? q.tiles[0] : 0), s);
+    if (rc) return rc;
+    p.A = (const T*)p.A + (long)p.M * p.lda;
+  }
+  return 0;
 }
 // dh^T [hidden][rows] = w^T . d^T: the hidden units' side is slow
 template <typename T>
 int product_dh(int cfg, const VhOperands& p, int splits, const VhStore& e, hipStream_t s) {
-  if (cfg == kSmall) return launch<T, 128, 64, 4, 1, true, false>(p, splits, e, s);
-  if (cfg == kMid) return launch<T, 128, 64, 2, 2, true, false>(p, splits, e, s);
-  if constexpr (sizeof(T) == 2) return launch<T, 256, 256, 2, 4, true, false>(p, splits, e, s);
+  if (cfg == kSmall) return launch<T, 128, 64, 4, 1, true, false, 3>(p, splits, e, s);
+  if (cfg == kMid) return launch<T, 128, 64, 2, 2, true, false, 2>(p, splits, e, s);
+  if constexpr (sizeof(T) == 2) return launch<T, 256, 256, 2, 4, true, false, 2>(p, splits, e, s);
   return -1;
 }
 // dw^T [hidden][classes] = h^T . d: both sides slow
-template <typename T>
-int product_dw(int cfg, const VhOperands& p, int splits, const VhStore& e, hipStream_t s) {
+template <typename T, bool ONCE>
+int product_dw(int cfg, const VhOperands& p, int splits, const VhStoreT<ONCE>& e, hipStream_t s) {
   if (cfg == kLarge) {
-    if constexpr (sizeof(T) == 2) return launch<T, 256, 256, 2, 4, true, true>(p, splits, e, s);
+    if constexpr (sizeof(T) == 2) return launch<T, 256, 256, 2, 4, true, true, 2>(p, splits, e, s);
     return -1;
   }
-  return launch<T, 128, 64, 2, 2, true, true>(p, splits, e, s);
+  return launch<T, 128, 64, 2, 2, true, true, 2>(p, splits, e, s);
 }
 
 // Workgroups that share a tile's K range: where the tiles alone leave CUs idle, the range is cut so that about `want`
@@ -907,7 +986,7 @@ struct Plan {
   long d, sum_h, sum_w, dbpart;
   long total;
   long ldk, ldv;            // padded hidden units, classes of a piece
-  int cfg, piece, pieces, row_tiles, class_tiles, splits_h, splits_w;
+  int cfg, piece, pieces, splits_h, splits_w;
 };
 
 int esize(int dtype) { return dtype == 1 ? 2 : 4; }
@@ -937,20 +1016,19 @@ Plan plan_for(int dtype, int backward, long n, int H, int V, bool h_ok, bool w_o
   if (q.piece > V) q.piece = V;
   q.pieces = cdiv(V, q.piece);
   if (!w_ok) q.w_copy = take((long)q.piece * q.ldk * E);
-  q.class_tiles = cdiv(V, logits_bm(q.cfg));
-  q.row_tiles = cdiv(n, rows_bn(q.cfg));
   if (!backward) {
-    q.part = take((long)q.class_tiles * n * 8);
+    const LogitsTiling t = logits_tiling(q.cfg, n, V);
+    q.part = take((long)(t.tiles[0] + t.tiles[1]) * n * 8);
     q.zlab = take(n * 4);
   } else {
     const int KT = 128 / E, want = q.cfg == kSmall ? 768 : (q.cfg == kMid ? 768 : 256);
     q.ldv = up(q.piece, KT);
     q.d = take(n * q.ldv * E);
-    q.splits_h = splits_for((long)cdiv(H, hidden_bm(q.cfg)) * q.row_tiles, cdiv(q.ldv, KT), want);
+    q.splits_h = splits_for((long)cdiv(H, hidden_bm(q.cfg)) * cdiv(n, rows_bn(q.cfg)), cdiv(q.ldv, KT), want);
     q.splits_w = splits_for((long)cdiv(H, hidden_bm(q.cfg)) * cdiv(q.piece, classes_bn(q.cfg)), cdiv(n, KT), want);
     if (q.pieces > 1 || q.splits_h > 1) q.sum_h = take(q.splits_h * n * H * 4);
     if (q.splits_w > 1) q.sum_w = take(q.splits_w * (long)q.piece * H * 4);
-    if (bias) q.dbpart = take((long)q.row_tiles * q.ldv * 4);
+    if (bias) q.dbpart = take((long)cdiv(n, 64) * q.ldv * 4);      // at most that many row tiles
   }
   q.total = at ? at : 256;
   return q;
@@ -1000,11 +1078,13 @@ int forward(const void* h, long ldh, const void* w, long ldw, const float* bias,
     p.A = at<T>(ws, q.w_copy);
     p.lda = q.ldk;
   }
-  VhForward e{bias, labels, at<float2>(ws, q.part), at<float>(ws, q.zlab), n};
-  VH_TRY((logits<T>(q.cfg, p, e, s)));
+  const LogitsTiling t = logits_tiling(q.cfg, n, V);
+  VH_TRY(logits_all<T>(t, p, [&](int, int c0, int tile0) {
+    return VhForward{bias ? bias + c0 : nullptr, labels, c0, at<float2>(ws, q.part) + (long)tile0 * n, at<float>(ws, q.zlab), n};
+  }, s));
   const int per = n >= 2048 ? 16 : 1;
   hipLaunchKernelGGL((per == 16 ? vh_join<16> : vh_join<1>), dim3(cdiv(n, per)), dim3(256), 0, s, at<float2>(ws, q.part), (long)n,
-                     q.class_tiles, at<float>(ws, q.zlab), labels, n, V, ignore, (float*)loss, (float*)lse);
+                     t.tiles[0] + t.tiles[1], at<float>(ws, q.zlab), labels, n, V, ignore, (float*)loss, (float*)lse);
   return (int)hipGetLastError();
 }
 
@@ -1027,18 +1107,28 @@ int backward(const void* h, long ldh, const void* w, long ldw, const float* bias
       ldwp = q.ldk;
     }
     T* d = at<T>(ws, q.d);
-    VhGradLogits e{bias ? bias + v0 : nullptr, labels, lse, row_scale, grad_scale, v0, V, ignore, d, ldv,
-                   db ? at<float>(ws, q.dbpart) : nullptr};
-    VH_TRY((logits<T>(q.cfg, VhOperands{wp, hp, ldwp, q.ldk, vn, n, (int)q.ldk, (int)q.ldk, 0, 0, 0, 0}, e, s)));
-    if (db) {
-      hipLaunchKernelGGL(vh_dbias, dim3(cdiv(vn, 256)), dim3(256), 0, s, at<float>(ws, q.dbpart), ldv, q.row_tiles, (float*)db + v0, vn);
+    const LogitsTiling t = logits_tiling(q.cfg, n, vn);
+    VH_TRY(logits_all<T>(t, VhOperands{wp, hp, ldwp, q.ldk, vn, n, (int)q.ldk, (int)q.ldk, 0, 0, 0, 0}, [&](int, int c0, int) {
+      return VhGradLogits{bias ? bias + v0 + c0 : nullptr, labels, lse, row_scale, grad_scale, v0 + c0, V, ignore, d + c0, ldv, (int)ldv - c0,
+                          db ? at<float>(ws, q.dbpart) + c0 : nullptr};
+    }, s));
+    for (int part = 0; db && part < 2; ++part) {
+      const int c0 = part ? t.first : 0, cn = part ? vn - t.first : t.first;
+      if (!cn) continue;
+      hipLaunchKernelGGL(vh_dbias, dim3(cdiv(cn, 256)), dim3(256), 0, s, at<float>(ws, q.dbpart) + c0, ldv, cdiv(n, t.kind[part].bn),
+                         (float*)db + v0 + c0, cn);
       VH_TRY((int)hipGetLastError());
     }
     if (dw) {
       void* out = (char*)dw + (long)v0 * H * (dw_f32 ? 4 : E);
       const bool split = q.splits_w > 1;
-      VhStore st{out, H, dw_f32, 1, vn, split ? at<float>(ws, q.sum_w) : nullptr, 1, !split};
-      VH_TRY((product_dw<T>(q.cfg, VhOperands{hp, d, q.ldk, ldv, H, (int)ldv, n, n, 0, 0, 0, 0}, q.splits_w, st, s)));
+      // A large dw would only push other things out of the 256 MB cache (16 rows, 4096 x 32000: 90 us with plain stores, 62 with
+      // non-temporal ones); a small one stays for whoever reads it next.
+      const bool once = !split && (long)V * H * (dw_f32 ? 4 : E) >= (64L << 20);
+      const VhOperands o{hp, d, q.ldk, ldv, H, (int)ldv, n, n, 0, 0, 0, 0};
+      float* sum = split ? at<float>(ws, q.sum_w) : nullptr;
+      if (once) VH_TRY((product_dw<T>(q.cfg, o, 1, VhStoreT<true>{out, H, dw_f32, 1, vn, sum, 1, 1}, s)));
+      else VH_TRY((product_dw<T>(q.cfg, o, q.splits_w, VhStore{out, H, dw_f32, 1, vn, sum, 1, !split}, s)));
       if (split)
         VH_TRY(dw_f32 ? launch_sum(at<float>(ws, q.sum_w), (long)vn * H, q.splits_w, (float*)out, s)
                       : launch_sum(at<float>(ws, q.sum_w), (long)vn * H, q.splits_w, (T*)out, s));

@@ -208,6 +208,19 @@ def test_pieces_bias_ignored_rows_and_row_scales(gpu_lib, n, hidden, classes, pi
 
 
 @gpu
+@pytest.mark.parametrize("n,hidden,classes,piece", [
+    (300, 64, 32000, 0),        # 256 x 128 tiles
+    (1000, 40, 10007, 0),       # 192 x 256
+    (777, 64, 50001, 0),        # three rounds of 256 x 256, the other classes in small tiles
+    (2049, 72, 20011, 8192),    # pieces tiled differently
+    (130, 8, 70001, 0)])
+def test_every_tiling_of_the_logits(gpu_lib, n, hidden, classes, piece):
+    h, w, y, b = make(n, hidden, classes, "bf16", bias=True, ignored=0.1, seed=classes)
+    y[:4] = torch.tensor([classes - 1, classes - 2, 0, 255], dtype=torch.int32, device=DEV)
+    check_all(h, w, y, b, grad_scale=1.0 / n, piece=piece)
+
+
+@gpu
 @pytest.mark.parametrize("dtype", ["bf16", "fp32"])
 def test_strided_and_unaligned_rows(gpu_lib, dtype):
     h, w, y, b = make(70, 96, 400, dtype, bias=True, seed=4)
