@@ -20,7 +20,7 @@ from typing import List, Optional, Sequence, Tuple
 import torch
 
 from . import native
-from .native import check, ptr
+from .native import check, on_device, ptr
 
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
@@ -154,18 +154,15 @@ class GlobalNormClip:
         self.chunks, self._in_place = chunks, in_place.value
         self.slots = int(self.lib.dtf_clip_partials(chunks))    # fp64 words of a call's workspace
 
-    def _call(self):
+    def _buffers(self):
         dev = self.device
-        stream = torch.cuda.current_stream(dev).cuda_stream
-        part = torch.empty(self.slots, dtype=torch.float64, device=dev)
-        norm = torch.empty((), dtype=torch.float32, device=dev)
-        return stream, part, norm
+        return torch.empty(self.slots, dtype=torch.float64, device=dev), torch.empty((), dtype=torch.float32, device=dev)
 
     def norm(self, scale: float = 1.0) -> torch.Tensor:
         """``scale`` * norm of all tensors, an fp32 scalar on the device."""
         scale = _scale(scale)
-        with torch.cuda.device(self.device):
-            stream, part, norm = self._call()
+        with on_device(self.device) as stream:
+            part, norm = self._buffers()
             check(self.lib.dtf_global_norm(ptr(self.table), self.chunks, ptr(part), self.slots, scale, None, None, 0, 0.0,
                                            ptr(norm), stream), "global_norm")
         return norm
@@ -178,8 +175,8 @@ class GlobalNormClip:
             raise ValueError(f"clip_norm must be positive and finite, got {clip_norm}")
         if self._clip_error:
             raise ValueError(self._clip_error)
-        with torch.cuda.device(self.device):
-            stream, part, norm = self._call()
+        with on_device(self.device) as stream:
+            part, norm = self._buffers()
             check(self.lib.dtf_clip_by_global_norm(ptr(self.table), self.chunks, self._in_place, ptr(part), self.slots, scale,
                                                    clip_norm, ptr(norm), stream), "clip_by_global_norm")
         return self.out, norm

@@ -25,21 +25,23 @@ from typing import Optional, Tuple
 import torch
 
 from . import native
-from .native import check, ptr
+from .native import check, on_device, ptr
 
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1}
 _MAX_ROW = 1 << 20          # rows, hidden units and row strides of one call
 
 
-def _rows(t: torch.Tensor, name: str) -> int:
+def _rows(t: torch.Tensor, name: str, rows: int, cols: int) -> int:
     """Row stride (elements) of a matrix with contiguous rows."""
-    if t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1):
+    ld, inner = t.stride()
+    if inner != 1 and cols > 1:
         raise ValueError(f"{name} must be a matrix with contiguous rows, got shape {tuple(t.shape)}, strides {t.stride()}")
-    ld = max(t.stride(0), t.shape[1]) if t.shape[0] <= 1 else t.stride(0)
-    if ld < t.shape[1]:
+    if rows <= 1:
+        ld = max(ld, cols)
+    if ld < cols:
         raise ValueError(f"rows of {name} share memory (strides {t.stride()})")
-    if ld > _MAX_ROW or t.shape[1] > _MAX_ROW:
-        raise ValueError(f"rows of {name} may be at most {_MAX_ROW} elements long and apart, got {max(ld, t.shape[1])}")
+    if ld > _MAX_ROW:
+        raise ValueError(f"rows of {name} may be at most {_MAX_ROW} elements long and apart, got {ld}")
     return ld
 
 
@@ -53,25 +55,28 @@ def _vector(t: Optional[torch.Tensor], name: str, n: int, dtype: torch.dtype, de
 
 
 def _check(h, wT, labels, bias, ignore_label) -> Tuple[int, int, int, int, int]:
-    if h.dtype not in _DTYPES or wT.dtype != h.dtype:
-        raise TypeError(f"h and wT must both be bf16 or both fp32, got {h.dtype} and {wT.dtype}")
-    ldh, ldw = _rows(h, "h"), _rows(wT, "wT")
-    n, hidden = h.shape
-    classes = wT.shape[0]
-    if wT.shape[1] != hidden:
-        raise ValueError(f"h has {hidden} hidden units, wT {wT.shape[1]}")
+    dtype, dev = h.dtype, h.device
+    if dtype not in _DTYPES or wT.dtype != dtype:
+        raise TypeError(f"h and wT must both be bf16 or both fp32, got {dtype} and {wT.dtype}")
+    for t, name in ((h, "h"), (wT, "wT")):
+        if t.dim() != 2:
+            raise ValueError(f"{name} must be a matrix with contiguous rows, got shape {tuple(t.shape)}")
+    (n, hidden), (classes, width) = h.shape, wT.shape
+    ldh, ldw = _rows(h, "h", n, hidden), _rows(wT, "wT", classes, width)
+    if width != hidden:
+        raise ValueError(f"h has {hidden} hidden units, wT {width}")
     if hidden < 1 or not 1 <= classes < 1 << 30:
         raise ValueError(f"at least one hidden unit and 1 to 2^30 - 1 classes expected, got wT {tuple(wT.shape)}")
     if n > _MAX_ROW:
         raise ValueError(f"at most {_MAX_ROW} rows per call, got {n}")
-    if wT.device != h.device:
-        raise ValueError(f"wT is on {wT.device}, the hidden rows on {h.device}")
-    _vector(labels, "labels", n, torch.int32, h.device)
-    _vector(bias, "bias", classes, torch.float32, h.device)
+    if wT.device != dev:
+        raise ValueError(f"wT is on {wT.device}, the hidden rows on {dev}")
+    _vector(labels, "labels", n, torch.int32, dev)
+    _vector(bias, "bias", classes, torch.float32, dev)
     if not -(1 << 31) <= ignore_label < 1 << 31:
         raise ValueError(f"ignore_label must be an int32, got {ignore_label}")
-    if h.device.type != "cuda":
-        raise ValueError(f"GPU tensors expected, got {h.device} (ops.reference.softmax_cross_entropy_with_logits runs on the CPU)")
+    if dev.type != "cuda":
+        raise ValueError(f"GPU tensors expected, got {dev} (ops.reference.softmax_cross_entropy_with_logits runs on the CPU)")
     return n, hidden, classes, ldh, ldw
 
 
@@ -80,13 +85,11 @@ def vocab_head_fwd(h: torch.Tensor, wT: torch.Tensor, labels: torch.Tensor, bias
     """(loss_rows, lse), fp32 [n]: per-row cross-entropy and the logarithm of the sum of exponentials of the logits (what the
     backward pass needs)."""
     n, hidden, classes, ldh, ldw = _check(h, wT, labels, bias, ignore_label)
-    loss = torch.empty(n, dtype=torch.float32, device=h.device)
-    lse = torch.empty(n, dtype=torch.float32, device=h.device)
+    loss, lse = torch.empty((2, n), dtype=torch.float32, device=h.device)
     if n == 0:
         return loss, lse
     lib, dt = native.load(), _DTYPES[h.dtype]
-    with torch.cuda.device(h.device):
-        stream = torch.cuda.current_stream(h.device).cuda_stream
+    with on_device(h.device) as stream:
         need = lib.dtf_vocab_head_workspace(dt, 0, ptr(h), ldh, ptr(wT), ldw, n, hidden, classes, int(bias is not None), 0)
         check(min(need, 0), "vocab_head_workspace")
         ws = torch.empty(need, dtype=torch.uint8, device=h.device)
@@ -144,8 +147,7 @@ def vocab_head_bwd(h: torch.Tensor, wT: torch.Tensor, labels: torch.Tensor, lse:
                 t.zero_()
         return dh, dwT, dbias
     lib, dt = native.load(), _DTYPES[h.dtype]
-    with torch.cuda.device(dev):
-        stream = torch.cuda.current_stream(dev).cuda_stream
+    with on_device(dev) as stream:
         need = lib.dtf_vocab_head_workspace(dt, 1, ptr(h), ldh, ptr(wT), ldw, n, hidden, classes, int(dbias is not None), piece)
         check(min(need, 0), "vocab_head_workspace")
         ws = torch.empty(need, dtype=torch.uint8, device=dev)
