@@ -370,6 +370,21 @@ __device__ __forceinline__ void vh_mainloop(const VhOperands& p, Tile& c, char* 
   vh_barrier();
 }
 
+// Which tile and which split a workgroup takes.  Workgroups are dealt round-robin over the 8 XCDs; each XCD gets one run of the
+// (split, band of four tile rows, column) order, so that its L2 serves all tiles of a split from one fetch of the split's
+// operands.
+__device__ __forceinline__ int vh_assign(int L, int gx, int gy, int splits, int& tx, int& ty) {
+  constexpr int NX = 8, BH = 4;
+  const int tiles = gx * gy, total = tiles * splits, xcd = L % NX, q = total / NX, r = total % NX;
+  int idx = xcd * q + min(xcd, r) + L / NX;
+  const int split = idx / tiles;
+  idx -= split * tiles;
+  const int band = idx / (BH * gx), rem = idx - band * BH * gx, h = min(BH, gy - band * BH);
+  tx = rem / h;
+  ty = band * BH + rem % h;
+  return split;
+}
+
 template <typename T, int BM, int BN, int NWM, int NWN, bool AS, bool BS, int D, class Epi>
 __global__ __launch_bounds__(NWM * NWN * 64, 1) void vh_gemm(VhOperands p, Epi e) {
   typedef VhTile<T, BM, BN, NWM, NWN> Tile;
@@ -383,10 +398,8 @@ __global__ __launch_bounds__(NWM * NWN * 64, 1) void vh_gemm(VhOperands p, Epi e
   c.wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   c.wm0 = (c.wave / NWN) * Tile::WM;
   c.wn0 = (c.wave % NWN) * Tile::WN;
-  const int tiles = p.tiles_m * p.tiles_n;
   int tx, ty;
-  xcd_tile_linear(blockIdx.x % tiles, p.tiles_m, p.tiles_n, tx, ty);
-  c.split = blockIdx.x / tiles;
+  c.split = vh_assign(blockIdx.x, p.tiles_m, p.tiles_n, p.splits, tx, ty);
   c.m0 = tx * BM;
   c.n0 = ty * BN;
   const int per = (p.ktiles + p.splits - 1) / p.splits, t0 = c.split * per;
@@ -530,8 +543,10 @@ struct VhForward {
   }
 };
 
-// Backward, first product: i = class (relative to the piece), j = row.  d[row][vh_place(class)] in the operand
-// type, places up to ldd (a multiple of the K tile) written as zeros; dbias partial sums per row tile from the values before rounding.
+// Backward, first product: i = class (relative to the piece), j = row.  d[row][vh_place(class)], places up to ldd (a multiple
+// of the K tile) written as zeros; dbias partial sums per row tile from the values before rounding.  d is rounded to the operand
+// type because the two products that read it multiply in that type (at most half a step of each value, sums in fp32); kept in
+// fp32 it would be rounded there all the same, after twice the traffic.
 struct VhGradLogits {
   const float* bias;        // of the piece
   const int* labels;
@@ -633,9 +648,9 @@ struct VhGradLogits {
 };
 
 // Plain product: out[j][i], j < rows, in the operand type or fp32; the product's j is a place of d where by_place is set
-// (its N is then the number of places).  With sum: fp32 [split][rows][M] running sums over the pieces of the classes, read unless `first` and written unless `last` (a single split:
-// the last piece's result goes to out).  ONCE: the result is not to be kept in the caches (a template argument: as a value the
-// compiler folds the two kinds of stores into the plain one).
+// (its N is then the number of places).  With sum: fp32 [split][rows][M] running sums over the pieces of the classes, read
+// unless `first` and written unless `last` (a single split: the last piece's result goes to out).  ONCE: the result is not to
+// be kept in the caches (a template argument: as a value the compiler folds the two kinds of stores into the plain one).
 template <bool ONCE>
 struct VhStoreT {
   void* out;
@@ -813,26 +828,27 @@ __global__ __launch_bounds__(256) void vh_copy(const T* __restrict__ src, long l
   }
 }
 
-// out[i] = sum of the splits' slabs, in order
+// out[i] = sum of the splits' slabs, in order, eight loads in flight
 template <typename O>
 __global__ __launch_bounds__(256) void vh_sum(const float* __restrict__ part, long n, int splits, O* __restrict__ out) {
   const long i = ((long)blockIdx.x * 256 + threadIdx.x) * 4;
-  if (i >= n) return;
-  if (!(n & 3)) {
-    f32x4 s = *reinterpret_cast<const f32x4*>(part + i);
+  if (i + 4 <= n) {
+    const float* p = part + i;
+    f32x4 s = *reinterpret_cast<const f32x4_any*>(p);
     int k = 1;
-    for (; k + 4 <= splits; k += 4) {
-      f32x4 v[4];
+    for (; k + 8 <= splits; k += 8) {
+      f32x4 v[8];
 #pragma unroll
-      for (int u = 0; u < 4; ++u) v[u] = *reinterpret_cast<const f32x4*>(part + (k + u) * n + i);
+      for (int u = 0; u < 8; ++u) v[u] = *reinterpret_cast<const f32x4_any*>(p + (k + u) * n);
 #pragma unroll
-      for (int u = 0; u < 4; ++u) s += v[u];
+      for (int u = 0; u < 8; ++u) s += v[u];
     }
-    for (; k < splits; ++k) s += *reinterpret_cast<const f32x4*>(part + k * n + i);
+#pragma unroll 4
+    for (; k < splits; ++k) s += *reinterpret_cast<const f32x4_any*>(p + k * n);
     typedef __attribute__((ext_vector_type(4))) O O4;
     *reinterpret_cast<O4*>(out + i) = (O4){(O)s[0], (O)s[1], (O)s[2], (O)s[3]};
   } else {
-    for (long j = i; j < n && j < i + 4; ++j) {
+    for (long j = i; j < n; ++j) {
       float s = part[j];
       for (int k = 1; k < splits; ++k) s += part[k * n + j];
       out[j] = (O)s;
@@ -857,18 +873,37 @@ constexpr int kPiece = 256;           // pieces are multiples of this many class
 //   kMid:   up to 128 rows, and fp32: 128 x 64 tiles of four waves, three workgroups per CU (fp32, 1024 x 1024 x 10000: forward
 //           198 us with 128 x 128 tiles, whose 640 do not divide evenly over the CUs, 174 us with these; 4096 x 1024 x 16000: 969
 //           and 976).
-//   kLarge: 256 x 256 tiles of eight waves, one workgroup per CU.
+//   kLarge: 256 x 256 tiles of eight waves, one workgroup per CU -- or 128 x 128 tiles of four, two per CU, where the large
+//           ones leave CUs idle.
 enum { kSmall, kMid, kLarge };
 int config_for(int E, long n) { return n <= 64 ? kSmall : (E == 4 || n <= 128 ? kMid : kLarge); }
-constexpr int rows_bn(int cfg) { return cfg == kLarge ? 256 : 64; }         // of dh
-constexpr int hidden_bm(int cfg) { return cfg == kLarge ? 256 : 128; }      // of dh and dw
-constexpr int classes_bn(int cfg) { return cfg == kLarge ? 256 : 64; }      // of dw
+
+// Tiles of the gradient products
+struct GradTile {
+  int bm, bn;             // hidden units; rows (dh) or classes (dw)
+  int want;               // workgroups that fill the card
+};
+constexpr GradTile kTiles256{256, 256, 256}, kTiles128{128, 128, 512}, kTiles64{128, 64, 768};
+// dh is cut along the classes into as many slabs as it takes to fill the card, so what many large tiles save in operand reads
+// few of them lose in slabs: 16 tiles (1000 rows, 1000 x 10007) 42 us against 33 with the small ones, 24 (1500 rows) 55 and 45,
+// 32 (4000 rows, 512 x 30000) 139 and 160, 64 (777 rows, 4096 x 50001) 342 and 364.
+GradTile dh_tile(int cfg, long n, int H) {
+  if (cfg != kLarge) return kTiles64;
+  return (long)cdiv(H, 256) * cdiv(n, 256) < 32 ? kTiles128 : kTiles256;
+}
+// dw has its classes to fill the card: rounds over it times their length, 0.57 of a large tile's for two small ones per CU.
+// 316 large tiles are two rounds (700 rows, 1024 x 20000: 47 us, small ones 40), 252 are one (500 rows, 1000 x 16000: 23 and 26).
+GradTile dw_tile(int cfg, int H, int classes) {
+  if (cfg != kLarge) return kTiles64;
+  const long large = (long)cdiv(H, 256) * cdiv(classes, 256), small = (long)cdiv(H, 128) * cdiv(classes, 128);
+  return 0.57 * cdiv(small, 512) < cdiv(large, 256) ? kTiles128 : kTiles256;
+}
 
 // How the logits product of some classes is tiled: the classes below `first` in tiles of one kind, the others in a second one.
 // The large kinds run one workgroup per CU, so what counts is the number of rounds over the 256 CUs times the length of a round
 // (measured at H = 4096, against 256 x 256: 0.82 for 192 x 256, 0.68 for 256 x 128), and a last round for a few tiles is as long
 // as any other: its classes go to small tiles instead.  777 rows x 50001 classes: 784 tiles are four rounds, 362 us; three
-// rounds and 91 small tiles 299 us.
+// rounds and 91 small tiles 330 us.
 struct LogitsTile {
   int bm, bn;
 };
@@ -952,18 +987,20 @@ int logits_all(const LogitsTiling& q, VhOperands p, const Make& make, hipStream_
 }
 // dh^T [hidden][rows] = w^T . d^T: the hidden units' side is slow
 template <typename T>
-int product_dh(int cfg, const VhOperands& p, int splits, const VhStore& e, hipStream_t s) {
+int product_dh(int cfg, const GradTile& t, const VhOperands& p, int splits, const VhStore& e, hipStream_t s) {
   if (cfg == kSmall) return launch<T, 128, 64, 4, 1, true, false, 3>(p, splits, e, s);
-  if (cfg == kMid) return launch<T, 128, 64, 2, 2, true, false, 2>(p, splits, e, s);
-  if constexpr (sizeof(T) == 2) return launch<T, 256, 256, 2, 4, true, false, 2>(p, splits, e, s);
-  return -1;
+  if constexpr (sizeof(T) == 2) {
+    if (t.bn == 256) return launch<T, 256, 256, 2, 4, true, false, 2>(p, splits, e, s);
+    if (t.bn == 128) return launch<T, 128, 128, 2, 2, true, false, 2>(p, splits, e, s);
+  }
+  return launch<T, 128, 64, 2, 2, true, false, 2>(p, splits, e, s);
 }
 // dw^T [hidden][classes] = h^T . d: both sides slow
 template <typename T, bool ONCE>
-int product_dw(int cfg, const VhOperands& p, int splits, const VhStoreT<ONCE>& e, hipStream_t s) {
-  if (cfg == kLarge) {
-    if constexpr (sizeof(T) == 2) return launch<T, 256, 256, 2, 4, true, true, 2>(p, splits, e, s);
-    return -1;
+int product_dw(const GradTile& t, const VhOperands& p, int splits, const VhStoreT<ONCE>& e, hipStream_t s) {
+  if constexpr (sizeof(T) == 2) {
+    if (t.bn == 256) return launch<T, 256, 256, 2, 4, true, true, 2>(p, splits, e, s);
+    if (t.bn == 128) return launch<T, 128, 128, 2, 2, true, true, 2>(p, splits, e, s);
   }
   return launch<T, 128, 64, 2, 2, true, true, 2>(p, splits, e, s);
 }
@@ -987,6 +1024,7 @@ struct Plan {
   long total;
   long ldk, ldv;            // padded hidden units, classes of a piece
   int cfg, piece, pieces, splits_h, splits_w;
+  GradTile tile_h, tile_w;
 };
 
 int esize(int dtype) { return dtype == 1 ? 2 : 4; }
@@ -1021,11 +1059,13 @@ Plan plan_for(int dtype, int backward, long n, int H, int V, bool h_ok, bool w_o
     q.part = take((long)(t.tiles[0] + t.tiles[1]) * n * 8);
     q.zlab = take(n * 4);
   } else {
-    const int KT = 128 / E, want = q.cfg == kSmall ? 768 : (q.cfg == kMid ? 768 : 256);
+    const int KT = 128 / E;
     q.ldv = up(q.piece, KT);
     q.d = take(n * q.ldv * E);
-    q.splits_h = splits_for((long)cdiv(H, hidden_bm(q.cfg)) * cdiv(n, rows_bn(q.cfg)), cdiv(q.ldv, KT), want);
-    q.splits_w = splits_for((long)cdiv(H, hidden_bm(q.cfg)) * cdiv(q.piece, classes_bn(q.cfg)), cdiv(n, KT), want);
+    q.tile_h = dh_tile(q.cfg, n, H);
+    q.tile_w = dw_tile(q.cfg, H, q.piece);
+    q.splits_h = splits_for((long)cdiv(H, q.tile_h.bm) * cdiv(n, q.tile_h.bn), cdiv(q.ldv, KT), q.tile_h.want);
+    q.splits_w = splits_for((long)cdiv(H, q.tile_w.bm) * cdiv(q.piece, q.tile_w.bn), cdiv(n, KT), q.tile_w.want);
     if (q.pieces > 1 || q.splits_h > 1) q.sum_h = take(q.splits_h * n * H * 4);
     if (q.splits_w > 1) q.sum_w = take(q.splits_w * (long)q.piece * H * 4);
     if (bias) q.dbpart = take((long)cdiv(n, 64) * q.ldv * 4);      // at most that many row tiles
@@ -1127,8 +1167,8 @@ int backward(const void* h, long ldh, const void* w, long ldw, const float* bias
       const bool once = !split && (long)V * H * (dw_f32 ? 4 : E) >= (64L << 20);
       const VhOperands o{hp, d, q.ldk, ldv, H, (int)ldv, n, n, 0, 0, 0, 0};
       float* sum = split ? at<float>(ws, q.sum_w) : nullptr;
-      if (once) VH_TRY((product_dw<T>(q.cfg, o, 1, VhStoreT<true>{out, H, dw_f32, 1, vn, sum, 1, 1}, s)));
-      else VH_TRY((product_dw<T>(q.cfg, o, q.splits_w, VhStore{out, H, dw_f32, 1, vn, sum, 1, !split}, s)));
+      if (once) VH_TRY((product_dw<T>(q.tile_w, o, 1, VhStoreT<true>{out, H, dw_f32, 1, vn, sum, 1, 1}, s)));
+      else VH_TRY((product_dw<T>(q.tile_w, o, q.splits_w, VhStore{out, H, dw_f32, 1, vn, sum, 1, !split}, s)));
       if (split)
         VH_TRY(dw_f32 ? launch_sum(at<float>(ws, q.sum_w), (long)vn * H, q.splits_w, (float*)out, s)
                       : launch_sum(at<float>(ws, q.sum_w), (long)vn * H, q.splits_w, (T*)out, s));
@@ -1136,7 +1176,7 @@ int backward(const void* h, long ldh, const void* w, long ldw, const float* bias
     if (dh) {
       const bool last = k == q.pieces - 1, split = q.splits_h > 1;
       VhStore st{dh, H, 0, 0, n, q.sum_h ? at<float>(ws, q.sum_h) : nullptr, k == 0, last && !split};
-      VH_TRY((product_dh<T>(q.cfg, VhOperands{wp, d, ldwp, ldv, H, n, vn, (int)ldv, 0, 0, 0, 0}, q.splits_h, st, s)));
+      VH_TRY((product_dh<T>(q.cfg, q.tile_h, VhOperands{wp, d, ldwp, ldv, H, n, vn, (int)ldv, 0, 0, 0, 0}, q.splits_h, st, s)));
       if (last && split) VH_TRY(launch_sum(at<float>(ws, q.sum_h), (long)n * H, q.splits_h, (T*)dh, s));
     }
   }

@@ -221,6 +221,18 @@ def test_every_tiling_of_the_logits(gpu_lib, n, hidden, classes, piece):
 
 
 @gpu
+@pytest.mark.parametrize("n,hidden,classes", [
+    (1100, 1800, 8000),         # dh and dw in 256 x 256 tiles
+    (1100, 1800, 18011),        # dw in 128 x 128 tiles
+    (300, 600, 40003),          # dh in 128 x 128 tiles and slabs
+    (700, 1000, 20011),         # both in 128 x 128 tiles
+    (1030, 2050, 4100)])        # a few rows, hidden units and classes over
+def test_every_tiling_of_the_gradients(gpu_lib, n, hidden, classes):
+    h, w, y, b = make(n, hidden, classes, "bf16", bias=True, ignored=0.1, seed=hidden)
+    check_all(h, w, y, b, grad_scale=1.0 / n)
+
+
+@gpu
 @pytest.mark.parametrize("dtype", ["bf16", "fp32"])
 def test_strided_and_unaligned_rows(gpu_lib, dtype):
     h, w, y, b = make(70, 96, 400, dtype, bias=True, seed=4)
