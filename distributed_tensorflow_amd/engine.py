@@ -459,7 +459,8 @@ class HipEngine:
                             adam_slot: int = 3):
         """Optimizer over arena floats [lo, hi) (+ bf16 shadow).  ``advance`` bumps the sample cursor,
         global_step and dropout offset (exactly one range per step does that); every range keeps its
-        own Adam step counter (state[adam_slot]) so ranges may be updated from different streams."""
+        own Adam step counter (state[adam_slot]) so ranges may be updated from different streams.  With clip_norm the
+        update uses the factor of the last launch_clip() (before the first one it is zero: nothing moves)."""
         check(self.lib.dtf_engine_update_range(self._d(), lo, hi, int(advance), int(advance_cursor), self.step_inc,
                                                adam_slot, self._s()), "update_range")
 

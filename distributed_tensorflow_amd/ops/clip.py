@@ -8,7 +8,8 @@ The plan is made once for tensors that stay where they are (gradient arenas, as 
 nothing but a table of their addresses and shapes in device memory; each call computes the norm anew from the values that
 the tensors then have.  Launches go to the current stream of the tensors' device and can be captured into a HIP graph (the
 plan has to outlive it): the table is only read, the workspace of a call comes from PyTorch's allocator on that stream, so
-calls on different streams and in different graphs share nothing that is written.  As in TensorFlow, a norm that is not finite makes every clipped value NaN.
+calls on different streams and in different graphs share nothing that is written.  As in TensorFlow, a norm that is not
+finite makes every clipped value NaN.
 Kernels: csrc/kernels/clip.hip.
 """
 from __future__ import annotations

@@ -13,8 +13,10 @@ A row whose label is ``ignore_label`` has loss 0 and takes no part in any gradie
 (padding); any other label outside the classes makes its loss, and with it every gradient it enters, NaN, as
 ``tf.nn.sparse_softmax_cross_entropy_with_logits`` does on a GPU.  A class can be masked by a bias of -inf.
 
-The backward pass computes the logits again, one piece of the classes at a time: its workspace holds two copies of the
-piece's bf16 / fp32 gradient of the logits and one of its weights.  Calls launch on the current stream of the operands'
+The backward pass computes the logits again, one piece of the classes at a time: its workspace holds the gradient of the
+piece's logits in the operands' type (at most 2^27 values, or 1024 classes of very many rows), a copy of ``h`` without its
+ignored rows, fp32 sums of ``dh`` where there are several pieces or the classes are cut among workgroups, and copies of rows
+that do not start on 16 bytes.  Calls launch on the current stream of the operands'
 device, take their workspace from PyTorch's allocator on that stream and keep nothing, so they can be captured into HIP
 graphs and run on several streams at once.  Kernels: csrc/kernels/vocab_head.hip.
 """
@@ -37,7 +39,7 @@ def _rows(t: torch.Tensor, name: str, rows: int, cols: int) -> int:
     if inner != 1 and cols > 1:
         raise ValueError(f"{name} must be a matrix with contiguous rows, got shape {tuple(t.shape)}, strides {t.stride()}")
     if rows <= 1:
-        ld = max(ld, cols)
+        ld = cols               # the stride of a single row says nothing
     if ld < cols:
         raise ValueError(f"rows of {name} share memory (strides {t.stride()})")
     if ld > _MAX_ROW:

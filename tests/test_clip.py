@@ -88,7 +88,7 @@ LISTS = [
     ([(0,), (5,), (0, 3)], [B, F, H]),
     ([(1023,), (4097,), (33, 65)], [F, B, H]),
     ([(3136, 1024), (1024, 10), (10,), (1024,), (5, 5, 32, 64), (64,), (5, 5, 1, 32), (32,)], [F] * 8),
-    ([(7,)] * 150 + [(2049,)] * 50, [B, F] * 100),          # more tensors than one launch's table holds
+    ([(7,)] * 150 + [(2049,)] * 50, [B, F] * 100),          # many small tensors
     ([(1 << 22,), (3,)], [B, F]),
 ]
 

@@ -399,6 +399,52 @@ def test_offsets_beyond_32_bits(gpu_lib):
     torch.cuda.empty_cache()
 
 
+@gpu
+def test_offsets_beyond_32_bits_many_rows(gpu_lib):
+    """The same for rows enough to run the large tiles: all classes but the last two have a weight of zero, so every row's
+    log-sum-exp is log(classes - 2 + exp(z_a) + exp(z_b)); the gradient's rows of those two, and of one in the middle."""
+    n, hidden, classes = 200, 4096, 600_000
+    g = torch.Generator(device=DEV).manual_seed(5)
+    w = torch.zeros((classes, hidden), dtype=torch.bfloat16, device=DEV)
+    w[-2:] = (torch.randn((2, hidden), device=DEV, generator=g) * 0.05).bfloat16()
+    h = torch.randn((n, hidden), device=DEV, generator=g).bfloat16()
+    y = torch.where(torch.arange(n, device=DEV) % 2 == 0, classes - 1, 300_001).to(torch.int32)
+    loss, lse = vocab_head_fwd(h, w, y)
+    hd = h.double()
+    z = hd @ w[-2:].double().t()
+    want = torch.log(torch.exp(z).sum(1) + (classes - 2))
+    e_z = 8 * math.sqrt(hidden + 64) * U * (hd.abs() @ w[-2:].double().abs().t())
+    e_lse = e_z.max(1).values + 8 * U * (1 + want)
+    within(lse, want, e_lse, "lse")
+    within(loss, torch.where(y == classes - 1, want - z[:, 1], want), 2 * e_lse + 8 * U * z.abs().sum(1), "loss")
+    dh, dw, _ = vocab_head_bwd(h, w, y, lse)
+    half = half_step(torch.bfloat16)
+    cols = torch.stack([torch.exp(-want), torch.exp(z[:, 0] - want), torch.exp(z[:, 1] - want)], 1)
+    hit = torch.stack([y == 300_001, y == classes - 2, y == classes - 1], 1).double()
+    d = cols - hit
+    e_d = cols * (2 * e_lse + 8 * U * (1 + want))[:, None] + 2 * U + half * d.abs()
+    got = d.t() @ hd
+    e = (e_d + 8 * math.sqrt(n) * U * d.abs()).t() @ hd.abs()
+    within(dw[[300_001, classes - 2, classes - 1]], got, e + half * (got.abs() + e), "dw")
+    # dh: only the last two classes' weights are not zero
+    d, e_d = d[:, 1:], e_d[:, 1:] + 8 * math.sqrt(classes) * U * d[:, 1:].abs()
+    got, e = d @ w[-2:].double(), e_d @ w[-2:].double().abs()
+    within(dh, got, e + half * (got.abs() + e), "dh")
+    del w, dw
+    torch.cuda.empty_cache()
+
+
+@gpu
+def test_stride_of_a_single_row_says_nothing(gpu_lib):
+    big = torch.zeros((2, (1 << 20) + 64), device=DEV)
+    h, w, y, _ = make(1, 32, 90, "fp32", seed=2)
+    big[0, :32] = h[0]
+    view = big[:1, :32]
+    assert view.stride(0) > 1 << 20
+    assert torch.equal(vocab_head_fwd(view, w, y)[1], vocab_head_fwd(h, w, y)[1])
+    assert torch.equal(vocab_head_fwd(h, view, torch.zeros_like(y))[1], vocab_head_fwd(h, h, torch.zeros_like(y))[1])
+
+
 # ---------------------------------------------------------------------------------------------- streams and graphs
 @gpu
 def test_graph_replays_and_streams(gpu_lib):
