@@ -804,27 +804,34 @@ __global__ __launch_bounds__(256) void vh_dbias(const float* __restrict__ part, 
 }
 
 // dst[r][c] = src[r][c] with rows ldd apart (16-byte multiples), columns C .. ldd - 1 zero.  labels given: the rows of
-// ignored labels are zero as well -- whatever lies there, 0 * NaN must not reach a gradient.  V elements per access.
-template <typename T, int V>
+// ignored labels are zero as well -- whatever lies there, 0 * NaN must not reach a gradient.  Whole 16-byte chunks from any
+// element of a row (global memory takes unaligned vector loads), the last chunk of a row element by element.
+template <typename T>
 __global__ __launch_bounds__(256) void vh_copy(const T* __restrict__ src, long lds_, int R, int C, T* __restrict__ dst, long ldd,
                                                const int* __restrict__ labels, int ignore) {
+  constexpr int V = 16 / sizeof(T);
   typedef __attribute__((ext_vector_type(V))) T vec;
+  typedef vec vec_any __attribute__((aligned(sizeof(T))));
   const int per = (int)(ldd / V);
-  for (int r = blockIdx.y; r < R; r += gridDim.y) {
-    const bool keep = !(labels && labels[r] == ignore);
-    for (int i = blockIdx.x * 256 + threadIdx.x; i < per; i += gridDim.x * 256) {
-      vec v;
+  const long n = (long)R * per;
+  for (long x = (long)blockIdx.x * 256 + threadIdx.x; x < n; x += (long)gridDim.x * 256) {
+    const long r = n >> 32 ? x / per : (long)((unsigned)x / (unsigned)per);
+    const int i = (int)(x - r * per) * V;
+    vec v;
 #pragma unroll
-      for (int e = 0; e < V; ++e) v[e] = (T)0.f;
-      if (keep) {
-        if constexpr (V == 1) {
-          if (i < C) v[0] = src[r * lds_ + i];
-        } else {
-          v = *reinterpret_cast<const vec*>(src + r * lds_ + (long)i * V);      // (C is a multiple of V)
-        }
+    for (int e = 0; e < V; ++e) v[e] = (T)0.f;
+    if (!(labels && labels[r] == ignore)) {
+      const T* p = src + r * lds_ + i;
+      if (i + V <= C) {
+        const vec y = *reinterpret_cast<const vec_any*>(p);
+        v = y;
+      } else {
+#pragma unroll
+        for (int e = 0; e < V; ++e)
+          if (i + e < C) v[e] = p[e];
       }
-      *reinterpret_cast<vec*>(dst + r * ldd + (long)i * V) = v;
     }
+    *reinterpret_cast<vec*>(dst + r * ldd + i) = v;
   }
 }
 
@@ -1080,13 +1087,10 @@ T* at(void* ws, long o) { return (T*)((char*)ws + o - 1); }
 bool rows_ok(const void* p, long ld, int H, int E) { return !((uintptr_t)p & 15) && !(ld * E & 15) && !((long)H * E & 15); }
 
 template <typename T>
-int launch_copy(const T* src, long lds, int R, int C, T* dst, long ldd, const int* labels, int ignore, hipStream_t s) {
-  constexpr int V = 16 / sizeof(T);
-  const bool ok = rows_ok(src, lds, C, sizeof(T));
-  const int x = cdiv(ok ? ldd / V : ldd, 256);
-  const dim3 grid(x > 64 ? 64 : x, R > 16384 ? 16384 : R);
-  if (ok) hipLaunchKernelGGL((vh_copy<T, V>), grid, dim3(256), 0, s, src, lds, R, C, dst, ldd, labels, ignore);
-  else hipLaunchKernelGGL((vh_copy<T, 1>), grid, dim3(256), 0, s, src, lds, R, C, dst, ldd, labels, ignore);
+int launch_copy(const T* src, long lds_, int R, int C, T* dst, long ldd, const int* labels, int ignore, hipStream_t s) {
+  const long chunks = (long)R * (ldd * (long)sizeof(T) / 16);
+  const int grid = chunks > 16384L * 256 ? 16384 : cdiv(chunks, 256);
+  hipLaunchKernelGGL(vh_copy<T>, dim3(grid), dim3(256), 0, s, src, lds_, R, C, dst, ldd, labels, ignore);
   return (int)hipGetLastError();
 }
 template <typename O>
