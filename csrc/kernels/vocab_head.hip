@@ -544,18 +544,21 @@ struct VhForward {
 };
 
 // Backward, first product: i = class (relative to the piece), j = row.  d[row][vh_place(class)], places up to ldd (a multiple
-// of the K tile) written as zeros; dbias partial sums per row tile from the values before rounding.  d is rounded to the operand
-// type because the two products that read it multiply in that type (at most half a step of each value, sums in fp32); kept in
-// fp32 it would be rounded there all the same, after twice the traffic.
+// of the K tile) written as zeros; dbias partial sums per row tile from the values before rounding.
+// d is rounded to the operand type because the two products that read it multiply in that type: at most half a step of each
+// value, summed in fp32.  The common factor grad_scale is left to those products' epilogues: 1/n times a label's -(1 - p), the
+// value that outweighs all others of its row and class, would be rounded the same way for every row.  With up to 32 rows, half
+// a tile of them, the rounding errors themselves are kept as n more rows, next to nothing in time: one row's gradient is then as
+// exact as if d had stayed in fp32 (one row: 0.17 % rms, the operand type's own rounding, instead of up to 0.4; 16 rows, 4096 x
+// 32000, backward 161 -> 166 us.  For 64 rows, a second tile, it would be 168 -> 211 us, and errors of many rows even out.)
 struct VhGradLogits {
   const float* bias;        // of the piece
   const int* labels;
   const float* lse;
   const float* row_scale;   // or nullptr
-  float grad_scale;
   int v0, classes, ignore;  // the product's first class, all classes
   void* d;
-  long ldd;
+  long ldd, rest;           // elements from a row to the row of its rounding errors (0: not kept)
   int places;               // of this product's classes: up to there d is written
   float* dbpart;            // [row tile][ldd] or nullptr
   template <int BM, int BN> using Inputs = VhLogitsInputs<BM, BN>;
@@ -563,7 +566,7 @@ struct VhGradLogits {
     const int y = labels[row];
     if (y == ignore) return {-1, 0.f, 0.f};
     const bool known = y >= 0 && y < classes;
-    const float sc = row_scale ? grad_scale * row_scale[row] : grad_scale;
+    const float sc = row_scale ? row_scale[row] : 1.f;
     // (a label that is no class: the whole row says so)
     return {known && y >= v0 ? y - v0 - m0 : -1, lse[row] * kLog2e, known ? sc : __builtin_nanf("")};
   }
@@ -578,6 +581,8 @@ struct VhGradLogits {
   template <typename T, int BM, int BN, int NWM, int NWN, class Tile>
   __device__ __forceinline__ void run(const VhOperands& p, Tile& c, int, int ty, char* lds, const Inputs<BM, BN>& in) const {
     constexpr int MT = Tile::MT, NTL = Tile::NTL;
+    constexpr bool REST = sizeof(T) == 2 && BM == 64;        // (the few rows' tiles)
+    static_assert(!REST || MT % 2, "the single-fragment branch stores the errors");
     const int i16 = c.lane & 15, g = c.lane >> 4;
     const int mw = c.m0 + c.wm0 + 4 * g;
     vh_add_bias(c, in, bias != nullptr, p.M);
@@ -621,7 +626,11 @@ struct VhGradLogits {
             const int m = mw + 16 * i;
             const f32x4 v = c.acc[i][j];
             const T4 y = {(T)v[0], (T)v[1], (T)v[2], (T)v[3]};
-            if (m < places) *reinterpret_cast<T4*>(o + (sizeof(T) == 2 ? vh_place(m) : m)) = y;
+            if (m >= places) continue;
+            T* const at = o + (sizeof(T) == 2 ? vh_place(m) : m);
+            *reinterpret_cast<T4*>(at) = y;
+            if (REST && rest) *reinterpret_cast<T4*>(at + rest) = (T4){(T)(v[0] - (float)y[0]), (T)(v[1] - (float)y[1]),
+                                                               (T)(v[2] - (float)y[2]), (T)(v[3] - (float)y[3])};
           }
         }
       }
@@ -660,6 +669,7 @@ struct VhStoreT {
   int rows;
   float* sum;
   int first, last;
+  float scale;              // of what goes to out
   // V values of a row, from the wave's staging rows to where they belong
   template <typename T, int V>
   __device__ __forceinline__ void put(const float* src, long row, int m, int M, int split) const {
@@ -692,6 +702,8 @@ struct VhStoreT {
         return;
       }
     }
+#pragma unroll
+    for (int q = 0; q < V; ++q) v[q] *= scale;
     if (out_f32 || sizeof(T) == 4) store<float, V, ONCE>((float*)out + row * ldo + m, v, M - m);
     else store<T, V, ONCE>((T*)out + row * ldo + m, v, M - m);
   }
@@ -794,21 +806,23 @@ __global__ __launch_bounds__(256) void vh_join(const float2* __restrict__ part, 
   loss[row] = y == ignore ? 0.f : (y >= 0 && y < classes ? l - zlab[row] : __builtin_nanf(""));
 }
 
-// db[v] = sum of the row tiles' partial sums, in order
-__global__ __launch_bounds__(256) void vh_dbias(const float* __restrict__ part, long ld, int tiles, float* __restrict__ db, int n) {
+// db[v] = scale * sum of the row tiles' partial sums, in order
+__global__ __launch_bounds__(256) void vh_dbias(const float* __restrict__ part, long ld, int tiles, float* __restrict__ db, int n,
+                                                float scale) {
   const int v = blockIdx.x * 256 + threadIdx.x;
   if (v >= n) return;
   float s = 0.f;
   for (int t = 0; t < tiles; ++t) s += part[(long)t * ld + v];
-  db[v] = s;
+  db[v] = s * scale;
 }
 
 // dst[r][c] = src[r][c] with rows ldd apart (16-byte multiples), columns C .. ldd - 1 zero.  labels given: the rows of
 // ignored labels are zero as well -- whatever lies there, 0 * NaN must not reach a gradient.  Whole 16-byte chunks from any
-// element of a row (global memory takes unaligned vector loads), the last chunk of a row element by element.
+// element of a row (global memory takes unaligned vector loads), the last chunk of a row element by element.  twin: elements to
+// a second copy (0: none).
 template <typename T>
 __global__ __launch_bounds__(256) void vh_copy(const T* __restrict__ src, long lds_, int R, int C, T* __restrict__ dst, long ldd,
-                                               const int* __restrict__ labels, int ignore) {
+                                               const int* __restrict__ labels, int ignore, long twin) {
   constexpr int V = 16 / sizeof(T);
   typedef __attribute__((ext_vector_type(V))) T vec;
   typedef vec vec_any __attribute__((aligned(sizeof(T))));
@@ -832,12 +846,13 @@ __global__ __launch_bounds__(256) void vh_copy(const T* __restrict__ src, long l
       }
     }
     *reinterpret_cast<vec*>(dst + r * ldd + i) = v;
+    if (twin) *reinterpret_cast<vec*>(dst + twin + r * ldd + i) = v;
   }
 }
 
-// out[i] = sum of the splits' slabs, in order, eight loads in flight
+// out[i] = scale * sum of the slabs, in order, eight loads in flight
 template <typename O>
-__global__ __launch_bounds__(256) void vh_sum(const float* __restrict__ part, long n, int splits, O* __restrict__ out) {
+__global__ __launch_bounds__(256) void vh_sum(const float* __restrict__ part, long n, int splits, O* __restrict__ out, float scale) {
   const long i = ((long)blockIdx.x * 256 + threadIdx.x) * 4;
   if (i + 4 <= n) {
     const float* p = part + i;
@@ -853,12 +868,13 @@ __global__ __launch_bounds__(256) void vh_sum(const float* __restrict__ part, lo
 #pragma unroll 4
     for (; k < splits; ++k) s += *reinterpret_cast<const f32x4_any*>(p + k * n);
     typedef __attribute__((ext_vector_type(4))) O O4;
+    s *= scale;
     *reinterpret_cast<O4*>(out + i) = (O4){(O)s[0], (O)s[1], (O)s[2], (O)s[3]};
   } else {
     for (long j = i; j < n; ++j) {
       float s = part[j];
       for (int k = 1; k < splits; ++k) s += part[k * n + j];
-      out[j] = (O)s;
+      out[j] = (O)(s * scale);
     }
   }
 }
@@ -1031,6 +1047,7 @@ struct Plan {
   long total;
   long ldk, ldv;            // padded hidden units, classes of a piece
   int cfg, piece, pieces, splits_h, splits_w;
+  int parts;                // rows of d per row of h: 2 with its rounding errors kept
   GradTile tile_h, tile_w;
 };
 
@@ -1056,7 +1073,9 @@ Plan plan_for(int dtype, int backward, long n, int H, int V, bool h_ok, bool w_o
   };
   q.cfg = config_for(E, n);
   q.ldk = up(H, 16 / E);
-  if (!h_ok || backward) q.h_copy = take(n * q.ldk * E);
+  q.parts = backward && E == 2 && n <= 32 ? 2 : 1;
+  const long dn = q.parts * n;
+  if (!h_ok || backward) q.h_copy = take(dn * q.ldk * E);
   q.piece = backward ? (piece > 0 ? (int)up(piece, kPiece) : piece_for(n, V)) : V;
   if (q.piece > V) q.piece = V;
   q.pieces = cdiv(V, q.piece);
@@ -1068,12 +1087,12 @@ Plan plan_for(int dtype, int backward, long n, int H, int V, bool h_ok, bool w_o
   } else {
     const int KT = 128 / E;
     q.ldv = up(q.piece, KT);
-    q.d = take(n * q.ldv * E);
+    q.d = take(dn * q.ldv * E);
     q.tile_h = dh_tile(q.cfg, n, H);
     q.tile_w = dw_tile(q.cfg, H, q.piece);
-    q.splits_h = splits_for((long)cdiv(H, q.tile_h.bm) * cdiv(n, q.tile_h.bn), cdiv(q.ldv, KT), q.tile_h.want);
-    q.splits_w = splits_for((long)cdiv(H, q.tile_w.bm) * cdiv(q.piece, q.tile_w.bn), cdiv(n, KT), q.tile_w.want);
-    if (q.pieces > 1 || q.splits_h > 1) q.sum_h = take(q.splits_h * n * H * 4);
+    q.splits_h = splits_for((long)cdiv(H, q.tile_h.bm) * cdiv(dn, q.tile_h.bn), cdiv(q.ldv, KT), q.tile_h.want);
+    q.splits_w = splits_for((long)cdiv(H, q.tile_w.bm) * cdiv(q.piece, q.tile_w.bn), cdiv(dn, KT), q.tile_w.want);
+    if (q.pieces > 1 || q.splits_h * q.parts > 1) q.sum_h = take(q.splits_h * dn * H * 4);
     if (q.splits_w > 1) q.sum_w = take(q.splits_w * (long)q.piece * H * 4);
     if (bias) q.dbpart = take((long)cdiv(n, 64) * q.ldv * 4);      // at most that many row tiles
   }
@@ -1087,15 +1106,15 @@ T* at(void* ws, long o) { return (T*)((char*)ws + o - 1); }
 bool rows_ok(const void* p, long ld, int H, int E) { return !((uintptr_t)p & 15) && !(ld * E & 15) && !((long)H * E & 15); }
 
 template <typename T>
-int launch_copy(const T* src, long lds_, int R, int C, T* dst, long ldd, const int* labels, int ignore, hipStream_t s) {
+int launch_copy(const T* src, long lds_, int R, int C, T* dst, long ldd, const int* labels, int ignore, long twin, hipStream_t s) {
   const long chunks = (long)R * (ldd * (long)sizeof(T) / 16);
   const int grid = chunks > 16384L * 256 ? 16384 : cdiv(chunks, 256);
-  hipLaunchKernelGGL(vh_copy<T>, dim3(grid), dim3(256), 0, s, src, lds_, R, C, dst, ldd, labels, ignore);
+  hipLaunchKernelGGL(vh_copy<T>, dim3(grid), dim3(256), 0, s, src, lds_, R, C, dst, ldd, labels, ignore, twin);
   return (int)hipGetLastError();
 }
 template <typename O>
-int launch_sum(const float* part, long n, int splits, O* out, hipStream_t s) {
-  hipLaunchKernelGGL(vh_sum<O>, dim3(cdiv(n, 1024)), dim3(256), 0, s, part, n, splits, out);
+int launch_sum(const float* part, long n, int splits, O* out, float scale, hipStream_t s) {
+  hipLaunchKernelGGL(vh_sum<O>, dim3(cdiv(n, 1024)), dim3(256), 0, s, part, n, splits, out, scale);
   return (int)hipGetLastError();
 }
 
@@ -1113,12 +1132,12 @@ int forward(const void* h, long ldh, const void* w, long ldw, const float* bias,
   const Plan q = plan_for(E == 2 ? 1 : 0, 0, n, H, V, h_ok, w_ok, bias != nullptr, 0);
   VhOperands p{w, h, ldw, ldh, V, n, (int)q.ldk, (int)q.ldk, 0, 0, 0, 0};
   if (!h_ok) {
-    VH_TRY(launch_copy((const T*)h, ldh, n, H, at<T>(ws, q.h_copy), q.ldk, nullptr, 0, s));
+    VH_TRY(launch_copy((const T*)h, ldh, n, H, at<T>(ws, q.h_copy), q.ldk, nullptr, 0, 0, s));
     p.B = at<T>(ws, q.h_copy);
     p.ldb = q.ldk;
   }
   if (!w_ok) {
-    VH_TRY(launch_copy((const T*)w, ldw, V, H, at<T>(ws, q.w_copy), q.ldk, nullptr, 0, s));
+    VH_TRY(launch_copy((const T*)w, ldw, V, H, at<T>(ws, q.w_copy), q.ldk, nullptr, 0, 0, s));
     p.A = at<T>(ws, q.w_copy);
     p.lda = q.ldk;
   }
@@ -1139,28 +1158,30 @@ int backward(const void* h, long ldh, const void* w, long ldw, const float* bias
   const int E = sizeof(T), KT = 128 / E;
   const Plan q = plan_for(E == 2 ? 1 : 0, 1, n, H, V, rows_ok(h, ldh, H, E), rows_ok(w, ldw, H, E), db != nullptr, piece);
   const T* hp = at<T>(ws, q.h_copy);
-  VH_TRY(launch_copy((const T*)h, ldh, n, H, at<T>(ws, q.h_copy), q.ldk, labels, ignore, s));
+  const int dn = q.parts * n;
+  VH_TRY(launch_copy((const T*)h, ldh, n, H, at<T>(ws, q.h_copy), q.ldk, labels, ignore, q.parts == 2 ? n * q.ldk : 0, s));
   for (int k = 0; k < q.pieces; ++k) {
     const int v0 = k * q.piece, vn = V - v0 < q.piece ? V - v0 : q.piece;
     const long ldv = up(vn, KT);
     const T* wp = (const T*)w + (long)v0 * ldw;
     long ldwp = ldw;
     if (q.w_copy) {
-      VH_TRY(launch_copy(wp, ldw, vn, H, at<T>(ws, q.w_copy), q.ldk, nullptr, 0, s));
+      VH_TRY(launch_copy(wp, ldw, vn, H, at<T>(ws, q.w_copy), q.ldk, nullptr, 0, 0, s));
       wp = at<T>(ws, q.w_copy);
       ldwp = q.ldk;
     }
     T* d = at<T>(ws, q.d);
     const LogitsTiling t = logits_tiling(q.cfg, n, vn);
     VH_TRY(logits_all<T>(t, VhOperands{wp, hp, ldwp, q.ldk, vn, n, (int)q.ldk, (int)q.ldk, 0, 0, 0, 0}, [&](int, int c0, int) {
-      return VhGradLogits{bias ? bias + v0 + c0 : nullptr, labels, lse, row_scale, grad_scale, v0 + c0, V, ignore, d + c0, ldv, (int)ldv - c0,
+      return VhGradLogits{bias ? bias + v0 + c0 : nullptr, labels, lse, row_scale, v0 + c0, V, ignore, d + c0, ldv,
+                          q.parts == 2 ? n * ldv : 0, (int)ldv - c0,
                           db ? at<float>(ws, q.dbpart) + c0 : nullptr};
     }, s));
     for (int part = 0; db && part < 2; ++part) {
       const int c0 = part ? t.first : 0, cn = part ? vn - t.first : t.first;
       if (!cn) continue;
       hipLaunchKernelGGL(vh_dbias, dim3(cdiv(cn, 256)), dim3(256), 0, s, at<float>(ws, q.dbpart) + c0, ldv, cdiv(n, t.kind[part].bn),
-                         (float*)db + v0 + c0, cn);
+                         (float*)db + v0 + c0, cn, grad_scale);
       VH_TRY((int)hipGetLastError());
     }
     if (dw) {
@@ -1169,19 +1190,19 @@ int backward(const void* h, long ldh, const void* w, long ldw, const float* bias
       // A large dw would only push other things out of the 256 MB cache (16 rows, 4096 x 32000: 90 us with plain stores, 62 with
       // non-temporal ones); a small one stays for whoever reads it next.
       const bool once = !split && (long)V * H * (dw_f32 ? 4 : E) >= (64L << 20);
-      const VhOperands o{hp, d, q.ldk, ldv, H, (int)ldv, n, n, 0, 0, 0, 0};
+      const VhOperands o{hp, d, q.ldk, ldv, H, (int)ldv, dn, dn, 0, 0, 0, 0};
       float* sum = split ? at<float>(ws, q.sum_w) : nullptr;
-      if (once) VH_TRY((product_dw<T>(q.tile_w, o, 1, VhStoreT<true>{out, H, dw_f32, 1, vn, sum, 1, 1}, s)));
-      else VH_TRY((product_dw<T>(q.tile_w, o, q.splits_w, VhStore{out, H, dw_f32, 1, vn, sum, 1, !split}, s)));
+      if (once) VH_TRY((product_dw<T>(q.tile_w, o, 1, VhStoreT<true>{out, H, dw_f32, 1, vn, sum, 1, 1, grad_scale}, s)));
+      else VH_TRY((product_dw<T>(q.tile_w, o, q.splits_w, VhStore{out, H, dw_f32, 1, vn, sum, 1, !split, grad_scale}, s)));
       if (split)
-        VH_TRY(dw_f32 ? launch_sum(at<float>(ws, q.sum_w), (long)vn * H, q.splits_w, (float*)out, s)
-                      : launch_sum(at<float>(ws, q.sum_w), (long)vn * H, q.splits_w, (T*)out, s));
+        VH_TRY(dw_f32 ? launch_sum(at<float>(ws, q.sum_w), (long)vn * H, q.splits_w, (float*)out, grad_scale, s)
+                      : launch_sum(at<float>(ws, q.sum_w), (long)vn * H, q.splits_w, (T*)out, grad_scale, s));
     }
     if (dh) {
-      const bool last = k == q.pieces - 1, split = q.splits_h > 1;
-      VhStore st{dh, H, 0, 0, n, q.sum_h ? at<float>(ws, q.sum_h) : nullptr, k == 0, last && !split};
-      VH_TRY((product_dh<T>(q.cfg, q.tile_h, VhOperands{wp, d, ldwp, ldv, H, n, vn, (int)ldv, 0, 0, 0, 0}, q.splits_h, st, s)));
-      if (last && split) VH_TRY(launch_sum(at<float>(ws, q.sum_h), (long)n * H, q.splits_h, (T*)dh, s));
+      const bool last = k == q.pieces - 1, split = q.splits_h * q.parts > 1;
+      VhStore st{dh, H, 0, 0, dn, q.sum_h ? at<float>(ws, q.sum_h) : nullptr, k == 0, last && !split, grad_scale};
+      VH_TRY((product_dh<T>(q.cfg, q.tile_h, VhOperands{wp, d, ldwp, ldv, H, dn, vn, (int)ldv, 0, 0, 0, 0}, q.splits_h, st, s)));
+      if (last && split) VH_TRY(launch_sum(at<float>(ws, q.sum_h), (long)n * H, q.splits_h * q.parts, (T*)dh, grad_scale, s));
     }
   }
   return 0;

@@ -445,6 +445,50 @@ def test_stride_of_a_single_row_says_nothing(gpu_lib):
     assert torch.equal(vocab_head_fwd(h, view, torch.zeros_like(y))[1], vocab_head_fwd(h, h, torch.zeros_like(y))[1])
 
 
+def without_own_rounding(x, grad_scale, kept):
+    """(dw, bound) in fp32 where d, relative to grad_scale, is rounded to bf16 once -- by its distance to the nearest bf16 value,
+    which changes by no more than d itself does -- or (kept) carries its rounding error in a second bf16 value: half^2."""
+    d1, e1 = x.d / grad_scale, x.e_d / grad_scale
+    far = x.half * x.half * d1.abs() if kept else (d1.float().bfloat16().double() - d1).abs() + U * d1.abs()
+    d, e_d = x.d.t(), (grad_scale * (2 * e1 + far)).t()
+    got = d @ x.h
+    e = (e_d + 8 * math.sqrt(2 * d.shape[1]) * U * d.abs()) @ x.h.abs()
+    return got, e + U * (got.abs() + e)
+
+
+@gpu
+@pytest.mark.parametrize("n", [300, 1000])
+def test_the_common_factor_is_not_rounded_into_the_gradient(gpu_lib, n):
+    """Classes that are all alike: a label's d is -(1 - 1/classes), next to a bf16 value, and would be off by 0.39 % in every row
+    if it were rounded after its product with a factor that lies halfway between two bf16 values."""
+    s = (1 + 2.0 ** -8) / 1024
+    h, w, y, b = make(n, 64, 3000, "bf16", seed=n)
+    h = h * 0.01
+    x = Exact(h, w, y, b, grad_scale=s)
+    _, lse = vocab_head_fwd(h, w, y, b)
+    dw = torch.empty(w.shape, device=DEV)
+    vocab_head_bwd(h, w, y, lse, b, grad_scale=s, dwT=dw)
+    got, e = without_own_rounding(x, s, False)
+    within(dw, got, e, "dw")
+    assert float(e[y.long()].abs().median()) < 2e-3 * float(got[y.long()].abs().median())
+
+
+@gpu
+@pytest.mark.parametrize("n,classes,piece", [(1, 400, 0), (1, 2000, 256), (5, 1111, 0), (17, 300, 0), (32, 4099, 1024)])
+def test_few_rows_keep_what_rounding_drops(gpu_lib, n, classes, piece):
+    h, w, y, b = make(n, 96, classes, "bf16", bias=True, ignored=0.1 if n > 1 else 0.0, seed=n + classes)
+    s = 0.3
+    x = Exact(h, w, y, b, grad_scale=s)
+    _, lse = vocab_head_fwd(h, w, y, b)
+    dw = torch.empty(w.shape, device=DEV)
+    dh, _, _ = vocab_head_bwd(h, w, y, lse, b, grad_scale=s, dwT=dw, piece=piece)
+    got, e = without_own_rounding(x, s, True)
+    within(dw, got, e, "dw")
+    got = x.d @ x.w
+    e = (2 * x.e_d + (x.half ** 2 + 8 * math.sqrt(2 * classes) * U) * x.d.abs()) @ x.w.abs()
+    within(dh, got, e + x.half * (got.abs() + e), "dh")
+
+
 # ---------------------------------------------------------------------------------------------- streams and graphs
 @gpu
 def test_graph_replays_and_streams(gpu_lib):
