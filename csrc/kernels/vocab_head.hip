@@ -20,22 +20,37 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 typedef f32x4 f32x4_any __attribute__((aligned(4)));
 
-template <typename T> struct VhType;
-template <> struct VhType<bf16> {
-  static __device__ __forceinline__ f32x4 mma(const u32x4& a, const u32x4& b, f32x4 c) {
-    return mfma16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c);
-  }
+__device__ __forceinline__ f32x4 vh_mma(const u32x4& a, const u32x4& b, f32x4 c) {
+  return mfma16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c);
+}
+
+// fp32 operands are multiplied on the bf16 matrix cores: a value is the sum of three bf16 values, each the rounding of what the
+// ones before it leave (8 + 8 + 8 bits and their signs hold all 24), products of two bf16 values are exact in the fp32
+// accumulators, and of the nine only the three below 2^-24 of the whole are left out:
+//   a b = a1 b1 + (a1 b2 + a2 b1) + (a1 b3 + a2 b2 + a3 b1) + at most 2^-23 |a b|
+// Six bf16 instructions do 16 x 16 x 32 in 96 cycles, the fp32 ones (16 x 16 x 4) take 256.  Values that round beyond bf16's
+// largest (3.39e38) count as infinite, and infinite ones give NaN (their second part is inf - inf).  Measured: 4096 x 1024 x
+// 16000 971 us with the fp32 instructions (138 TFLOP/s, their peak is 157), 660 this way.
+struct VhSplit {
+  u32x4 part[3];
 };
-template <> struct VhType<float> {
-  // lane group g holds k = 4 g .. 4 g + 3 of both operands; step s multiplies k = 4 g + s, so that the four steps cover
-  // all sixteen
-  static __device__ __forceinline__ f32x4 mma(const u32x4& a, const u32x4& b, f32x4 c) {
-    const f32x4 x = __builtin_bit_cast(f32x4, a), y = __builtin_bit_cast(f32x4, b);
+__device__ __forceinline__ VhSplit vh_split(const u32x4& k0, const u32x4& k1) {
+  const f32x4 x = __builtin_bit_cast(f32x4, k0), y = __builtin_bit_cast(f32x4, k1);
+  float v[8] = {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
+  VhSplit s;
 #pragma unroll
-    for (int s = 0; s < 4; ++s) c = __builtin_amdgcn_mfma_f32_16x16x4f32(x[s], y[s], c, 0, 0, 0);
-    return c;
-  }
-};
+  for (int q = 0; q < 3; ++q)
+#pragma unroll
+    for (int e = 0; e < 8; e += 2) {
+      typedef __attribute__((ext_vector_type(2))) bf16 bf16x2;
+      const bf16x2 h = {(bf16)v[e], (bf16)v[e + 1]};
+      const unsigned w = __builtin_bit_cast(unsigned, h);
+      s.part[q][e / 2] = w;
+      v[e] -= __builtin_bit_cast(float, w << 16);               // (both halves from the pair: one conversion, not three)
+      v[e + 1] -= __builtin_bit_cast(float, w & 0xffff0000u);
+    }
+  return s;
+}
 
 __device__ __forceinline__ void vh_dma16(__amdgpu_buffer_rsrc_t r, const void* lds, uint32_t voff, uint32_t soff) {
 #if defined(__HIP_DEVICE_COMPILE__)
@@ -163,19 +178,20 @@ struct VhFrags {
     else if (E == 2) off = (4 * g + (i16 >> 2)) * ROWB + (((r0 >> 4) ^ vh_window_key<E, ROWB>(4 * g + (i16 >> 2))) << 5) + 8 * (i16 & 3);
     else off = 4 * g * ROWB + (((r0 >> 4) ^ vh_window_key<E, ROWB>(4 * g)) << 6) + 4 * i16;
   }
-  __device__ __forceinline__ void read(u32x4 (&f)[CNT], const char* lds, int half) const {
+  __device__ __forceinline__ u32x4 one(const char* lds, int half, int i) const {
     static_assert(!SLOW || E == 4, "bf16 slow operands are read by read_tr");
     if constexpr (!SLOW) {
-      const char* p = lds + (off ^ (half << 6));
-#pragma unroll
-      for (int i = 0; i < CNT; ++i) f[i] = *reinterpret_cast<const u32x4*>(p + i * 2048);
+      return *reinterpret_cast<const u32x4*>(lds + (off ^ (half << 6)) + i * 2048);
     } else {
-      const char* p = lds + half * 16 * ROWB;
+      u32x4 f;
 #pragma unroll
-      for (int i = 0; i < CNT; ++i)
-#pragma unroll
-        for (int s = 0; s < 4; ++s) f[i][s] = *reinterpret_cast<const unsigned*>(p + (off ^ (i << 6)) + s * ROWB);
+      for (int s = 0; s < 4; ++s) f[s] = *reinterpret_cast<const unsigned*>(lds + half * 16 * ROWB + (off ^ (i << 6)) + s * ROWB);
+      return f;
     }
+  }
+  __device__ __forceinline__ void read(u32x4 (&f)[CNT], const char* lds, int half) const {
+#pragma unroll
+    for (int i = 0; i < CNT; ++i) f[i] = one(lds, half, i);
   }
   // Fragments i .. i + 3 (or both of CNT == 2) of a bf16 slow operand.  The reads and the wait for them are one block: nothing
   // between them can use, move or reuse a register that is still being written.
@@ -221,11 +237,12 @@ struct VhFrags {
 // Main loop: K tiles t0 .. t1 - 1 in D LDS buffers (two for the large tiles, which take all of LDS; four for small ones, whose
 // tiles are over sooner than their operands arrive).
 //
-// Both operands fast (or fp32): a tile is multiplied in two halves, and the fragments of a half are read during the MFMAs of
+// bf16, both operands fast: a tile is multiplied in two halves, and the fragments of a half are read during the MFMAs of
 // the half before it, one barrier per tile:
 //   read the second half of tile t | MFMAs on the first | wait until tile t + 1 has landed, barrier
 //   DMA of tile t + D into the buffer of tile t | read the first half of tile t + 1 | MFMAs on the second half of tile t
-// A bf16 slow operand (its fragments are read right before their MFMAs; the other wave of the SIMD covers the wait):
+// fp32, and a bf16 slow operand (fragments are read, fp32 ones split, right before their MFMAs; the other wave of the SIMD covers
+// that):
 //   wait until tile t has landed, barrier | DMA of tile t + D - 1 into the buffer of tile t - 1 | both halves of tile t
 //
 // The epilogue's inputs (labels, log-sum-exps, biases of the tile) are requested before the first operand tile and put into
@@ -259,9 +276,35 @@ __device__ __forceinline__ void vh_mainloop(const VhOperands& p, Tile& c, char* 
     for (int j = 0; j < NTL; ++j) c.acc[i][j] = (f32x4){0.f, 0.f, 0.f, 0.f};
   if (t0 >= t1) return;
   const auto early = e.template request<BM, BN, NT>(p, c.m0, c.n0, tid);
-  u32x4 fb[2][NTL];
-
-  if constexpr (sizeof(T) == 2 && (AS || BS)) {
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int d = 0; d + 1 < D; ++d)
+      if (t0 + d < t1) dma(t0 + d, lds + d * STAGE);
+    e.template keep<BM, BN, NT>(early, in, tid);
+    char* buf = lds;
+    char* last = lds + (D - 1) * STAGE;         // the buffer of tile t - 1
+#pragma unroll 1
+    for (int t = t0; t < t1; ++t) {
+      if (D > 2 && t + D - 1 <= t1) vh_wait<(D - 2) * NDMA>();
+      else vh_wait<0>();
+      vh_barrier();
+      if (t + D - 1 < t1) dma(t + D - 1, last);
+      VhSplit b[NTL];
+#pragma unroll
+      for (int j = 0; j < NTL; ++j) b[j] = vh_split(rb.one(buf + ABYTES, 0, j), rb.one(buf + ABYTES, 1, j));
+#pragma unroll
+      for (int i = 0; i < MT; ++i) {
+        const VhSplit a = vh_split(ra.one(buf, 0, i), ra.one(buf, 1, i));
+        constexpr int TERMS[6][2] = {{0, 2}, {2, 0}, {1, 1}, {0, 1}, {1, 0}, {0, 0}};      // the smallest first
+#pragma unroll
+        for (int q = 0; q < 6; ++q)
+#pragma unroll
+          for (int j = 0; j < NTL; ++j) c.acc[i][j] = vh_mma(a.part[TERMS[q][0]], b[j].part[TERMS[q][1]], c.acc[i][j]);
+      }
+      last = buf;
+      buf = next(buf);
+    }
+  } else if constexpr (AS || BS) {
     typedef VhFrags<T, BM, AS, MT> RA;
     typedef VhFrags<T, BN, BS, NTL> RB;
     static_assert(AS && MT % RA::TR == 0 && (!BS || NTL % RB::TR == 0), "slow products: dh (A) and dw (A and B)");
@@ -269,6 +312,7 @@ __device__ __forceinline__ void vh_mainloop(const VhOperands& p, Tile& c, char* 
     for (int d = 0; d + 1 < D; ++d)
       if (t0 + d < t1) dma(t0 + d, lds + d * STAGE);
     e.template keep<BM, BN, NT>(early, in, tid);
+    u32x4 fb[2][NTL];
     char* buf = lds;
     char* last = lds + (D - 1) * STAGE;         // the buffer of tile t - 1
 #pragma unroll 1
@@ -293,14 +337,14 @@ __device__ __forceinline__ void vh_mainloop(const VhOperands& p, Tile& c, char* 
 #pragma unroll
           for (int k = 0; k < RA::TR; ++k)
 #pragma unroll
-            for (int j = 0; j < NTL; ++j) c.acc[i + k][j] = VhType<T>::mma(a[k], fb[BS ? 0 : h][j], c.acc[i + k][j]);
+            for (int j = 0; j < NTL; ++j) c.acc[i + k][j] = vh_mma(a[k], fb[BS ? 0 : h][j], c.acc[i + k][j]);
         }
       }
       last = buf;
       buf = next(buf);
     }
   } else {
-    u32x4 fa[2][MT];
+    u32x4 fa[2][MT], fb[2][NTL];
     auto frags = [&](int x, const char* buf, int half) {
       ra.read(fa[x], buf, half);
       rb.read(fb[x], buf + ABYTES, half);
@@ -309,10 +353,10 @@ __device__ __forceinline__ void vh_mainloop(const VhOperands& p, Tile& c, char* 
 #pragma unroll
       for (int i = 0; i < MT; ++i)
 #pragma unroll
-        for (int j = 0; j < NTL; ++j) c.acc[i][j] = VhType<T>::mma(fa[x][i], fb[x][j], c.acc[i][j]);
+        for (int j = 0; j < NTL; ++j) c.acc[i][j] = vh_mma(fa[x][i], fb[x][j], c.acc[i][j]);
     };
     // the schedule of a half: the DMAs one MFMA apart, then the fragment reads spread over the others
-    constexpr int R = (AS ? 4 * MT : MT) + (BS ? 4 * NTL : NTL), X = MT * NTL * (sizeof(T) == 2 ? 1 : 4);
+    constexpr int R = MT + NTL, X = MT * NTL;
     constexpr int PER = (X - NDMA) / R > 0 ? (X - NDMA) / R : 1;
     auto spread = [&](bool dmas) {
       if (dmas) {
@@ -893,13 +937,11 @@ constexpr int kPiece = 256;           // pieces are multiples of this many class
 // Tile configurations, chosen by the number of rows.
 //   kSmall: up to 64 rows -- every product streams the weight or its gradient once and is bound by memory: small tiles of the
 //           classes / hidden units, several workgroups per CU.
-//   kMid:   up to 128 rows, and fp32: 128 x 64 tiles of four waves, three workgroups per CU (fp32, 1024 x 1024 x 10000: forward
-//           198 us with 128 x 128 tiles, whose 640 do not divide evenly over the CUs, 174 us with these; 4096 x 1024 x 16000: 969
-//           and 976).
+//   kMid:   up to 128 rows: 128 x 64 tiles of four waves, three workgroups per CU.
 //   kLarge: 256 x 256 tiles of eight waves, one workgroup per CU -- or 128 x 128 tiles of four, two per CU, where the large
 //           ones leave CUs idle.
 enum { kSmall, kMid, kLarge };
-int config_for(int E, long n) { return n <= 64 ? kSmall : (E == 4 || n <= 128 ? kMid : kLarge); }
+int config_for(long n) { return n <= 64 ? kSmall : (n <= 128 ? kMid : kLarge); }
 
 // Tiles of the gradient products
 struct GradTile {
@@ -910,23 +952,26 @@ constexpr GradTile kTiles256{256, 256, 256}, kTiles128{128, 128, 512}, kTiles64{
 // dh is cut along the classes into as many slabs as it takes to fill the card, so what many large tiles save in operand reads
 // few of them lose in slabs: 16 tiles (1000 rows, 1000 x 10007) 42 us against 33 with the small ones, 24 (1500 rows) 55 and 45,
 // 32 (4000 rows, 512 x 30000) 139 and 160, 64 (777 rows, 4096 x 50001) 342 and 364.
-GradTile dh_tile(int cfg, long n, int H) {
+// fp32 products take a wave all its registers in large tiles, and wait less for each other in small ones (4096 x 1024 x 16000: dh
+// 906 and 753 us, dw 931 and 740).
+GradTile dh_tile(int E, int cfg, long n, int H) {
   if (cfg != kLarge) return kTiles64;
-  return (long)cdiv(H, 256) * cdiv(n, 256) < 32 ? kTiles128 : kTiles256;
+  return E == 4 || (long)cdiv(H, 256) * cdiv(n, 256) < 32 ? kTiles128 : kTiles256;
 }
 // dw has its classes to fill the card: rounds over it times their length, 0.57 of a large tile's for two small ones per CU.
 // 316 large tiles are two rounds (700 rows, 1024 x 20000: 47 us, small ones 40), 252 are one (500 rows, 1000 x 16000: 23 and 26).
-GradTile dw_tile(int cfg, int H, int classes) {
+GradTile dw_tile(int E, int cfg, int H, int classes) {
   if (cfg != kLarge) return kTiles64;
   const long large = (long)cdiv(H, 256) * cdiv(classes, 256), small = (long)cdiv(H, 128) * cdiv(classes, 128);
-  return 0.57 * cdiv(small, 512) < cdiv(large, 256) ? kTiles128 : kTiles256;
+  return E == 4 || 0.57 * cdiv(small, 512) < cdiv(large, 256) ? kTiles128 : kTiles256;
 }
 
 // How the logits product of some classes is tiled: the classes below `first` in tiles of one kind, the others in a second one.
 // The large kinds run one workgroup per CU, so what counts is the number of rounds over the 256 CUs times the length of a round
 // (measured at H = 4096, against 256 x 256: 0.82 for 192 x 256, 0.68 for 256 x 128), and a last round for a few tiles is as long
 // as any other: its classes go to small tiles instead.  777 rows x 50001 classes: 784 tiles are four rounds, 362 us; three
-// rounds and 91 small tiles 330 us.
+// rounds and 91 small tiles 330 us.  Logits that fill no round of small tiles are theirs altogether: a few large tiles take long
+// over their K (300 rows, 2048 x 5000, 200 small tiles: 30 and 20 us; fp32, whose tiles take longer, gains up to 768 of them).
 struct LogitsTile {
   int bm, bn;
 };
@@ -935,10 +980,10 @@ struct LogitsTiling {
   int first;              // classes of the first kind (a multiple of its bm, or all)
   int tiles[2];           // class tiles of either
 };
-LogitsTiling logits_tiling(int cfg, long n, int classes) {
+LogitsTiling logits_tiling(int E, int cfg, long n, int classes) {
   LogitsTiling q{{{128, 64}, {128, 64}}, classes, {0, 0}};
-  if (cfg == kSmall) q.kind[0] = {64, 64};
-  if (cfg == kLarge) {
+  if (cfg == kSmall) q.kind[0] = {64, E == 4 && n <= 32 ? 32 : 64};
+  if (cfg == kLarge && (long)cdiv(classes, 128) * cdiv(n, 64) > (E == 4 ? 768 : 512)) {
     const struct { LogitsTile t; double length; } kinds[3] = {{{256, 256}, 1.0}, {{192, 256}, 0.82}, {{256, 128}, 0.68}};
     // small tiles: three to a CU; the first of a CU costs more than the next two
     auto small = [&](int rest) {
@@ -985,14 +1030,18 @@ template <typename T, class Epi>
 int logits(LogitsTile t, const VhOperands& p, const Epi& e, hipStream_t s) {
   // buffers: 16 rows, 4096 x 32000 bf16: 65.5 us with two, 63.3 with three, 56.1 with four; 128 x 64 tiles of bf16 alone on their
   // CUs gain from a third (prompt of 777 rows: 357 -> 344 us), fp32 ones are long enough
-  if (t.bm == 64) return launch<T, 64, 64, 4, 1, false, false, 4>(p, 1, e, s);
-  if (t.bm == 128) return launch<T, 128, 64, 2, 2, false, false, sizeof(T) == 2 ? 3 : 2>(p, 1, e, s);
-  if constexpr (sizeof(T) == 2) {
-    if (t.bm == 192) return launch<T, 192, 256, 2, 4, false, false, 2>(p, 1, e, s);
-    if (t.bn == 128) return launch<T, 256, 128, 4, 2, false, false, 3>(p, 1, e, s);
-    return launch<T, 256, 256, 2, 4, false, false, 2>(p, 1, e, s);
+  // fp32: the fewer fragments of the rows' side a wave splits the better (one row, 1024 x 32000: 59 us with 64 rows' tiles of waves
+  // side by side, 39 with 32 rows' ones; 64 rows, 1024 x 20000: 56 us side by side, 49 two by two)
+  if constexpr (sizeof(T) == 4) {
+    if (t.bn == 32) return launch<T, 64, 32, 4, 1, false, false, 4>(p, 1, e, s);
+    if (t.bm == 64) return launch<T, 64, 64, 2, 2, false, false, 4>(p, 1, e, s);
+  } else {
+    if (t.bm == 64) return launch<T, 64, 64, 4, 1, false, false, 4>(p, 1, e, s);
   }
-  return -1;
+  if (t.bm == 128) return launch<T, 128, 64, 2, 2, false, false, sizeof(T) == 2 ? 3 : 2>(p, 1, e, s);
+  if (t.bm == 192) return launch<T, 192, 256, 2, 4, false, false, 2>(p, 1, e, s);
+  if (t.bn == 128) return launch<T, 256, 128, 4, 2, false, false, 3>(p, 1, e, s);
+  return launch<T, 256, 256, 2, 4, false, false, 2>(p, 1, e, s);
 }
 // The same for all classes: e(kind, first class, first class tile) is the epilogue of a part
 template <typename T, class Make>
@@ -1012,19 +1061,17 @@ int logits_all(const LogitsTiling& q, VhOperands p, const Make& make, hipStream_
 template <typename T>
 int product_dh(int cfg, const GradTile& t, const VhOperands& p, int splits, const VhStore& e, hipStream_t s) {
   if (cfg == kSmall) return launch<T, 128, 64, 4, 1, true, false, 3>(p, splits, e, s);
-  if constexpr (sizeof(T) == 2) {
+  if constexpr (sizeof(T) == 2)
     if (t.bn == 256) return launch<T, 256, 256, 2, 4, true, false, 2>(p, splits, e, s);
-    if (t.bn == 128) return launch<T, 128, 128, 2, 2, true, false, 2>(p, splits, e, s);
-  }
+  if (t.bn == 128) return launch<T, 128, 128, 2, 2, true, false, 2>(p, splits, e, s);
   return launch<T, 128, 64, 2, 2, true, false, 2>(p, splits, e, s);
 }
 // dw^T [hidden][classes] = h^T . d: both sides slow
 template <typename T, bool ONCE>
 int product_dw(const GradTile& t, const VhOperands& p, int splits, const VhStoreT<ONCE>& e, hipStream_t s) {
-  if constexpr (sizeof(T) == 2) {
+  if constexpr (sizeof(T) == 2)
     if (t.bn == 256) return launch<T, 256, 256, 2, 4, true, true, 2>(p, splits, e, s);
-    if (t.bn == 128) return launch<T, 128, 128, 2, 2, true, true, 2>(p, splits, e, s);
-  }
+  if (t.bn == 128) return launch<T, 128, 128, 2, 2, true, true, 2>(p, splits, e, s);
   return launch<T, 128, 64, 2, 2, true, true, 2>(p, splits, e, s);
 }
 
@@ -1071,7 +1118,7 @@ Plan plan_for(int dtype, int backward, long n, int H, int V, bool h_ok, bool w_o
     at += up(bytes, 256);
     return o + 1;           // 0 stands for "none"
   };
-  q.cfg = config_for(E, n);
+  q.cfg = config_for(n);
   q.ldk = up(H, 16 / E);
   q.parts = backward && E == 2 && n <= 32 ? 2 : 1;
   const long dn = q.parts * n;
@@ -1081,20 +1128,20 @@ Plan plan_for(int dtype, int backward, long n, int H, int V, bool h_ok, bool w_o
   q.pieces = cdiv(V, q.piece);
   if (!w_ok) q.w_copy = take((long)q.piece * q.ldk * E);
   if (!backward) {
-    const LogitsTiling t = logits_tiling(q.cfg, n, V);
+    const LogitsTiling t = logits_tiling(E, q.cfg, n, V);
     q.part = take((long)(t.tiles[0] + t.tiles[1]) * n * 8);
     q.zlab = take(n * 4);
   } else {
     const int KT = 128 / E;
     q.ldv = up(q.piece, KT);
     q.d = take(dn * q.ldv * E);
-    q.tile_h = dh_tile(q.cfg, n, H);
-    q.tile_w = dw_tile(q.cfg, H, q.piece);
+    q.tile_h = dh_tile(E, q.cfg, n, H);
+    q.tile_w = dw_tile(E, q.cfg, H, q.piece);
     q.splits_h = splits_for((long)cdiv(H, q.tile_h.bm) * cdiv(dn, q.tile_h.bn), cdiv(q.ldv, KT), q.tile_h.want);
     q.splits_w = splits_for((long)cdiv(H, q.tile_w.bm) * cdiv(q.piece, q.tile_w.bn), cdiv(dn, KT), q.tile_w.want);
     if (q.pieces > 1 || q.splits_h * q.parts > 1) q.sum_h = take(q.splits_h * dn * H * 4);
     if (q.splits_w > 1) q.sum_w = take(q.splits_w * (long)q.piece * H * 4);
-    if (bias) q.dbpart = take((long)cdiv(n, 64) * q.ldv * 4);      // at most that many row tiles
+    if (bias) q.dbpart = take((long)cdiv(n, 32) * q.ldv * 4);      // at most that many row tiles
   }
   q.total = at ? at : 256;
   return q;
@@ -1141,7 +1188,7 @@ int forward(const void* h, long ldh, const void* w, long ldw, const float* bias,
     p.A = at<T>(ws, q.w_copy);
     p.lda = q.ldk;
   }
-  const LogitsTiling t = logits_tiling(q.cfg, n, V);
+  const LogitsTiling t = logits_tiling(E, q.cfg, n, V);
   VH_TRY(logits_all<T>(t, p, [&](int, int c0, int tile0) {
     return VhForward{bias ? bias + c0 : nullptr, labels, c0, at<float2>(ws, q.part) + (long)tile0 * n, at<float>(ws, q.zlab), n};
   }, s));
@@ -1171,7 +1218,7 @@ int backward(const void* h, long ldh, const void* w, long ldw, const float* bias
       ldwp = q.ldk;
     }
     T* d = at<T>(ws, q.d);
-    const LogitsTiling t = logits_tiling(q.cfg, n, vn);
+    const LogitsTiling t = logits_tiling(E, q.cfg, n, vn);
     VH_TRY(logits_all<T>(t, VhOperands{wp, hp, ldwp, q.ldk, vn, n, (int)q.ldk, (int)q.ldk, 0, 0, 0, 0}, [&](int, int c0, int) {
       return VhGradLogits{bias ? bias + v0 + c0 : nullptr, labels, lse, row_scale, v0 + c0, V, ignore, d + c0, ldv,
                           q.parts == 2 ? n * ldv : 0, (int)ldv - c0,

@@ -2,7 +2,8 @@
 
 Bounds (u = 2^-24, half = half a rounding step of the operand type):
   logits    a sum of H products, the rounding errors of its partial sums (each at most u times S_iv = sum_k |h_ik w_vk|) wander:
-            e_z = 8 sqrt(H + 64) u S; the largest over a row counts for the row's log-sum-exp
+            e_z = 8 sqrt(H + 64) u S; the largest over a row counts for the row's log-sum-exp (fp32 products are themselves
+            off by 2^-23 = 2 u at most, which the 64 covers)
   lse       e_lse = max_v e_z + 8 u (1 + |lse|)              loss  e_lse + e_z + 8 u (1 + |lse| + |z_y|)
   d         |s| (p (e_z + e_lse + 8 u (1 + |z| + |lse|)) + 2 u), and the rounding to the operand type: half |d|
   products  every error of d times the other factor, summed, plus the accumulation 8 sqrt(terms) u sum |d| |w|, plus half of
@@ -208,27 +209,29 @@ def test_pieces_bias_ignored_rows_and_row_scales(gpu_lib, n, hidden, classes, pi
 
 
 @gpu
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
 @pytest.mark.parametrize("n,hidden,classes,piece", [
     (300, 64, 32000, 0),        # 256 x 128 tiles
     (1000, 40, 10007, 0),       # 192 x 256
     (777, 64, 50001, 0),        # three rounds of 256 x 256, the other classes in small tiles
     (2049, 72, 20011, 8192),    # pieces tiled differently
     (130, 8, 70001, 0)])
-def test_every_tiling_of_the_logits(gpu_lib, n, hidden, classes, piece):
-    h, w, y, b = make(n, hidden, classes, "bf16", bias=True, ignored=0.1, seed=classes)
+def test_every_tiling_of_the_logits(gpu_lib, n, hidden, classes, piece, dtype):
+    h, w, y, b = make(n, hidden, classes, dtype, bias=True, ignored=0.1, seed=classes)
     y[:4] = torch.tensor([classes - 1, classes - 2, 0, 255], dtype=torch.int32, device=DEV)
     check_all(h, w, y, b, grad_scale=1.0 / n, piece=piece)
 
 
 @gpu
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
 @pytest.mark.parametrize("n,hidden,classes", [
     (1100, 1800, 8000),         # dh and dw in 256 x 256 tiles
     (1100, 1800, 18011),        # dw in 128 x 128 tiles
     (300, 600, 40003),          # dh in 128 x 128 tiles and slabs
     (700, 1000, 20011),         # both in 128 x 128 tiles
     (1030, 2050, 4100)])        # a few rows, hidden units and classes over
-def test_every_tiling_of_the_gradients(gpu_lib, n, hidden, classes):
-    h, w, y, b = make(n, hidden, classes, "bf16", bias=True, ignored=0.1, seed=hidden)
+def test_every_tiling_of_the_gradients(gpu_lib, n, hidden, classes, dtype):
+    h, w, y, b = make(n, hidden, classes, dtype, bias=True, ignored=0.1, seed=hidden)
     check_all(h, w, y, b, grad_scale=1.0 / n)
 
 
