@@ -292,14 +292,30 @@ __device__ __forceinline__ void vh_mainloop(const VhOperands& p, Tile& c, char* 
       VhSplit b[NTL];
 #pragma unroll
       for (int j = 0; j < NTL; ++j) b[j] = vh_split(rb.one(buf + ABYTES, 0, j), rb.one(buf + ABYTES, 1, j));
+      VhSplit a = vh_split(ra.one(buf, 0, 0), ra.one(buf, 1, 0));
 #pragma unroll
       for (int i = 0; i < MT; ++i) {
-        const VhSplit a = vh_split(ra.one(buf, 0, i), ra.one(buf, 1, i));
         constexpr int TERMS[6][2] = {{0, 2}, {2, 0}, {1, 1}, {0, 1}, {1, 0}, {0, 0}};      // the smallest first
+        VhSplit ahead = a;
+        if (i + 1 < MT) ahead = vh_split(ra.one(buf, 0, i + 1), ra.one(buf, 1, i + 1));
 #pragma unroll
         for (int q = 0; q < 6; ++q)
 #pragma unroll
           for (int j = 0; j < NTL; ++j) c.acc[i][j] = vh_mma(a.part[TERMS[q][0]], b[j].part[TERMS[q][1]], c.acc[i][j]);
+        a = ahead;
+        // the next fragment (44 vector instructions) is split in the shadow of this one's MFMAs, behind the first two, while it
+        // arrives (4096 x 1024 x 16000 forward 650 -> 608 us)
+        if (i + 1 < MT) {
+          constexpr int PER = (44 + 6 * NTL - 3) / (6 * NTL - 2);
+          __builtin_amdgcn_sched_group_barrier(0x100, AS ? 8 : 2, 0);
+          __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
+#pragma unroll
+          for (int x = 2; x < 6 * NTL; ++x) {
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x002, PER, 0);
+          }
+          __builtin_amdgcn_sched_barrier(0);
+        }
       }
       last = buf;
       buf = next(buf);
@@ -937,7 +953,8 @@ constexpr int kPiece = 256;           // pieces are multiples of this many class
 // Tile configurations, chosen by the number of rows.
 //   kSmall: up to 64 rows -- every product streams the weight or its gradient once and is bound by memory: small tiles of the
 //           classes / hidden units, several workgroups per CU.
-//   kMid:   up to 128 rows: 128 x 64 tiles of four waves, three workgroups per CU.
+//   kMid:   up to 128 rows: 128 x 64 tiles of four waves, three workgroups per CU (fp32 logits in 64 x 64: 128 rows, 2048 x
+//           8000: 73 and 55 us).
 //   kLarge: 256 x 256 tiles of eight waves, one workgroup per CU -- or 128 x 128 tiles of four, two per CU, where the large
 //           ones leave CUs idle.
 enum { kSmall, kMid, kLarge };
@@ -982,7 +999,7 @@ struct LogitsTiling {
 };
 LogitsTiling logits_tiling(int E, int cfg, long n, int classes) {
   LogitsTiling q{{{128, 64}, {128, 64}}, classes, {0, 0}};
-  if (cfg == kSmall) q.kind[0] = {64, E == 4 && n <= 32 ? 32 : 64};
+  if (cfg == kSmall || (E == 4 && cfg == kMid)) q.kind[0] = {64, E == 4 && n <= 32 ? 32 : 64};
   if (cfg == kLarge && (long)cdiv(classes, 128) * cdiv(n, 64) > (E == 4 ? 768 : 512)) {
     const struct { LogitsTile t; double length; } kinds[3] = {{{256, 256}, 1.0}, {{192, 256}, 0.82}, {{256, 128}, 0.68}};
     // small tiles: three to a CU; the first of a CU costs more than the next two
@@ -1034,7 +1051,7 @@ int logits(LogitsTile t, const VhOperands& p, const Epi& e, hipStream_t s) {
   // side by side, 39 with 32 rows' ones; 64 rows, 1024 x 20000: 56 us side by side, 49 two by two)
   if constexpr (sizeof(T) == 4) {
     if (t.bn == 32) return launch<T, 64, 32, 4, 1, false, false, 4>(p, 1, e, s);
-    if (t.bm == 64) return launch<T, 64, 64, 2, 2, false, false, 4>(p, 1, e, s);
+    if (t.bm == 64) return launch<T, 64, 64, 2, 2, false, false, 3>(p, 1, e, s);
   } else {
     if (t.bm == 64) return launch<T, 64, 64, 4, 1, false, false, 4>(p, 1, e, s);
   }
