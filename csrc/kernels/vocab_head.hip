@@ -24,13 +24,14 @@ __device__ __forceinline__ f32x4 vh_mma(const u32x4& a, const u32x4& b, f32x4 c)
   return mfma16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c);
 }
 
-// fp32 operands are multiplied on the bf16 matrix cores: a value is the sum of three bf16 values, each the rounding of what the
-// ones before it leave (8 + 8 + 8 bits and their signs hold all 24), products of two bf16 values are exact in the fp32
-// accumulators, and of the nine only the three below 2^-24 of the whole are left out:
-//   a b = a1 b1 + (a1 b2 + a2 b1) + (a1 b3 + a2 b2 + a3 b1) + at most 2^-23 |a b|
-// Six bf16 instructions do 16 x 16 x 32 in 96 cycles, the fp32 ones (16 x 16 x 4) take 256.  Values that round beyond bf16's
-// largest (3.39e38) count as infinite, and infinite ones give NaN (their second part is inf - inf).  Measured: 4096 x 1024 x
-// 16000 971 us with the fp32 instructions (138 TFLOP/s, their peak is 157), 660 this way.
+// fp32 operands are multiplied on the bf16 matrix cores: a value is the sum of three bf16 values, each the leading 8 bits of what
+// the ones before it leave (together all 24), products of two bf16 values are exact in the fp32 accumulators, and of the nine the
+// three smallest are left out:
+//   a b = a1 b1 + (a1 b2 + a2 b1) + (a1 b3 + a2 b2 + a3 b1) + at most 2^-21 |a b| (2^-23 on average)
+// Six bf16 instructions do 16 x 16 x 32 in 96 cycles, the fp32 ones (16 x 16 x 4) take 256.  An infinite value gives NaN (its
+// second part is inf - inf).  The leading bits are cut off, not rounded: the conversion instruction is several times slower than a
+// mask and a byte permutation, and rounding gains little (4096 x 1024 x 16000 forward: error of the log-sum-exp 5.6e-8 and
+// 6.5e-8, 605 and 567 us; with the fp32 instructions 971 us, 138 TFLOP/s of their 157).
 struct VhSplit {
   u32x4 part[3];
 };
@@ -42,12 +43,10 @@ __device__ __forceinline__ VhSplit vh_split(const u32x4& k0, const u32x4& k1) {
   for (int q = 0; q < 3; ++q)
 #pragma unroll
     for (int e = 0; e < 8; e += 2) {
-      typedef __attribute__((ext_vector_type(2))) bf16 bf16x2;
-      const bf16x2 h = {(bf16)v[e], (bf16)v[e + 1]};
-      const unsigned w = __builtin_bit_cast(unsigned, h);
-      s.part[q][e / 2] = w;
-      v[e] -= __builtin_bit_cast(float, w << 16);               // (both halves from the pair: one conversion, not three)
-      v[e + 1] -= __builtin_bit_cast(float, w & 0xffff0000u);
+      const unsigned lo = __builtin_bit_cast(unsigned, v[e]), hi = __builtin_bit_cast(unsigned, v[e + 1]);
+      s.part[q][e / 2] = __builtin_amdgcn_perm(hi, lo, 0x07060302u);
+      v[e] -= __builtin_bit_cast(float, lo & 0xffff0000u);
+      v[e + 1] -= __builtin_bit_cast(float, hi & 0xffff0000u);
     }
   return s;
 }
@@ -304,7 +303,7 @@ __device__ __forceinline__ void vh_mainloop(const VhOperands& p, Tile& c, char* 
           for (int j = 0; j < NTL; ++j) c.acc[i][j] = vh_mma(a.part[TERMS[q][0]], b[j].part[TERMS[q][1]], c.acc[i][j]);
         a = ahead;
         // the next fragment (44 vector instructions) is split in the shadow of this one's MFMAs, behind the first two, while it
-        // arrives (4096 x 1024 x 16000 forward 650 -> 608 us)
+        // arrives (4096 x 1024 x 16000 forward, 7 % less)
         if (i + 1 < MT) {
           constexpr int PER = (44 + 6 * NTL - 3) / (6 * NTL - 2);
           __builtin_amdgcn_sched_group_barrier(0x100, AS ? 8 : 2, 0);

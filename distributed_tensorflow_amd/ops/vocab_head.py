@@ -6,8 +6,8 @@
 The ten-class head of the engine keeps a row's logits in registers; here the classes may be a vocabulary.  Conventions are
 the engine's: rows of hidden units ``h`` [n, hidden], the weight transposed ``wT`` [classes, hidden], int32 labels, the
 per-row loss and everything that is summed in fp32; both operands bf16 (gradients of them bf16 as well, ``dwT`` on request
-fp32) or both fp32 (every product to within 2^-23, from three bf16 parts of each value on the bf16 matrix cores; values from
-3.39e38 on count as infinite, and infinite ones make NaN).  Rows of ``h`` and ``wT`` may be further apart than they are long; rows that
+fp32) or both fp32 (every product to within 2^-21, on average 2^-23, from three bf16 parts of each value on the bf16 matrix
+cores; infinite values make NaN).  Rows of ``h`` and ``wT`` may be further apart than they are long; rows that
 do not start on 16 bytes are copied once per call.
 
 A row whose label is ``ignore_label`` has loss 0 and takes no part in any gradient, whatever its hidden units hold

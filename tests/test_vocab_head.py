@@ -3,7 +3,7 @@
 Bounds (u = 2^-24, half = half a rounding step of the operand type):
   logits    a sum of H products, the rounding errors of its partial sums (each at most u times S_iv = sum_k |h_ik w_vk|) wander:
             e_z = 8 sqrt(H + 64) u S; the largest over a row counts for the row's log-sum-exp (fp32 products are themselves
-            off by 2^-23 = 2 u at most, which the 64 covers)
+            off by 2^-21 = 8 u at most, which the 64 covers)
   lse       e_lse = max_v e_z + 8 u (1 + |lse|)              loss  e_lse + e_z + 8 u (1 + |lse| + |z_y|)
   d         |s| (p (e_z + e_lse + 8 u (1 + |z| + |lse|)) + 2 u), and the rounding to the operand type: half |d|
   products  every error of d times the other factor, summed, plus the accumulation 8 sqrt(terms) u sum |d| |w|, plus half of
