@@ -986,8 +986,11 @@ GradTile dw_tile(int E, int cfg, int H, int classes) {
 // The large kinds run one workgroup per CU, so what counts is the number of rounds over the 256 CUs times the length of a round
 // (measured at H = 4096, against 256 x 256: 0.82 for 192 x 256, 0.68 for 256 x 128), and a last round for a few tiles is as long
 // as any other: its classes go to small tiles instead.  777 rows x 50001 classes: 784 tiles are four rounds, 362 us; three
-// rounds and 91 small tiles 330 us.  Logits that fill no round of small tiles are theirs altogether: a few large tiles take long
-// over their K (300 rows, 2048 x 5000, 200 small tiles: 30 and 20 us; fp32, whose tiles take longer, gains up to 768 of them).
+// rounds and 91 small tiles 330 us.  Logits of few tiles are cut as small as the
+// CUs hold them at once, because a workgroup alone on its CU takes long over its K (300 rows, 2048 x 5000 bf16: 30 us in large
+// tiles, 20 in 200 of 128 x 64; 526 rows, 2944 x 537 fp32: 101 us in 45 tiles of 128 x 64, 52 in 153 of 64 x 32).  Room for
+// 512 tiles in bf16 (500 rows, 1000 x 12000: 24 us large, 30 in 752 small ones), 768 in fp32, whose tiles take longer (600 rows,
+// 2048 x 8000: 180 us large, 170 in 630 small ones).
 struct LogitsTile {
   int bm, bn;
 };
@@ -999,7 +1002,15 @@ struct LogitsTiling {
 LogitsTiling logits_tiling(int E, int cfg, long n, int classes) {
   LogitsTiling q{{{128, 64}, {128, 64}}, classes, {0, 0}};
   if (cfg == kSmall || (E == 4 && cfg == kMid)) q.kind[0] = {64, E == 4 && n <= 32 ? 32 : 64};
-  if (cfg == kLarge && (long)cdiv(classes, 128) * cdiv(n, 64) > (E == 4 ? 768 : 512)) {
+  // the smallest tiles that all CUs hold at once
+  const long room = E == 4 ? 768 : 512;
+  bool few = false;
+  for (const LogitsTile& t : {LogitsTile{32, 32}, LogitsTile{64, 32}, LogitsTile{64, 64}, LogitsTile{128, 64}}) {
+    if (few || (E == 2 && (t.bn == 32 || cfg == kSmall)) || (t.bm == 128 && cfg != kLarge)) continue;
+    few = (long)cdiv(classes, t.bm) * cdiv(n, t.bn) <= room;
+    if (few) q.kind[0] = t;
+  }
+  if (cfg == kLarge && !few) {
     const struct { LogitsTile t; double length; } kinds[3] = {{{256, 256}, 1.0}, {{192, 256}, 0.82}, {{256, 128}, 0.68}};
     // small tiles: three to a CU; the first of a CU costs more than the next two
     auto small = [&](int rest) {
@@ -1049,6 +1060,7 @@ int logits(LogitsTile t, const VhOperands& p, const Epi& e, hipStream_t s) {
   // fp32: the fewer fragments of the rows' side a wave splits the better (one row, 1024 x 32000: 59 us with 64 rows' tiles of waves
   // side by side, 39 with 32 rows' ones; 64 rows, 1024 x 20000: 56 us side by side, 49 two by two)
   if constexpr (sizeof(T) == 4) {
+    if (t.bm == 32) return launch<T, 32, 32, 2, 2, false, false, 4>(p, 1, e, s);
     if (t.bn == 32) return launch<T, 64, 32, 4, 1, false, false, 4>(p, 1, e, s);
     if (t.bm == 64) return launch<T, 64, 64, 2, 2, false, false, 3>(p, 1, e, s);
   } else {

@@ -215,7 +215,10 @@ def test_pieces_bias_ignored_rows_and_row_scales(gpu_lib, n, hidden, classes, pi
     (1000, 40, 10007, 0),       # 192 x 256
     (777, 64, 50001, 0),        # three rounds of 256 x 256, the other classes in small tiles
     (2049, 72, 20011, 8192),    # pieces tiled differently
-    (130, 8, 70001, 0)])
+    (130, 8, 70001, 0),
+    (5, 48, 30000, 0),          # from here on what few rows and classes run: 64 x 32 tiles (fp32)
+    (2, 40, 60001, 0), (40, 24, 60001, 0), (100, 64, 20011, 0),     # 64 x 64
+    (150, 72, 20011, 0), (200, 72, 20011, 0)])                      # 128 x 64
 def test_every_tiling_of_the_logits(gpu_lib, n, hidden, classes, piece, dtype):
     h, w, y, b = make(n, hidden, classes, dtype, bias=True, ignored=0.1, seed=classes)
     y[:4] = torch.tensor([classes - 1, classes - 2, 0, 255], dtype=torch.int32, device=DEV)
