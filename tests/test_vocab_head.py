@@ -221,7 +221,7 @@ def test_pieces_bias_ignored_rows_and_row_scales(gpu_lib, n, hidden, classes, pi
     (150, 72, 20011, 0), (200, 72, 20011, 0)])                      # 128 x 64
 def test_every_tiling_of_the_logits(gpu_lib, n, hidden, classes, piece, dtype):
     h, w, y, b = make(n, hidden, classes, dtype, bias=True, ignored=0.1, seed=classes)
-    y[:4] = torch.tensor([classes - 1, classes - 2, 0, 255], dtype=torch.int32, device=DEV)
+    y[:4] = torch.tensor([classes - 1, classes - 2, 0, 255], dtype=torch.int32, device=DEV)[:n]
     check_all(h, w, y, b, grad_scale=1.0 / n, piece=piece)
 
 
