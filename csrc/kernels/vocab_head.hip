@@ -85,7 +85,8 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t vh_rsrc(const char* p, size_t 
 
 struct VhOperands {
   // Fast operand: [rows][K], ld elements between rows, k contiguous.  Slow operand: [K][rows], ld elements between the K
-  // rows, padded to 16 bytes.  Rows start on 16 bytes.  A fast operand's K is a multiple of 16 bytes.
+  // rows.  Rows start on 4 bytes, 16-byte LDS-DMAs need no more; their descriptors are checked for every 4 bytes, so that no read
+  // goes behind an operand.  What a fast operand's last 16 bytes of K hold behind K (its next row) meets zeros of the other one.
   const void *A, *B;
   long lda, ldb;
   int M, N, Ka, Kb;       // Ka, Kb: k from there on counts as zero
@@ -132,7 +133,7 @@ struct VhLoader {
     K = K_;
     rows = total - r0;
     if (SLOW) {
-      rows = (rows + 16 / E - 1) & ~(16 / E - 1);      // whole chunks: a slow operand's K rows are padded to them
+      rows = (rows + 4 / E - 1) & ~(4 / E - 1);        // whole words: an odd number of bf16 values is padded
       base = (const char*)p + (size_t)r0 * E;
     } else {
       base = (const char*)p + (size_t)r0 * ld;
@@ -1179,6 +1180,11 @@ template <typename T>
 T* at(void* ws, long o) { return (T*)((char*)ws + o - 1); }
 
 bool rows_ok(const void* p, long ld, int H, int E) { return !((uintptr_t)p & 15) && !(ld * E & 15) && !((long)H * E & 15); }
+// The weight is read where it lies if its rows start on 4 bytes and what follows a row of broken 16 bytes is the next row.  (16
+// rows, 4095 x 32000 fp32: copied first 332 us forward and 596 backward, read where it lies 116 and 399.)
+bool w_rows_ok(const void* p, long ld, int H, int E) {
+  return !((uintptr_t)p & 3) && !(ld * E & 3) && (!((long)H * E & 15) || ld == H);
+}
 
 template <typename T>
 int launch_copy(const T* src, long lds_, int R, int C, T* dst, long ldd, const int* labels, int ignore, long twin, hipStream_t s) {
@@ -1203,9 +1209,9 @@ template <typename T>
 int forward(const void* h, long ldh, const void* w, long ldw, const float* bias, const int* labels, int n, int H, int V, int ignore,
             void* loss, void* lse, void* ws, hipStream_t s) {
   const int E = sizeof(T);
-  const bool h_ok = rows_ok(h, ldh, H, E), w_ok = rows_ok(w, ldw, H, E);
+  const bool h_ok = rows_ok(h, ldh, H, E), w_ok = w_rows_ok(w, ldw, H, E);
   const Plan q = plan_for(E == 2 ? 1 : 0, 0, n, H, V, h_ok, w_ok, bias != nullptr, 0);
-  VhOperands p{w, h, ldw, ldh, V, n, (int)q.ldk, (int)q.ldk, 0, 0, 0, 0};
+  VhOperands p{w, h, ldw, ldh, V, n, H, (int)q.ldk, 0, 0, 0, 0};
   if (!h_ok) {
     VH_TRY(launch_copy((const T*)h, ldh, n, H, at<T>(ws, q.h_copy), q.ldk, nullptr, 0, 0, s));
     p.B = at<T>(ws, q.h_copy);
@@ -1215,6 +1221,7 @@ int forward(const void* h, long ldh, const void* w, long ldw, const float* bias,
     VH_TRY(launch_copy((const T*)w, ldw, V, H, at<T>(ws, q.w_copy), q.ldk, nullptr, 0, 0, s));
     p.A = at<T>(ws, q.w_copy);
     p.lda = q.ldk;
+    p.Ka = (int)q.ldk;
   }
   const LogitsTiling t = logits_tiling(E, q.cfg, n, V);
   VH_TRY(logits_all<T>(t, p, [&](int, int c0, int tile0) {
@@ -1231,7 +1238,7 @@ int backward(const void* h, long ldh, const void* w, long ldw, const float* bias
              const float* row_scale, float grad_scale, int n, int H, int V, int ignore, int piece, void* dh, void* dw, int dw_f32,
              void* db, void* ws, hipStream_t s) {
   const int E = sizeof(T), KT = 128 / E;
-  const Plan q = plan_for(E == 2 ? 1 : 0, 1, n, H, V, rows_ok(h, ldh, H, E), rows_ok(w, ldw, H, E), db != nullptr, piece);
+  const Plan q = plan_for(E == 2 ? 1 : 0, 1, n, H, V, rows_ok(h, ldh, H, E), w_rows_ok(w, ldw, H, E), db != nullptr, piece);
   const T* hp = at<T>(ws, q.h_copy);
   const int dn = q.parts * n;
   VH_TRY(launch_copy((const T*)h, ldh, n, H, at<T>(ws, q.h_copy), q.ldk, labels, ignore, q.parts == 2 ? n * q.ldk : 0, s));
@@ -1247,7 +1254,7 @@ int backward(const void* h, long ldh, const void* w, long ldw, const float* bias
     }
     T* d = at<T>(ws, q.d);
     const LogitsTiling t = logits_tiling(E, q.cfg, n, vn);
-    VH_TRY(logits_all<T>(t, VhOperands{wp, hp, ldwp, q.ldk, vn, n, (int)q.ldk, (int)q.ldk, 0, 0, 0, 0}, [&](int, int c0, int) {
+    VH_TRY(logits_all<T>(t, VhOperands{wp, hp, ldwp, q.ldk, vn, n, q.w_copy ? (int)q.ldk : H, (int)q.ldk, 0, 0, 0, 0}, [&](int, int c0, int) {
       return VhGradLogits{bias ? bias + v0 + c0 : nullptr, labels, lse, row_scale, v0 + c0, V, ignore, d + c0, ldv,
                           q.parts == 2 ? n * ldv : 0, (int)ldv - c0,
                           db ? at<float>(ws, q.dbpart) + c0 : nullptr};
@@ -1297,7 +1304,7 @@ long dtf_vocab_head_workspace(int dtype, int backward_pass, const void* h, long 
                               int bias, int piece) {
   if (!sizes_ok(dtype, n, H, V, ldh, ldw) || piece < 0 || piece > kMaxRow) return -3;
   const int E = esize(dtype);
-  return plan_for(dtype, backward_pass, n, H, V, rows_ok(h, ldh, H, E), rows_ok(w, ldw, H, E), bias != 0, piece).total;
+  return plan_for(dtype, backward_pass, n, H, V, rows_ok(h, ldh, H, E), w_rows_ok(w, ldw, H, E), bias != 0, piece).total;
 }
 
 // loss[n], lse[n] (fp32) of h [n][H] (rows ldh apart) against w [V][H] (rows ldw apart), bias [V] fp32 or NULL, labels int32

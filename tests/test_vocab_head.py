@@ -240,6 +240,23 @@ def test_every_tiling_of_the_gradients(gpu_lib, n, hidden, classes, dtype):
 
 @gpu
 @pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+@pytest.mark.parametrize("n,hidden,classes", [(1, 6, 40), (3, 74, 500), (70, 1002, 777), (300, 38, 3001), (520, 202, 2049), (150, 1001, 300)])
+def test_rows_that_start_on_four_bytes(gpu_lib, n, hidden, classes, dtype):
+    """Weights whose rows are no multiple of 16 bytes, read where they lie: at the end of their memory NaN follow."""
+    h, w, y, b = make(n, hidden, classes, dtype, bias=True, ignored=0.1 if n > 1 else 0.0, seed=hidden)
+    base = check_all(h, w, y, b, grad_scale=1.0 / n)
+    room = torch.full((classes * hidden + 64,), math.nan, device=DEV).to(w.dtype)
+    for start in (0, 2, 6):
+        v = room[start:start + classes * hidden].view(classes, hidden)
+        v.copy_(w)
+        loss, lse = vocab_head_fwd(h, v, y, b)
+        again = (loss, lse) + vocab_head_bwd(h, v, y, lse, b, grad_scale=1.0 / n)
+        assert all(torch.equal(a, c) for a, c in zip(base, again)), start
+        v.fill_(math.nan)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
 def test_strided_and_unaligned_rows(gpu_lib, dtype):
     h, w, y, b = make(70, 96, 400, dtype, bias=True, seed=4)
     base = check_all(h, w, y, b)
