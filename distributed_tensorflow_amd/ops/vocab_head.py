@@ -19,9 +19,9 @@ weight makes NaN, of its own class or of the one before it.
 The backward pass computes the logits again, one piece of the classes at a time: its workspace holds the gradient of the
 piece's logits in the operands' type (at most 2^27 values, or 1024 classes of very many rows), a copy of ``h`` without its
 ignored rows, fp32 sums of ``dh`` where there are several pieces or the classes are cut among workgroups, and the copies
-above.  Calls launch on the current stream of the operands'
-device, take their workspace from PyTorch's allocator on that stream and keep nothing, so they can be captured into HIP
-graphs and run on several streams at once.  Kernels: csrc/kernels/vocab_head.hip.
+above.  Calls launch on the current stream of the operands' device, take their workspace from PyTorch's allocator on that
+stream and keep nothing, so they can be captured into HIP graphs and run on several streams at once.
+Kernels: csrc/kernels/vocab_head.hip.
 """
 from __future__ import annotations
 
