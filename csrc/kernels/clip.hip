@@ -92,7 +92,7 @@ __device__ __forceinline__ long span_at(long e, int cols, long pitch) {
 // Walks the 16-byte vectors of a contiguous chunk, kDeep of them in flight per thread, then its last elements.  (Two to eight
 // are within 2 % for large lists; four is best for those of 10 to 100 MB, where eight leave chunks to the one-vector loop.)
 constexpr int kDeep = 4;
-constexpr int kKeepChunks = 3072;     // of 64 KB: 192 MB (smaller chunks belong to lists that fit the cache altogether)
+constexpr int kKeepChunks = 192 << 4;     // of 64 KB: 192 MB (smaller chunks belong to lists that fit the cache altogether)
 template <typename T, bool PASS_BY>
 __device__ __forceinline__ double chunk_sumsq(const ClipChunk& s) {
   constexpr int VE = 16 / sizeof(T);
