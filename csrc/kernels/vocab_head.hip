@@ -430,6 +430,51 @@ __device__ __forceinline__ void vh_mainloop(const VhOperands& p, Tile& c, char* 
   vh_barrier();
 }
 
+// dst[r][c] = src[r][c], r < R, with rows ldd apart (16-byte multiples), columns C .. ldd - 1 zero and rows from `rows` on zero.
+// labels given: the rows of ignored labels are zero as well -- whatever lies there, 0 * NaN must not reach a gradient.  Whole
+// 16-byte chunks from any element of a row (global memory takes unaligned vector loads), the last chunk of a row element by
+// element.  twin: elements to a second copy (0: none).
+struct VhCopy {
+  const void* src;
+  long lds_;
+  int R, rows, C;
+  void* dst;
+  long ldd;
+  const int* labels;
+  int ignore;
+  long twin;
+  int blocks;           // workgroups that do this besides a product (0: a launch of its own)
+};
+template <typename T>
+__device__ __forceinline__ void vh_copy_rows(const VhCopy& c, long first, long step) {
+  constexpr int V = 16 / sizeof(T);
+  typedef __attribute__((ext_vector_type(V))) T vec;
+  typedef vec vec_any __attribute__((aligned(sizeof(T))));
+  const int per = (int)(c.ldd / V);
+  const long n = (long)c.R * per;
+  for (long x = first; x < n; x += step) {
+    const long r = n >> 32 ? x / per : (long)((unsigned)x / (unsigned)per);
+    const int i = (int)(x - r * per) * V;
+    vec v;
+#pragma unroll
+    for (int e = 0; e < V; ++e) v[e] = (T)0.f;
+    if (r < c.rows && !(c.labels && c.labels[r] == c.ignore)) {
+      const T* p = (const T*)c.src + r * c.lds_ + i;
+      if (i + V <= c.C) {
+        const vec y = *reinterpret_cast<const vec_any*>(p);
+        v = y;
+      } else {
+#pragma unroll
+        for (int e = 0; e < V; ++e)
+          if (i + e < c.C) v[e] = p[e];
+      }
+    }
+    T* const o = (T*)c.dst + r * c.ldd + i;
+    *reinterpret_cast<vec*>(o) = v;
+    if (c.twin) *reinterpret_cast<vec*>(o + c.twin) = v;
+  }
+}
+
 // Which tile and which split a workgroup takes.  Workgroups are dealt round-robin over the 8 XCDs; each XCD gets one run of the
 // (split, band of four tile rows, column) order, so that its L2 serves all tiles of a split from one fetch of the split's
 // operands.
@@ -453,6 +498,13 @@ __global__ __launch_bounds__(NWM * NWN * 64, 1) void vh_gemm(VhOperands p, Epi e
   typedef typename Epi::template Inputs<BM, BN> Inputs;
   __shared__ __attribute__((aligned(16))) char lds[D * (BM + BN) * 128 + sizeof(Inputs)];
   Inputs& in = *reinterpret_cast<Inputs*>(lds + D * (BM + BN) * 128);
+  if constexpr (Epi::kCopies) {         // the workgroups behind the tiles
+    const int tiles = p.tiles_m * p.tiles_n * p.splits;
+    if ((int)blockIdx.x >= tiles) {
+      vh_copy_rows<T>(e.copy, (long)(blockIdx.x - tiles) * Tile::NT + threadIdx.x, (long)e.copy.blocks * Tile::NT);
+      return;
+    }
+  }
   Tile c;
   c.lane = threadIdx.x & 63;
   c.wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -536,6 +588,7 @@ __device__ __forceinline__ MaxSum join(MaxSum a, MaxSum b) {
 
 // Forward: i = class, j = row.  part[class tile][row] = (maximum, sum) in base 2, zlab[row] = the label's logit.
 struct VhForward {
+  static constexpr bool kCopies = false;
   const float* bias;
   const int* labels;
   int c0;                   // the product's first class
@@ -608,19 +661,23 @@ struct VhForward {
 // d is rounded to the operand type because the two products that read it multiply in that type: at most half a step of each
 // value, summed in fp32.  The common factor grad_scale is left to those products' epilogues: 1/n times a label's -(1 - p), the
 // value that outweighs all others of its row and class, would be rounded the same way for every row.  With up to 32 rows, half
-// a tile of them, the rounding errors themselves are kept as n more rows, next to nothing in time: one row's gradient is then as
+// a tile of them, the rounding errors themselves are kept as rows 32 to 63, next to nothing in time: one row's gradient is then as
 // exact as if d had stayed in fp32 (one row: 0.17 % rms, the operand type's own rounding, instead of up to 0.4; 16 rows, 4096 x
 // 32000, backward 161 -> 166 us.  For 64 rows, a second tile, it would be 168 -> 211 us, and errors of many rows even out.)
 struct VhGradLogits {
+  static constexpr bool kCopies = true;
+  VhCopy copy;              // h for dw: does not depend on d and needs no launch of its own
   const float* bias;        // of the piece
   const int* labels;
   const float* lse;
   const float* row_scale;   // or nullptr
   int v0, classes, ignore;  // the product's first class, all classes
   void* d;
-  long ldd, rest;           // elements from a row to the row of its rounding errors (0: not kept)
+  long ldd, rest;           // elements from a row to the row of its rounding errors (0: not kept; else rows up to 32 are written)
   int places;               // of this product's classes: up to there d is written
   float* dbpart;            // [row tile][ldd] or nullptr
+  int dbplaces;             // up to there it is written
+  float dbscale;
   template <int BM, int BN> using Inputs = VhLogitsInputs<BM, BN>;
   __device__ __forceinline__ VhRowInputs row_inputs(int row, int m0) const {
     const int y = labels[row];
@@ -649,7 +706,7 @@ struct VhGradLogits {
 #pragma unroll
     for (int j = 0; j < NTL; ++j) {
       const int jl = c.wn0 + 16 * j + i16, row = c.n0 + jl;
-      const bool live = row < p.N;
+      const bool live = row < (REST && rest ? 32 : p.N);
       const VhRowInputs x = in.row[jl];
       const int y = x.label - (c.wm0 + 4 * g);
       const bool hit = y >= 0 && y < Tile::WM, dead = x.sc == 0.f;
@@ -711,7 +768,7 @@ struct VhGradLogits {
       float s = red[0][i];
 #pragma unroll
       for (int w = 1; w < NWN; ++w) s += red[w][i];
-      if (c.m0 + i < places) dbpart[(long)ty * ldd + c.m0 + i] = s;
+      if (c.m0 + i < dbplaces) dbpart[(long)ty * ldd + c.m0 + i] = s * dbscale;
     }
   }
 };
@@ -722,6 +779,7 @@ struct VhGradLogits {
 // be kept in the caches (a template argument: as a value the compiler folds the two kinds of stores into the plain one).
 template <bool ONCE>
 struct VhStoreT {
+  static constexpr bool kCopies = false;
   void* out;
   long ldo;
   int out_f32;
@@ -730,6 +788,7 @@ struct VhStoreT {
   float* sum;
   int first, last;
   float scale;              // of what goes to out
+  int fold;                 // rows 32 to 63 are added to 0 to 31
   // V values of a row, from the wave's staging rows to where they belong
   template <typename T, int V>
   __device__ __forceinline__ void put(const float* src, long row, int m, int M, int split) const {
@@ -804,6 +863,13 @@ struct VhStoreT {
     float* const st = reinterpret_cast<float*>(lds) + c.wave * 16 * PITCH;
     const int i16 = c.lane & 15, g = c.lane >> 4;
     const int rl = c.lane / LPR, cl = (c.lane % LPR) * V, m = c.m0 + c.wm0 + cl;
+    if constexpr (sizeof(T) == 2 && NWN == 1 && NTL == 4) {       // (the few rows' dh)
+      if (fold)
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) c.acc[i][j] += c.acc[i][j + 2];
+    }
 #pragma unroll
     for (int j = 0; j < NTL; ++j) {
 #pragma unroll
@@ -876,38 +942,9 @@ __global__ __launch_bounds__(256) void vh_dbias(const float* __restrict__ part, 
   db[v] = s * scale;
 }
 
-// dst[r][c] = src[r][c] with rows ldd apart (16-byte multiples), columns C .. ldd - 1 zero.  labels given: the rows of
-// ignored labels are zero as well -- whatever lies there, 0 * NaN must not reach a gradient.  Whole 16-byte chunks from any
-// element of a row (global memory takes unaligned vector loads), the last chunk of a row element by element.  twin: elements to
-// a second copy (0: none).
 template <typename T>
-__global__ __launch_bounds__(256) void vh_copy(const T* __restrict__ src, long lds_, int R, int C, T* __restrict__ dst, long ldd,
-                                               const int* __restrict__ labels, int ignore, long twin) {
-  constexpr int V = 16 / sizeof(T);
-  typedef __attribute__((ext_vector_type(V))) T vec;
-  typedef vec vec_any __attribute__((aligned(sizeof(T))));
-  const int per = (int)(ldd / V);
-  const long n = (long)R * per;
-  for (long x = (long)blockIdx.x * 256 + threadIdx.x; x < n; x += (long)gridDim.x * 256) {
-    const long r = n >> 32 ? x / per : (long)((unsigned)x / (unsigned)per);
-    const int i = (int)(x - r * per) * V;
-    vec v;
-#pragma unroll
-    for (int e = 0; e < V; ++e) v[e] = (T)0.f;
-    if (!(labels && labels[r] == ignore)) {
-      const T* p = src + r * lds_ + i;
-      if (i + V <= C) {
-        const vec y = *reinterpret_cast<const vec_any*>(p);
-        v = y;
-      } else {
-#pragma unroll
-        for (int e = 0; e < V; ++e)
-          if (i + e < C) v[e] = p[e];
-      }
-    }
-    *reinterpret_cast<vec*>(dst + r * ldd + i) = v;
-    if (twin) *reinterpret_cast<vec*>(dst + twin + r * ldd + i) = v;
-  }
+__global__ __launch_bounds__(256) void vh_copy(VhCopy c) {
+  vh_copy_rows<T>(c, (long)blockIdx.x * 256 + threadIdx.x, (long)gridDim.x * 256);
 }
 
 // out[i] = scale * sum of the slabs, in order, eight loads in flight
@@ -1047,7 +1084,8 @@ int launch(VhOperands p, int splits, const Epi& e, hipStream_t s) {
   p.tiles_n = cdiv(p.N, BN);
   p.ktiles = cdiv(p.Ka > p.Kb ? p.Ka : p.Kb, 128 / sizeof(T));
   p.splits = splits;
-  const long grid = (long)p.tiles_m * p.tiles_n * splits;
+  long grid = (long)p.tiles_m * p.tiles_n * splits;
+  if constexpr (Epi::kCopies) grid += e.copy.blocks;
   if (grid > 0x7fffffff) return -1;
   hipLaunchKernelGGL((vh_gemm<T, BM, BN, NWM, NWN, AS, BS, D, Epi>), dim3((unsigned)grid), dim3(NWM * NWN * 64), 0, s, p, e);
   return (int)hipGetLastError();
@@ -1123,7 +1161,7 @@ struct Plan {
   long total;
   long ldk, ldv;            // padded hidden units, classes of a piece
   int cfg, piece, pieces, splits_h, splits_w;
-  int parts;                // rows of d per row of h: 2 with its rounding errors kept
+  int parts, drows;         // parts == 2: d has 64 rows, its rounding errors from row 32 on
   GradTile tile_h, tile_w;
 };
 
@@ -1150,7 +1188,8 @@ Plan plan_for(int dtype, int backward, long n, int H, int V, bool h_ok, bool w_o
   q.cfg = config_for(n);
   q.ldk = up(H, 16 / E);
   q.parts = backward && E == 2 && n <= 32 ? 2 : 1;
-  const long dn = q.parts * n;
+  q.drows = q.parts == 2 ? 64 : (int)n;
+  const long dn = q.drows;
   if (!h_ok || backward) q.h_copy = take(dn * q.ldk * E);
   q.piece = backward ? (piece > 0 ? (int)up(piece, kPiece) : piece_for(n, V)) : V;
   if (q.piece > V) q.piece = V;
@@ -1168,7 +1207,7 @@ Plan plan_for(int dtype, int backward, long n, int H, int V, bool h_ok, bool w_o
     q.tile_w = dw_tile(E, q.cfg, H, q.piece);
     q.splits_h = splits_for((long)cdiv(H, q.tile_h.bm) * cdiv(dn, q.tile_h.bn), cdiv(q.ldv, KT), q.tile_h.want);
     q.splits_w = splits_for((long)cdiv(H, q.tile_w.bm) * cdiv(q.piece, q.tile_w.bn), cdiv(dn, KT), q.tile_w.want);
-    if (q.pieces > 1 || q.splits_h * q.parts > 1) q.sum_h = take(q.splits_h * dn * H * 4);
+    if (q.pieces > 1 || q.splits_h > 1) q.sum_h = take(q.splits_h * n * H * 4);
     if (q.splits_w > 1) q.sum_w = take(q.splits_w * (long)q.piece * H * 4);
     if (bias) q.dbpart = take((long)cdiv(n, 32) * q.ldv * 4);      // at most that many row tiles
   }
@@ -1187,10 +1226,10 @@ bool w_rows_ok(const void* p, long ld, int H, int E) {
 }
 
 template <typename T>
-int launch_copy(const T* src, long lds_, int R, int C, T* dst, long ldd, const int* labels, int ignore, long twin, hipStream_t s) {
-  const long chunks = (long)R * (ldd * (long)sizeof(T) / 16);
+int launch_copy(const VhCopy& c, hipStream_t s) {
+  const long chunks = (long)c.R * (c.ldd * (long)sizeof(T) / 16);
   const int grid = chunks > 16384L * 256 ? 16384 : cdiv(chunks, 256);
-  hipLaunchKernelGGL(vh_copy<T>, dim3(grid), dim3(256), 0, s, src, lds_, R, C, dst, ldd, labels, ignore, twin);
+  hipLaunchKernelGGL(vh_copy<T>, dim3(grid), dim3(256), 0, s, c);
   return (int)hipGetLastError();
 }
 template <typename O>
@@ -1213,12 +1252,12 @@ int forward(const void* h, long ldh, const void* w, long ldw, const float* bias,
   const Plan q = plan_for(E == 2 ? 1 : 0, 0, n, H, V, h_ok, w_ok, bias != nullptr, 0);
   VhOperands p{w, h, ldw, ldh, V, n, H, (int)q.ldk, 0, 0, 0, 0};
   if (!h_ok) {
-    VH_TRY(launch_copy((const T*)h, ldh, n, H, at<T>(ws, q.h_copy), q.ldk, nullptr, 0, 0, s));
+    VH_TRY(launch_copy<T>(VhCopy{h, ldh, n, n, H, at<T>(ws, q.h_copy), q.ldk, nullptr, 0, 0, 0}, s));
     p.B = at<T>(ws, q.h_copy);
     p.ldb = q.ldk;
   }
   if (!w_ok) {
-    VH_TRY(launch_copy((const T*)w, ldw, V, H, at<T>(ws, q.w_copy), q.ldk, nullptr, 0, 0, s));
+    VH_TRY(launch_copy<T>(VhCopy{w, ldw, V, V, H, at<T>(ws, q.w_copy), q.ldk, nullptr, 0, 0, 0}, s));
     p.A = at<T>(ws, q.w_copy);
     p.lda = q.ldk;
     p.Ka = (int)q.ldk;
@@ -1238,30 +1277,43 @@ int backward(const void* h, long ldh, const void* w, long ldw, const float* bias
              const float* row_scale, float grad_scale, int n, int H, int V, int ignore, int piece, void* dh, void* dw, int dw_f32,
              void* db, void* ws, hipStream_t s) {
   const int E = sizeof(T), KT = 128 / E;
-  const Plan q = plan_for(E == 2 ? 1 : 0, 1, n, H, V, rows_ok(h, ldh, H, E), w_rows_ok(w, ldw, H, E), db != nullptr, piece);
+  const bool h_ok = rows_ok(h, ldh, H, E);
+  const Plan q = plan_for(E == 2 ? 1 : 0, 1, n, H, V, h_ok, w_rows_ok(w, ldw, H, E), db != nullptr, piece);
   const T* hp = at<T>(ws, q.h_copy);
-  const int dn = q.parts * n;
-  VH_TRY(launch_copy((const T*)h, ldh, n, H, at<T>(ws, q.h_copy), q.ldk, labels, ignore, q.parts == 2 ? n * q.ldk : 0, s));
+  const int dn = q.drows;
+  VhCopy copy{h, ldh, q.parts == 2 ? 32 : n, n, H, at<T>(ws, q.h_copy), q.ldk, labels, ignore, q.parts == 2 ? 32 * q.ldk : 0, 0};
+  // Only dw needs the copy where h is aligned: few rows are copied next to the first product (16 rows, 4096 x 32000: 4.5 us less);
+  // among large tiles, which hold a CU each, the copy is a launch of its own.
+  const bool beside = h_ok && q.cfg != kLarge;
+  if (beside) copy.blocks = (int)(copy.R * (q.ldk * E / 16) / 1024 + 1);
+  else VH_TRY(launch_copy<T>(copy, s));
+  const T* hl = beside ? (const T*)h : hp;
+  const long ldl = beside ? ldh : q.ldk;
   for (int k = 0; k < q.pieces; ++k) {
     const int v0 = k * q.piece, vn = V - v0 < q.piece ? V - v0 : q.piece;
     const long ldv = up(vn, KT);
     const T* wp = (const T*)w + (long)v0 * ldw;
     long ldwp = ldw;
     if (q.w_copy) {
-      VH_TRY(launch_copy(wp, ldw, vn, H, at<T>(ws, q.w_copy), q.ldk, nullptr, 0, 0, s));
+      VH_TRY(launch_copy<T>(VhCopy{wp, ldw, vn, vn, H, at<T>(ws, q.w_copy), q.ldk, nullptr, 0, 0, 0}, s));
       wp = at<T>(ws, q.w_copy);
       ldwp = q.ldk;
     }
     T* d = at<T>(ws, q.d);
     const LogitsTiling t = logits_tiling(E, q.cfg, n, vn);
-    VH_TRY(logits_all<T>(t, VhOperands{wp, hp, ldwp, q.ldk, vn, n, q.w_copy ? (int)q.ldk : H, (int)q.ldk, 0, 0, 0, 0}, [&](int, int c0, int) {
-      return VhGradLogits{bias ? bias + v0 + c0 : nullptr, labels, lse, row_scale, v0 + c0, V, ignore, d + c0, ldv,
-                          q.parts == 2 ? n * ldv : 0, (int)ldv - c0,
-                          db ? at<float>(ws, q.dbpart) + c0 : nullptr};
+    VH_TRY(logits_all<T>(t, VhOperands{wp, hl, ldwp, ldl, vn, n, q.w_copy ? (int)q.ldk : H, (int)q.ldk, 0, 0, 0, 0}, [&](int part, int c0, int) {
+      VhCopy now = copy;
+      if (k || part) now.blocks = 0;
+      // one tile of rows: its sums are the whole ones
+      const bool whole = n <= t.kind[part].bn;
+      float* dbp = !db ? nullptr : whole ? (float*)db + v0 + c0 : at<float>(ws, q.dbpart) + c0;
+      return VhGradLogits{now, bias ? bias + v0 + c0 : nullptr, labels, lse, row_scale, v0 + c0, V, ignore, d + c0, ldv,
+                          q.parts == 2 ? 32 * ldv : 0, (int)ldv - c0, dbp, whole ? (part ? vn - t.first : t.first) : (int)ldv - c0,
+                          whole ? grad_scale : 1.f};
     }, s));
     for (int part = 0; db && part < 2; ++part) {
       const int c0 = part ? t.first : 0, cn = part ? vn - t.first : t.first;
-      if (!cn) continue;
+      if (!cn || n <= t.kind[part].bn) continue;
       hipLaunchKernelGGL(vh_dbias, dim3(cdiv(cn, 256)), dim3(256), 0, s, at<float>(ws, q.dbpart) + c0, ldv, cdiv(n, t.kind[part].bn),
                          (float*)db + v0 + c0, cn, grad_scale);
       VH_TRY((int)hipGetLastError());
@@ -1274,17 +1326,17 @@ int backward(const void* h, long ldh, const void* w, long ldw, const float* bias
       const bool once = !split && (long)V * H * (dw_f32 ? 4 : E) >= (64L << 20);
       const VhOperands o{hp, d, q.ldk, ldv, H, (int)ldv, dn, dn, 0, 0, 0, 0};
       float* sum = split ? at<float>(ws, q.sum_w) : nullptr;
-      if (once) VH_TRY((product_dw<T>(q.tile_w, o, 1, VhStoreT<true>{out, H, dw_f32, 1, vn, sum, 1, 1, grad_scale}, s)));
-      else VH_TRY((product_dw<T>(q.tile_w, o, q.splits_w, VhStore{out, H, dw_f32, 1, vn, sum, 1, !split, grad_scale}, s)));
+      if (once) VH_TRY((product_dw<T>(q.tile_w, o, 1, VhStoreT<true>{out, H, dw_f32, 1, vn, sum, 1, 1, grad_scale, 0}, s)));
+      else VH_TRY((product_dw<T>(q.tile_w, o, q.splits_w, VhStore{out, H, dw_f32, 1, vn, sum, 1, !split, grad_scale, 0}, s)));
       if (split)
         VH_TRY(dw_f32 ? launch_sum(at<float>(ws, q.sum_w), (long)vn * H, q.splits_w, (float*)out, grad_scale, s)
                       : launch_sum(at<float>(ws, q.sum_w), (long)vn * H, q.splits_w, (T*)out, grad_scale, s));
     }
     if (dh) {
-      const bool last = k == q.pieces - 1, split = q.splits_h * q.parts > 1;
-      VhStore st{dh, H, 0, 0, dn, q.sum_h ? at<float>(ws, q.sum_h) : nullptr, k == 0, last && !split, grad_scale};
+      const bool last = k == q.pieces - 1, split = q.splits_h > 1;
+      VhStore st{dh, H, 0, 0, n, q.sum_h ? at<float>(ws, q.sum_h) : nullptr, k == 0, last && !split, grad_scale, q.parts == 2};
       VH_TRY((product_dh<T>(q.cfg, q.tile_h, VhOperands{wp, d, ldwp, ldv, H, dn, vn, (int)ldv, 0, 0, 0, 0}, q.splits_h, st, s)));
-      if (last && split) VH_TRY(launch_sum(at<float>(ws, q.sum_h), (long)n * H, q.splits_h * q.parts, (T*)dh, grad_scale, s));
+      if (last && split) VH_TRY(launch_sum(at<float>(ws, q.sum_h), (long)n * H, q.splits_h, (T*)dh, grad_scale, s));
     }
   }
   return 0;
