@@ -17,7 +17,6 @@
 namespace dtf {
 
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kLn2 = 0.6931471805599453f;
 typedef f32x4 f32x4_any __attribute__((aligned(4)));
 
 __device__ __forceinline__ f32x4 vh_mma(const u32x4& a, const u32x4& b, f32x4 c) {
@@ -30,11 +29,14 @@ __device__ __forceinline__ f32x4 vh_mma(const u32x4& a, const u32x4& b, f32x4 c)
 //   a b = a1 b1 + (a1 b2 + a2 b1) + (a1 b3 + a2 b2 + a3 b1) + at most 2^-21 |a b| (2^-23 on average)
 // Six bf16 instructions do 16 x 16 x 32 in 96 cycles, the fp32 ones (16 x 16 x 4) take 256.  An infinite value gives NaN (its
 // second part is inf - inf).  The leading bits are cut off, not rounded: the conversion instruction is several times slower than a
-// mask and a byte permutation, and rounding gains little (4096 x 1024 x 16000 forward: error of the log-sum-exp 5.6e-8 and
-// 6.5e-8, 605 and 567 us; with the fp32 instructions 971 us, 138 TFLOP/s of their 157).
+// mask and a byte permutation (4096 x 1024 x 16000 forward 605 and 567 us; with the fp32 instructions 971, 138 TFLOP/s of their
+// 157).  ROUND: the first part is rounded (half a step added before the cut), so that what is left out has no sign of its own (at
+// most 2^-22): one instruction more per value, for few rows, whose single losses show it (1 x 300 x 700, lse near its label's
+// logit: loss off by 4.6e-6 of itself, 1.2e-6 with it).  Values that round beyond 3.39e38 count as infinite there.
 struct VhSplit {
   u32x4 part[3];
 };
+template <bool ROUND>
 __device__ __forceinline__ VhSplit vh_split(const u32x4& k0, const u32x4& k1) {
   const f32x4 x = __builtin_bit_cast(f32x4, k0), y = __builtin_bit_cast(f32x4, k1);
   float v[8] = {x[0], x[1], x[2], x[3], y[0], y[1], y[2], y[3]};
@@ -43,7 +45,8 @@ __device__ __forceinline__ VhSplit vh_split(const u32x4& k0, const u32x4& k1) {
   for (int q = 0; q < 3; ++q)
 #pragma unroll
     for (int e = 0; e < 8; e += 2) {
-      const unsigned lo = __builtin_bit_cast(unsigned, v[e]), hi = __builtin_bit_cast(unsigned, v[e + 1]);
+      const unsigned half = ROUND && q == 0 ? 0x8000u : 0u;
+      const unsigned lo = __builtin_bit_cast(unsigned, v[e]) + half, hi = __builtin_bit_cast(unsigned, v[e + 1]) + half;
       s.part[q][e / 2] = __builtin_amdgcn_perm(hi, lo, 0x07060302u);
       v[e] -= __builtin_bit_cast(float, lo & 0xffff0000u);
       v[e + 1] -= __builtin_bit_cast(float, hi & 0xffff0000u);
@@ -289,19 +292,28 @@ __device__ __forceinline__ void vh_mainloop(const VhOperands& p, Tile& c, char* 
       else vh_wait<0>();
       vh_barrier();
       if (t + D - 1 < t1) dma(t + D - 1, last);
+      // Few rows' logits: a K tile is summed by itself and then added, one rounding of the long sum instead of six (3 rows, 3883 x
+      // 3931: losses off by up to 2.0e-6 of themselves, 3.9e-7 with it; 100 rows, 1024 x 10000: 3.4e-7 and 8.6e-8).  Large tiles
+      // have no room for it among their vector instructions.
+      constexpr bool FEW = MT * NTL <= 4;
       VhSplit b[NTL];
 #pragma unroll
-      for (int j = 0; j < NTL; ++j) b[j] = vh_split(rb.one(buf + ABYTES, 0, j), rb.one(buf + ABYTES, 1, j));
-      VhSplit a = vh_split(ra.one(buf, 0, 0), ra.one(buf, 1, 0));
+      for (int j = 0; j < NTL; ++j) b[j] = vh_split<FEW>(rb.one(buf + ABYTES, 0, j), rb.one(buf + ABYTES, 1, j));
+      VhSplit a = vh_split<FEW>(ra.one(buf, 0, 0), ra.one(buf, 1, 0));
 #pragma unroll
       for (int i = 0; i < MT; ++i) {
         constexpr int TERMS[6][2] = {{0, 2}, {2, 0}, {1, 1}, {0, 1}, {1, 0}, {0, 0}};      // the smallest first
         VhSplit ahead = a;
-        if (i + 1 < MT) ahead = vh_split(ra.one(buf, 0, i + 1), ra.one(buf, 1, i + 1));
+        if (i + 1 < MT) ahead = vh_split<FEW>(ra.one(buf, 0, i + 1), ra.one(buf, 1, i + 1));
+        f32x4 sum[NTL];
+#pragma unroll
+        for (int j = 0; j < NTL; ++j) sum[j] = FEW ? (f32x4){0.f, 0.f, 0.f, 0.f} : c.acc[i][j];
 #pragma unroll
         for (int q = 0; q < 6; ++q)
 #pragma unroll
-          for (int j = 0; j < NTL; ++j) c.acc[i][j] = vh_mma(a.part[TERMS[q][0]], b[j].part[TERMS[q][1]], c.acc[i][j]);
+          for (int j = 0; j < NTL; ++j) sum[j] = vh_mma(a.part[TERMS[q][0]], b[j].part[TERMS[q][1]], sum[j]);
+#pragma unroll
+        for (int j = 0; j < NTL; ++j) c.acc[i][j] = FEW ? c.acc[i][j] + sum[j] : sum[j];
         a = ahead;
         // the next fragment (44 vector instructions) is split in the shadow of this one's MFMAs, behind the first two, while it
         // arrives (4096 x 1024 x 16000 forward, 7 % less)
@@ -926,10 +938,13 @@ __global__ __launch_bounds__(256) void vh_join(const float2* __restrict__ part, 
   }
   if (sl || row >= n) return;
   a = red[0][rl];
-  const float l = kLn2 * (a.m + __builtin_amdgcn_logf(a.s));     // (the hardware's base-2 logarithm, one step of error)
-  lse[row] = l;
+  // In 64 bits: a loss near zero is the difference of two large numbers.  The exponent of the sum apart, so that the hardware's
+  // logarithm (base 2, of 1/2 to 1) is off by a step of 1 at most; divided by the float that the logits were multiplied with.
+  const double l = ((double)a.m + (__builtin_amdgcn_frexp_expf(a.s) + (double)__builtin_amdgcn_logf(__builtin_amdgcn_frexp_mantf(a.s)))) /
+                   (double)kLog2e;
+  lse[row] = (float)l;
   const int y = labels[row];
-  loss[row] = y == ignore ? 0.f : (y >= 0 && y < classes ? l - zlab[row] : __builtin_nanf(""));
+  loss[row] = y == ignore ? 0.f : (y >= 0 && y < classes ? (float)(l - (double)zlab[row]) : __builtin_nanf(""));
 }
 
 // db[v] = scale * sum of the row tiles' partial sums, in order
