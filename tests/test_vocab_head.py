@@ -514,8 +514,10 @@ def test_few_rows_keep_what_rounding_drops(gpu_lib, n, classes, piece):
 
 # ---------------------------------------------------------------------------------------------- streams and graphs
 @gpu
-def test_graph_replays_and_streams(gpu_lib):
-    a = make(130, 64, 900, "bf16", bias=True, ignored=0.2, seed=20)
+@pytest.mark.parametrize("n,hidden,classes,dtype", [(130, 64, 900, "bf16"), (5, 64, 900, "bf16"), (20, 37, 700, "fp32"),
+                                                    (40, 33, 900, "bf16"), (300, 72, 2100, "fp32")])
+def test_graph_replays_and_streams(gpu_lib, n, hidden, classes, dtype):
+    a = make(n, hidden, classes, dtype, bias=True, ignored=0.2, seed=20)
     graphs, results = [], []
     for _ in range(2):
         torch.cuda.synchronize()
@@ -525,7 +527,7 @@ def test_graph_replays_and_streams(gpu_lib):
             results.append((loss, lse) + vocab_head_bwd(a[0], a[1], a[2], lse, a[3], piece=256))
         graphs.append(g)
     for rep in range(3):
-        fresh = make(130, 64, 900, "bf16", bias=True, ignored=0.2, seed=30 + rep)
+        fresh = make(n, hidden, classes, dtype, bias=True, ignored=0.2, seed=30 + rep)
         for t, f in zip(a, fresh):
             t.copy_(f)
         loss, lse = vocab_head_fwd(*a)
