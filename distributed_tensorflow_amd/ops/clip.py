@@ -6,10 +6,12 @@
 
 The plan is made once for tensors that stay where they are (gradient arenas, as everywhere in this package) and holds
 nothing but a table of their addresses and shapes in device memory; each call computes the norm anew from the values that
-the tensors then have.  Launches go to the current stream of the tensors' device and can be captured into a HIP graph (the
-plan has to outlive it): the table is only read, the workspace of a call comes from PyTorch's allocator on that stream, so
-calls on different streams and in different graphs share nothing that is written.  As in TensorFlow, a norm that is not
-finite makes every clipped value NaN.
+the tensors then have.  A tensor whose memory is replaced (a gradient that is made anew each step) needs a new plan, which
+costs a copy to the device and a wait for it and cannot be made while a stream is captured.  Launches go to the current
+stream of the tensors' device: the table is only read, the workspace of a call comes from PyTorch's allocator on that
+stream, so calls on different streams and in different graphs share nothing that is written.  A plan may be dropped while
+its calls still run on any stream; one whose call was captured into a HIP graph has to outlive the graph and its replays.
+As in TensorFlow, a norm that is not finite makes every clipped value NaN.
 Kernels: csrc/kernels/clip.hip.
 """
 from __future__ import annotations
@@ -142,7 +144,7 @@ class GlobalNormClip:
         if self.device.type != "cuda":
             raise ValueError(f"GPU tensors expected, got {self.device} (ops.reference.clip_by_global_norm runs on the CPU)")
         self.lib = native.load()
-        self._keep = ([t.detach() for t in tensors], [o.detach() for o in outs])     # the memory stays allocated
+        kept = [t.detach() for t in tensors] + [o.detach() for o in outs]            # the memory stays allocated
         self.out = list(outs)
         in_place = ctypes.c_int()
         chunks = int(self.lib.dtf_clip_table(len(tensors), spans, None, 0, ctypes.byref(in_place)))
@@ -152,6 +154,9 @@ class GlobalNormClip:
         self.table = host.to(self.device)                # 64 bytes per chunk, the same for every call
         # every other stream may read the table from here on: the copy is done
         torch.cuda.current_stream(self.device).synchronize()
+        self._memory = [self.table] + list({t.untyped_storage().data_ptr(): t for t in kept if t.numel()}.values())
+        self._keep, self._streams = kept, set()
+        self._used_on(torch.cuda.current_stream(self.device).cuda_stream)
         self.chunks, self._in_place = chunks, in_place.value
         self.slots = int(self.lib.dtf_clip_partials(chunks))    # fp64 words of a call's workspace
 
@@ -159,10 +164,22 @@ class GlobalNormClip:
         dev = self.device
         return torch.empty(self.slots, dtype=torch.float64, device=dev), torch.empty((), dtype=torch.float32, device=dev)
 
+    def _used_on(self, stream: int):
+        """Called on the current stream, whose handle is ``stream``.  The allocator hands out the memory of a dropped plan (its
+        table, and tensors that nobody else keeps) as soon as the streams recorded for it have done what they were given
+        until then, so every stream that a call goes to is recorded, once."""
+        if stream in self._streams or torch.cuda.is_current_stream_capturing():
+            return
+        now = torch.cuda.current_stream(self.device)
+        for t in self._memory:
+            t.record_stream(now)
+        self._streams.add(stream)
+
     def norm(self, scale: float = 1.0) -> torch.Tensor:
         """``scale`` * norm of all tensors, an fp32 scalar on the device."""
         scale = _scale(scale)
         with on_device(self.device) as stream:
+            self._used_on(stream)
             part, norm = self._buffers()
             check(self.lib.dtf_global_norm(ptr(self.table), self.chunks, ptr(part), self.slots, scale, None, None, 0, 0.0,
                                            ptr(norm), stream), "global_norm")
@@ -177,6 +194,7 @@ class GlobalNormClip:
         if self._clip_error:
             raise ValueError(self._clip_error)
         with on_device(self.device) as stream:
+            self._used_on(stream)
             part, norm = self._buffers()
             check(self.lib.dtf_clip_by_global_norm(ptr(self.table), self.chunks, self._in_place, ptr(part), self.slots, scale,
                                                    clip_norm, ptr(norm), stream), "clip_by_global_norm")
