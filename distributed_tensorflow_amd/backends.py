@@ -25,6 +25,7 @@ class Backend:
     spec: ModelSpec
     layout: ArenaLayout
     batch: int
+    clip_norm: float = 0.0      # > 0: apply_gradients() clips by the global norm first
 
     # flat state -----------------------------------------------------------
     @property
@@ -118,6 +119,7 @@ class CpuBackend(Backend):
         self.layout = self.model.layout
         self._metrics = (float("nan"), float("nan"))
 
+    clip_norm = property(lambda self: self.model.clip_norm)
     params = property(lambda self: self.model.arena)
     grads = property(lambda self: self.model.grad_arena)
 
@@ -204,6 +206,7 @@ class HipBackend(Backend):
         self.use_graph = bool(use_graph) and batch > 1024 and dtype == "bf16"
         self._host_step = 0
 
+    clip_norm = property(lambda self: self.engine.clip_norm)
     params = property(lambda self: self.engine.params)
     grads = property(lambda self: self.engine.grads)
     ctrl_src = property(lambda self: self.engine.ctrl_src)

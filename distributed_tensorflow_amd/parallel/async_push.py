@@ -36,7 +36,7 @@ import torch.distributed as dist
 from ..backends import Backend
 from ..cluster import TaskInfo
 from ..ops import native
-from .strategies import broadcast_state, ps_shards
+from .strategies import broadcast_state, ps_shards, refuse_clipping
 
 KIND_GRAD, KIND_BYE, KIND_MASTER, KIND_ADAM_M, KIND_ADAM_V = 1, 2, 3, 4, 5
 
@@ -93,6 +93,7 @@ class PushFabric:
     def __init__(self, backend: Backend, task: TaskInfo, staleness: int):
         if backend.name != "hip":
             raise ValueError("the peer-to-peer parameter server needs the hip backend")
+        refuse_clipping(backend)
         if not 0 <= staleness <= MAX_STALENESS:
             raise ValueError(f"--staleness must be in [0, {MAX_STALENESS}] for --async_impl=push")
         self.lib = native.load()

@@ -77,6 +77,14 @@ def _get_int(t: torch.Tensor, i: int) -> int:
     return int(t[i:i + 1].view(torch.int32)[0].item())
 
 
+def refuse_clipping(backend: Backend):
+    """For strategies whose updates never see one whole gradient: a parameter server gets it shard by shard, or summed over
+    the workers of a round.  Applied there, the backend's clipping would go by the norm of something else, or not at all."""
+    if backend.clip_norm:
+        raise ValueError("asynchronous updates apply shards or sums of the workers' gradients: no gradient clipping "
+                         "(a backend with clip_norm needs LocalStrategy or SyncAllReduce)")
+
+
 class LocalStrategy:
     name = "local"
     coordinated_stop = False      # a stop request takes effect at once, locally
@@ -280,6 +288,7 @@ class AsyncP2PWorker:
     coordinated_stop = False      # asynchronous workers come and go on their own (reference M:174-176)
 
     def __init__(self, backend: Backend, task: TaskInfo, chief_rank: int):
+        refuse_clipping(backend)
         self.b, self.task, self.chief_rank = backend, task, chief_rank
         self.shards, self.step_owner = ps_shards(task, backend)
         dev = backend.params.device
@@ -329,6 +338,7 @@ class AsyncP2PServer:
     """One ps task: owns a shard of the variables, applies gradients in arrival order."""
 
     def __init__(self, backend: Backend, task: TaskInfo, chief_rank: int, training_iter: int, log=None):
+        refuse_clipping(backend)
         self.b, self.task, self.chief_rank, self.training_iter = backend, task, chief_rank, training_iter
         self.shards, self.step_owner = ps_shards(task, backend)
         self.ranges = self.shards[task.task_index]
@@ -392,6 +402,7 @@ class AsyncRounds:
     coordinated_stop = False
 
     def __init__(self, backend: Backend, task: TaskInfo, chief_rank: int, staleness: int = 1, optimizer: str = "sgd"):
+        refuse_clipping(backend)
         if staleness not in (0, 1):
             raise ValueError("staleness must be 0 or 1 rounds")
         if optimizer != "sgd":
