@@ -124,6 +124,7 @@ class DeviceDataset:
 
 class HipEngine:
     STATE_CURSOR, STATE_STEP, STATE_DROPOUT, STATE_ADAM_T, STATE_ADAM_T2 = 0, 1, 2, 3, 4
+    _clip_current = False      # the clipping factor in device memory is that of the gradients in the arena
 
     def __init__(self, spec: ModelSpec, batch: int, dataset: Optional[DeviceDataset] = None,
                  optimizer: str = "sgd", learning_rate: float = 1e-3, keep_prob: float = 1.0,
@@ -338,9 +339,11 @@ class HipEngine:
 
     def set_learning_rate(self, lr: float):
         self.hyper[0] = lr
+        self._clip_current = False
 
     def set_grad_scale(self, s: float):
         self.hyper[4] = s
+        self._clip_current = False
 
     @property
     def global_step(self) -> int:
@@ -437,12 +440,14 @@ class HipEngine:
 
     def launch_backward_dense(self):
         """head wgrad + fc1 wgrad: after this the first (head|wd1) part of the grad arena is final."""
+        self._clip_current = False
         check(self.lib.dtf_engine_backward_dense(self._d(), self._s()), "backward_dense")
 
     def launch_backward_conv(self, images: torch.Tensor, idx: Optional[torch.Tensor], record_dgrad: bool = False):
         """fc1 dgrad -> {conv2 dgrad -> conv1 wgrad} || conv2 wgrad (side stream) -> slab reduce.
         ``record_dgrad`` records the native event ``ev_dgrad`` right after fc1 dgrad, the last reader
         of the bf16 wd1 copy (see wait_dgrad_event)."""
+        self._clip_current = False
         check(self.lib.dtf_engine_backward_conv(self._d(), ptr(images), ptr(idx), int(record_dgrad), self._s()),
               "backward_conv")
 
@@ -453,6 +458,7 @@ class HipEngine:
     def launch_backward(self, images: torch.Tensor, idx: Optional[torch.Tensor]):
         """Whole backward; with multi_stream the dense-layer weight gradients run on a side stream
         concurrent with the conv chain (fork/join, preserved by HIP-graph capture)."""
+        self._clip_current = False
         check(self.lib.dtf_engine_backward(self._d(), ptr(images), ptr(idx), self._s()), "backward")
 
     def launch_update_range(self, lo: int, hi: int, advance: bool, advance_cursor: bool = True,
@@ -460,7 +466,10 @@ class HipEngine:
         """Optimizer over arena floats [lo, hi) (+ bf16 shadow).  ``advance`` bumps the sample cursor,
         global_step and dropout offset (exactly one range per step does that); every range keeps its
         own Adam step counter (state[adam_slot]) so ranges may be updated from different streams.  With clip_norm the
-        update uses the factor of the last launch_clip() (before the first one it is zero: nothing moves)."""
+        update goes by what the last launch_clip() left, its hyper-parameters and the factor: RuntimeError where new
+        gradients were launched, or a hyper-parameter was set, since then."""
+        if self.clip_norm and not self._clip_current:
+            raise RuntimeError("the clipping factor is not that of these gradients and hyper-parameters: launch_clip() first")
         check(self.lib.dtf_engine_update_range(self._d(), lo, hi, int(advance), int(advance_cursor), self.step_inc,
                                                adam_slot, self._s()), "update_range")
 
@@ -471,6 +480,7 @@ class HipEngine:
     def launch_clip(self):
         """Norm of the gradients in the arena and the clipping factor for the updates that follow (no-op with clip_norm 0)."""
         check(self.lib.dtf_engine_clip(self._d(), self._s()), "clip")
+        self._clip_current = True
 
     def grad_norm(self) -> float:
         """Global norm of the last clipped step's gradients, before clipping (reads device memory: synchronises)."""
@@ -486,6 +496,7 @@ class HipEngine:
     # ------------------------------------------------------------------ steps
     def launch_train_step(self):
         """One full optimisation step on the resident dataset: a single native call."""
+        self._clip_current = False
         check(self.lib.dtf_engine_train_step(self._d(), self.step_inc, self._s()), "train_step")
 
     @property
@@ -526,6 +537,7 @@ class HipEngine:
         return g
 
     def train_step(self):
+        self._clip_current = False
         if self._graph is not None:
             self._graph.replay()
         else:

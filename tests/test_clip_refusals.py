@@ -39,3 +39,57 @@ def test_the_mailbox_parameter_server_refuses_clipping(make):
     """Before anything collective or native: no process group and no GPU here."""
     with pytest.raises(ValueError, match="no gradient clipping"):
         make(SimpleNamespace(name="hip", clip_norm=1.0, engine=SimpleNamespace(clip_norm=1.0)))
+
+
+# ------------------------------------------------------------------------------------------- the engine's phases
+class Lib:
+    """Stands for the kernel library: every call succeeds and is noted."""
+
+    def __init__(self):
+        self.calls = []
+
+    def __getattr__(self, name):
+        return lambda *a: self.calls.append(name) or 0
+
+
+@pytest.fixture
+def engine(monkeypatch):
+    from distributed_tensorflow_amd.engine import HipEngine
+    monkeypatch.setattr(HipEngine, "_s", lambda self: 0)
+    monkeypatch.setattr(HipEngine, "_d", lambda self: None)
+    monkeypatch.setattr(HipEngine, "__del__", lambda self: None)
+    eng = object.__new__(HipEngine)
+    eng.lib, eng.clip_norm, eng.step_inc, eng.dtype, eng.dense_g16 = Lib(), 1.0, 1, "bf16", None
+    eng.layout, eng.hyper, eng.B, eng._graph = SimpleNamespace(total=64), torch.zeros(12), 4, None
+    return eng
+
+
+X = torch.zeros(1)
+NEW_GRADIENTS = [
+    lambda e: e.launch_backward_dense(), lambda e: e.launch_backward_conv(X, None), lambda e: e.launch_backward(X, None),
+    lambda e: e.launch_train_step(), lambda e: e.set_learning_rate(0.1), lambda e: e.set_grad_scale(0.5),
+]
+
+
+@pytest.mark.parametrize("k", range(len(NEW_GRADIENTS)))
+def test_an_update_with_the_factor_of_another_gradient_is_refused(engine, k):
+    """The clipping factor, the learning rate and the gradient scale of an update are those of the last launch_clip()."""
+    with pytest.raises(RuntimeError, match=r"launch_clip\(\) first"):
+        engine.launch_update_range(0, 64, True)             # no factor at all yet
+    engine.launch_clip()
+    engine.launch_update_range(0, 32, False)                # the ranges of one step share the factor
+    engine.launch_update_range(32, 64, True)
+    NEW_GRADIENTS[k](engine)
+    done = len(engine.lib.calls)
+    with pytest.raises(RuntimeError, match=r"launch_clip\(\) first"):
+        engine.launch_update_range(0, 64, True)
+    assert len(engine.lib.calls) == done                    # nothing was launched
+    engine.launch_update()
+    assert engine.lib.calls[done:done + 2] == ["dtf_engine_clip", "dtf_engine_update_range"]
+
+
+def test_without_clipping_the_ranges_need_nothing(engine):
+    engine.clip_norm = 0.0
+    engine.launch_update_range(0, 64, True)
+    engine.launch_backward_dense()
+    engine.launch_update_range(0, 64, True)
