@@ -407,6 +407,9 @@ class HipEngine:
         there.  Mixed-precision configuration only.  Returns the buffer (flat, wd1's element count)."""
         if self.dtype != "bf16":
             raise ValueError("the 16-bit gradient collective belongs to the bf16 configuration")
+        if self.clip_norm:
+            raise ValueError("the global norm is that of the fp32 arena, which a 16-bit dense gradient does not reach: no gradient "
+                             "clipping with it")
         if self.dense_g16 is None:
             lo, hi = self.layout.segment("wd1", "wd1")
             self.dense_g16 = torch.zeros(hi - lo, dtype=torch.bfloat16, device=self.device)

@@ -93,3 +93,10 @@ def test_without_clipping_the_ranges_need_nothing(engine):
     engine.launch_update_range(0, 64, True)
     engine.launch_backward_dense()
     engine.launch_update_range(0, 64, True)
+
+
+def test_the_16_bit_dense_gradient_has_no_norm(engine):
+    """With it the fc1 weight gradient never reaches the fp32 arena, whose norm is taken."""
+    with pytest.raises(ValueError, match="no gradient clipping"):
+        engine.enable_dense_g16()
+    assert engine.dense_g16 is None
