@@ -164,14 +164,33 @@ __device__ __forceinline__ double norm_of(const double* part, int np, double sca
   for (int i = threadIdx.x; i < np; i += kClipThreads) a += part[i];
   return scale * sqrt(block_sum(a, red));
 }
-// what a gradient value is multiplied with
-__device__ __forceinline__ float clip_factor(double norm, double scale, double limit) {
-  if (!(norm <= 1.7976931348623157e308)) return __builtin_nanf("");     // inf or NaN: every result says so
-  return (float)(norm > limit ? scale * (limit / norm) : scale);
+// What a gradient value is multiplied with.  By the norm in 64 bits: that it is returned as infinity where fp32 does not hold it
+// (two values of 3e38) makes no value wrong.
+__device__ __forceinline__ double clip_factor(double norm, double scale, double limit) {
+  if (!(norm <= 1.7976931348623157e308)) return __builtin_nan("");      // inf or NaN: every result says so
+  return norm > limit ? scale * (limit / norm) : scale;
 }
+// The factor as m * 2^e: e is 0, but where it is subnormal in fp32 (limit 1e-3, norm 1e38: two digits left) or beyond it, and its
+// products need not be.  m is then chosen so that x * m neither overflows (m <= 1 for small factors) nor loses digits of a small x
+// (m from 2^126 on for large ones).
+struct ClipFactor {
+  float m;
+  int e;
+  __device__ __forceinline__ explicit ClipFactor(double c) : m((float)c), e(0) {
+    if (!(c > 0.0)) return;
+    if (m < 1.17549435e-38f) {
+      m = (float)__builtin_amdgcn_frexp_mant(c);
+      e = __builtin_amdgcn_frexp_exp(c);
+    } else if (m > 3.40282347e38f) {
+      m = (float)(__builtin_amdgcn_frexp_mant(c) * 0x1p127);
+      e = __builtin_amdgcn_frexp_exp(c) - 127;
+    }
+  }
+  __device__ __forceinline__ float times(float x) const { return __builtin_amdgcn_ldexpf(x * m, e); }
+};
 
 template <typename T>
-__device__ __forceinline__ void chunk_scale(const ClipChunk& s, float f) {
+__device__ __forceinline__ void chunk_scale(const ClipChunk& s, const ClipFactor& f) {
   constexpr int VE = 16 / sizeof(T);
   const T* p = (const T*)s.in;
   T* o = (T*)s.out;
@@ -179,7 +198,7 @@ __device__ __forceinline__ void chunk_scale(const ClipChunk& s, float f) {
     float y[VE];
     unpack(p, x, y);
 #pragma unroll
-    for (int i = 0; i < VE; ++i) y[i] *= f;
+    for (int i = 0; i < VE; ++i) y[i] = f.times(y[i]);
     return pack<T, VE>(y);
   };
   if (s.cols == 0) {
@@ -193,13 +212,13 @@ __device__ __forceinline__ void chunk_scale(const ClipChunk& s, float f) {
       for (int u = 0; u < kDeep; ++u) store_any_once(o + (v + u * kClipThreads) * VE, scaled(x[u]));
     }
     for (; v < vend; v += kClipThreads) store_any(o + v * VE, scaled(load_any(p + v * VE)));
-    for (int e = vend * VE + threadIdx.x; e < s.n; e += kClipThreads) o[e] = (T)((float)p[e] * f);
+    for (int e = vend * VE + threadIdx.x; e < s.n; e += kClipThreads) o[e] = (T)f.times((float)p[e]);
   } else if (s.cols % VE == 0) {
     for (int e = threadIdx.x * VE; e + VE <= s.n; e += kClipThreads * VE)
       store_any(o + span_at(s.lo + e, s.cols, s.out_pitch), scaled(load_any(p + span_at(s.lo + e, s.cols, s.in_pitch))));
   } else {
     for (int e = threadIdx.x; e < s.n; e += kClipThreads)
-      o[span_at(s.lo + e, s.cols, s.out_pitch)] = (T)((float)p[span_at(s.lo + e, s.cols, s.in_pitch)] * f);
+      o[span_at(s.lo + e, s.cols, s.out_pitch)] = (T)f.times((float)p[span_at(s.lo + e, s.cols, s.in_pitch)]);
   }
 }
 
@@ -209,9 +228,9 @@ __global__ __launch_bounds__(kClipThreads) void clip_scale(const ClipChunk* __re
                                                            int in_place, float* __restrict__ norm_out) {
   __shared__ double red[4];
   const double norm = norm_of(part, np, scale, red);
-  const float f = clip_factor(norm, scale, limit);
+  const ClipFactor f(clip_factor(norm, scale, limit));
   if (blockIdx.x == 0 && threadIdx.x == 0) *norm_out = (float)norm;
-  if (in_place && f == 1.0f) return;
+  if (in_place && f.m == 1.0f && f.e == 0) return;
   for (int c = chunks - 1 - (int)blockIdx.x; c >= 0; c -= gridDim.x) {
     const ClipChunk s = table[c];
     if (s.dtype == 0) chunk_scale<float>(s, f);
@@ -222,7 +241,8 @@ __global__ __launch_bounds__(kClipThreads) void clip_scale(const ClipChunk* __re
 
 // One workgroup: the norm alone, and -- hyper given -- the step's hyper-parameters with the gradient scale (hyper[4])
 // multiplied by the factor, for update kernels that read them from device memory (optim.hip): the clipped update then
-// needs no pass over the gradients.  The gradient scale itself is read from hyper, so a replayed graph follows it.
+// needs no pass over the gradients.  The gradient scale itself is read from hyper, so a replayed graph follows it.  (The factor is
+// an fp32 number like the others there: below 1.2e-38, a norm of 1e38 against a limit of 1, it loses digits.)
 __global__ __launch_bounds__(kClipThreads) void norm_finish(const double* __restrict__ part, int np, double scale,
                                                             const float* __restrict__ hyper, float* __restrict__ hyper_out,
                                                             int n_hyper, double limit, float* __restrict__ norm_out) {
@@ -231,7 +251,7 @@ __global__ __launch_bounds__(kClipThreads) void norm_finish(const double* __rest
   const double norm = norm_of(part, np, sc, red);
   if (threadIdx.x == 0 && norm_out) *norm_out = (float)norm;
   if (hyper && (int)threadIdx.x < n_hyper)
-    hyper_out[threadIdx.x] = threadIdx.x == 4 ? clip_factor(norm, sc, limit) : hyper[threadIdx.x];
+    hyper_out[threadIdx.x] = threadIdx.x == 4 ? (float)clip_factor(norm, sc, limit) : hyper[threadIdx.x];
 }
 
 }  // namespace dtf
