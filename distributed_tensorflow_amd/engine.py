@@ -134,7 +134,8 @@ class HipEngine:
                  clip_norm: float = 0.0):
         """clip_norm > 0: every update applies gradients scaled by clip_norm / max(norm, clip_norm), norm = the global norm
         of the (scaled) gradients of all eight tensors, which ``grad_norm()`` reads back (tf.clip_by_global_norm before
-        apply_gradients); 0: no clipping.  A norm that is not finite makes the parameters NaN."""
+        apply_gradients); 0: no clipping.  A gradient that is not finite makes the parameters NaN.  The factor is an fp32
+        number: limits below 1.2e-38 of the norm leave it less than 24 bits."""
         if not (clip_norm >= 0.0 and math.isfinite(clip_norm)):
             raise ValueError(f"clip_norm must be finite and not negative, got {clip_norm}")
         if not torch.cuda.is_available():

@@ -11,7 +11,9 @@ costs a copy to the device and a wait for it and cannot be made while a stream i
 stream of the tensors' device: the table is only read, the workspace of a call comes from PyTorch's allocator on that
 stream, so calls on different streams and in different graphs share nothing that is written.  A plan may be dropped while
 its calls still run on any stream; one whose call was captured into a HIP graph has to outlive the graph and its replays.
-As in TensorFlow, a norm that is not finite makes every clipped value NaN.
+As in TensorFlow, a norm that is not finite (a value that is not, in some tensor) makes every clipped value NaN.  Norm and
+factor are 64-bit numbers: a list of finite values whose norm is beyond fp32 is clipped all the same, though the norm that
+is returned, an fp32 scalar, is then infinity.
 Kernels: csrc/kernels/clip.hip.
 """
 from __future__ import annotations
@@ -176,7 +178,7 @@ class GlobalNormClip:
         self._streams.add(stream)
 
     def norm(self, scale: float = 1.0) -> torch.Tensor:
-        """``scale`` * norm of all tensors, an fp32 scalar on the device."""
+        """``scale`` * norm of all tensors, an fp32 scalar on the device (infinity from 3.4e38 on)."""
         scale = _scale(scale)
         with on_device(self.device) as stream:
             self._used_on(stream)

@@ -70,8 +70,8 @@ def global_norm(tensors, scale: float = 1.0) -> torch.Tensor:
 
 
 def clip_by_global_norm(tensors, clip_norm: float, scale: float = 1.0):
-    """tf.clip_by_global_norm of scale * tensors: (clipped copies, norm before clipping).  A norm that is not finite
-    makes every value NaN."""
+    """tf.clip_by_global_norm of scale * tensors: (clipped copies, norm before clipping, in 64 bits).  A norm that is not
+    finite makes every value NaN."""
     norm = global_norm(tensors, scale)
     if not bool(torch.isfinite(norm)):
         factor = torch.full_like(norm, float("nan"))

@@ -1,6 +1,7 @@
 """Norms and clipping factors at the ends of fp32's range (ops/clip.py, csrc/kernels/clip.hip).
 
-A factor may be subnormal in fp32 (limit 1e-3, norm 1e38) or beyond it (a large `scale`) while its products
+The norm and the factor are 64-bit numbers.  Returned as fp32 the norm may round to infinity while the clipped values are
+ordinary numbers; a factor may be subnormal in fp32 (limit 1e-3, norm 1e38) or beyond it (a large `scale`) while its products
 are not.  A product is off by the factor's rounding and its own (2 x 2^-24), plus half of the type's for bf16 (2^-8) and fp16
 (2^-11), plus half of the smallest step of the type below its normal range."""
 import math
@@ -9,6 +10,7 @@ import pytest
 import torch
 
 from distributed_tensorflow_amd.ops import GlobalNormClip
+from distributed_tensorflow_amd.ops import reference as R
 
 gpu = pytest.mark.gpu
 F, B, H = torch.float32, torch.bfloat16, torch.float16
@@ -71,3 +73,31 @@ def test_fp16_with_a_factor_beyond_fp32(gpu_lib):
     assert bool((got == 0).all()) and abs(float(n) - norm) <= norm * 2.0 ** -23
     (got,), _ = GlobalNormClip([t], out=[torch.empty_like(t)]).clip(1e300, scale=0.0)
     assert bool((got == 0).all())
+
+
+# ---------------------------------------------------------------------- a norm that fp32 does not hold
+def two(device):
+    return [torch.full((2,), 3e38, device=device), torch.full((3,), -2e38, device=device)]
+
+
+def test_reference_goes_by_the_norm_in_64_bits():
+    out, norm = R.clip_by_global_norm(two("cpu"), 1.0)
+    want = math.sqrt(2 * 9.0 + 3 * 4.0) * 1e38
+    assert float(norm) == pytest.approx(want, rel=1e-6)
+    assert torch.allclose(out[0].double(), torch.full((2,), 3e38 / want, dtype=torch.float64), rtol=1e-6)
+
+
+@gpu
+@pytest.mark.parametrize("in_place", [False, True])
+def test_a_norm_beyond_fp32_is_returned_as_infinity_and_clips(gpu_lib, in_place):
+    tensors = two("cuda")
+    norm = math.sqrt(2 * float(tensors[0][0]) ** 2 + 3 * float(tensors[1][0]) ** 2)
+    before = [t.double() for t in tensors]
+    got, n = GlobalNormClip(tensors, out=None if in_place else [torch.empty_like(t) for t in tensors]).clip(2.0)
+    assert float(n) == math.inf and float(GlobalNormClip([t.clone() for t in two("cuda")]).norm()) == math.inf
+    for o, b in zip(got, before):
+        check(o, b * (2.0 / norm))
+    # within the limit nothing changes
+    tensors = two("cuda")
+    got, n = GlobalNormClip(tensors).clip(1e39)
+    assert float(n) == math.inf and all(torch.equal(o, b) for o, b in zip(got, two("cuda")))
