@@ -13,7 +13,8 @@ stream, so calls on different streams and in different graphs share nothing that
 its calls still run on any stream; one whose call was captured into a HIP graph has to outlive the graph and its replays.
 As in TensorFlow, a norm that is not finite (a value that is not, in some tensor) makes every clipped value NaN.  Norm and
 factor are 64-bit numbers: a list of finite values whose norm is beyond fp32 is clipped all the same, though the norm that
-is returned, an fp32 scalar, is then infinity.
+is returned, an fp32 scalar, is then infinity.  Autograd does not record the calls: tensors that require gradients are taken
+under ``torch.no_grad()`` only.
 Kernels: csrc/kernels/clip.hip.
 """
 from __future__ import annotations
@@ -25,7 +26,7 @@ from typing import List, Optional, Sequence, Tuple
 import torch
 
 from . import native
-from .native import check, on_device, ptr
+from .native import check, no_autograd, on_device, ptr
 
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
@@ -105,6 +106,8 @@ class GlobalNormClip:
     of a matrix).  out: where the clipped values go, tensors of the same shapes and types; None clips in place (and then
     a norm within the limit leaves every value untouched, without a pass over them)."""
 
+    _requires: Sequence[torch.Tensor] = ()      # a tensor that requires gradients, where there is one
+
     def __init__(self, tensors: Sequence[torch.Tensor], out: Optional[Sequence[torch.Tensor]] = None):
         tensors = list(tensors)
         if not tensors:
@@ -120,6 +123,8 @@ class GlobalNormClip:
         for t, o in zip(tensors, outs):
             if not isinstance(o, torch.Tensor) or o.layout != torch.strided or o.dtype != t.dtype or o.shape != t.shape:
                 raise ValueError("every output needs the shape and type of its tensor")
+        no_autograd(tensors + outs)
+        self._requires = [t for t in tensors + outs if t.requires_grad][:1]
         self.device = tensors[0].device
         spans = (ClipSpan * len(tensors))()
         ins, writes = [], []
@@ -180,6 +185,7 @@ class GlobalNormClip:
     def norm(self, scale: float = 1.0) -> torch.Tensor:
         """``scale`` * norm of all tensors, an fp32 scalar on the device (infinity from 3.4e38 on)."""
         scale = _scale(scale)
+        no_autograd(self._requires)
         with on_device(self.device) as stream:
             self._used_on(stream)
             part, norm = self._buffers()
@@ -195,6 +201,7 @@ class GlobalNormClip:
             raise ValueError(f"clip_norm must be positive and finite, got {clip_norm}")
         if self._clip_error:
             raise ValueError(self._clip_error)
+        no_autograd(self._requires)
         with on_device(self.device) as stream:
             self._used_on(stream)
             part, norm = self._buffers()

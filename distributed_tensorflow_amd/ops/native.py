@@ -278,6 +278,12 @@ class on_device:
             torch.cuda.set_device(self.back)
 
 
+def no_autograd(tensors):
+    """For calls that record nothing: ValueError where PyTorch would record them (None stands for a tensor left out)."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise ValueError("operands or outputs require gradients, and this call would not be recorded: call it under torch.no_grad()")
+
+
 def check(rc: int, what: str):
     if rc != 0:
         raise RuntimeError(f"{what} failed: code {rc}"

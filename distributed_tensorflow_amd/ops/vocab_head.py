@@ -20,7 +20,8 @@ The backward pass computes the logits again, one piece of the classes at a time:
 piece's logits in the operands' type (at most 2^27 values, or 1024 classes of very many rows), a copy of ``h`` without its
 ignored rows, fp32 sums of ``dh`` where there are several pieces or the classes are cut among workgroups, and the copies
 above.  Calls launch on the current stream of the operands' device, take their workspace from PyTorch's allocator on that
-stream and keep nothing, so they can be captured into HIP graphs and run on several streams at once.
+stream and keep nothing, so they can be captured into HIP graphs and run on several streams at once.  Autograd does not record
+them: operands that require gradients are taken under ``torch.no_grad()`` only.
 Kernels: csrc/kernels/vocab_head.hip.
 """
 from __future__ import annotations
@@ -30,7 +31,7 @@ from typing import Optional, Tuple
 import torch
 
 from . import native
-from .native import check, on_device, ptr
+from .native import check, no_autograd, on_device, ptr
 
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1}
 _MAX_ROW = 1 << 20          # rows, hidden units and row strides of one call
@@ -59,7 +60,7 @@ def _vector(t: Optional[torch.Tensor], name: str, n: int, dtype: torch.dtype, de
         raise ValueError(f"{name} is on {t.device}, the hidden rows on {device}")
 
 
-def _check(h, wT, labels, bias, ignore_label) -> Tuple[int, int, int, int, int]:
+def _check(h, wT, labels, bias, ignore_label, *others) -> Tuple[int, int, int, int, int]:
     dtype, dev = h.dtype, h.device
     if dtype not in _DTYPES or wT.dtype != dtype:
         raise TypeError(f"h and wT must both be bf16 or both fp32, got {dtype} and {wT.dtype}")
@@ -80,6 +81,7 @@ def _check(h, wT, labels, bias, ignore_label) -> Tuple[int, int, int, int, int]:
     _vector(bias, "bias", classes, torch.float32, dev)
     if not -(1 << 31) <= ignore_label < 1 << 31:
         raise ValueError(f"ignore_label must be an int32, got {ignore_label}")
+    no_autograd((h, wT, bias) + others)
     if dev.type != "cuda":
         raise ValueError(f"GPU tensors expected, got {dev} (ops.reference.softmax_cross_entropy_with_logits runs on the CPU)")
     return n, hidden, classes, ldh, ldw
@@ -116,7 +118,7 @@ def vocab_head_bwd(h: torch.Tensor, wT: torch.Tensor, labels: torch.Tensor, lse:
     are not wanted.  ``row_scale``: fp32 [n], the upstream gradient of the loss rows (default: ones).  ``dh`` / ``dwT`` /
     ``dbias``: where to write (contiguous, 16-byte aligned; ``dwT`` in the operands' type or fp32), e.g. views of a gradient
     arena.  ``piece``: classes per piece (rounded up to 256; 0: chosen from n)."""
-    n, hidden, classes, ldh, ldw = _check(h, wT, labels, bias, ignore_label)
+    n, hidden, classes, ldh, ldw = _check(h, wT, labels, bias, ignore_label, lse, row_scale, dh, dwT, dbias)
     _vector(lse, "lse", n, torch.float32, h.device)
     _vector(row_scale, "row_scale", n, torch.float32, h.device)
     if lse is None:
