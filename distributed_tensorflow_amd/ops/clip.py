@@ -107,6 +107,7 @@ class GlobalNormClip:
     a norm within the limit leaves every value untouched, without a pass over them)."""
 
     _requires: Sequence[torch.Tensor] = ()      # a tensor that requires gradients, where there is one
+    _written: Sequence[torch.Tensor] = ()       # whose version counters a clipping call raises: views of one tensor share theirs
 
     def __init__(self, tensors: Sequence[torch.Tensor], out: Optional[Sequence[torch.Tensor]] = None):
         tensors = list(tensors)
@@ -163,6 +164,7 @@ class GlobalNormClip:
         torch.cuda.current_stream(self.device).synchronize()
         self._memory = [self.table] + list({t.untyped_storage().data_ptr(): t for t in kept if t.numel()}.values())
         self._keep, self._streams = kept, set()
+        self._written = list({id(b): b for b in (o._base if o._is_view() else o for o in outs)}.values())
         self._used_on(torch.cuda.current_stream(self.device).cuda_stream)
         self.chunks, self._in_place = chunks, in_place.value
         self.slots = int(self.lib.dtf_clip_partials(chunks))    # fp64 words of a call's workspace
@@ -207,6 +209,7 @@ class GlobalNormClip:
             part, norm = self._buffers()
             check(self.lib.dtf_clip_by_global_norm(ptr(self.table), self.chunks, self._in_place, ptr(part), self.slots, scale,
                                                    clip_norm, ptr(norm), stream), "clip_by_global_norm")
+        torch.autograd.graph.increment_version(self._written)
         return self.out, norm
 
 

@@ -141,6 +141,7 @@ def vocab_head_bwd(h: torch.Tensor, wT: torch.Tensor, labels: torch.Tensor, lse:
             if a < d and c < b:
                 raise ValueError(f"{name} shares memory with an operand or another output")
         reads.append(t)
+    given = [t for t in (dh, dwT, dbias) if t is not None]
     dev = h.device
     if dh is None and need_dh:
         dh = torch.empty((n, hidden), dtype=h.dtype, device=dev)
@@ -153,6 +154,8 @@ def vocab_head_bwd(h: torch.Tensor, wT: torch.Tensor, labels: torch.Tensor, lse:
             if t is not None:
                 t.zero_()
         return dh, dwT, dbias
+    if given:
+        torch.autograd.graph.increment_version(given)       # written in place
     lib, dt = native.load(), _DTYPES[h.dtype]
     with on_device(dev) as stream:
         need = lib.dtf_vocab_head_workspace(dt, 1, ptr(h), ldh, ptr(wT), ldw, n, hidden, classes, int(dbias is not None), piece)

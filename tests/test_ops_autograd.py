@@ -1,5 +1,5 @@
 """The head and the clipping next to PyTorch's autograd: they record nothing, so under grad mode operands that require gradients
-are refused."""
+are refused, and what they write in place counts as written (a backward pass that saved it must not use it)."""
 import pytest
 import torch
 
@@ -64,3 +64,42 @@ def test_parameters_under_no_grad(gpu_lib):
         plan.norm()
     with pytest.raises(ValueError, match="require gradients"):
         plan.clip(1.0)
+
+
+@gpu
+def test_what_is_written_counts_as_written(gpu_lib):
+    """Saved for a backward pass and then overwritten: autograd has to notice."""
+    h, w, y, b = operands("cuda")
+    _, lse = vocab_head_fwd(h, w, y, b)
+
+    def saved(t):
+        x = torch.ones_like(t, requires_grad=True)
+        return (x * t).sum()        # keeps t for x's gradient
+
+    dh, dw, db = torch.zeros_like(h), torch.zeros_like(w), torch.zeros_like(b)
+    sums = [saved(t) for t in (dh, dw, db)]
+    vocab_head_bwd(h, w, y, lse, b, dh=dh, dwT=dw, dbias=db)
+    flat = torch.ones(100, device="cuda")
+    views = list(torch.split(flat, [30, 70]))
+    alone = torch.ones(5, device="cuda")
+    sums += [saved(flat), saved(views[1]), saved(alone)]
+    GlobalNormClip(views + [alone]).clip(1.0)
+    out = [torch.zeros_like(t) for t in views]
+    sums += [saved(t) for t in out]
+    GlobalNormClip(views, out=out).clip(1.0)
+    for s in sums:
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            s.backward()
+    # what is only read stays usable
+    kept = saved(flat)
+    GlobalNormClip(views).norm()
+    GlobalNormClip(views, out=out).clip(1.0)
+    kept.backward()
+
+
+@gpu
+def test_inference_tensors_have_no_counter(gpu_lib):
+    with torch.inference_mode():
+        t = torch.ones(100, device="cuda")
+        GlobalNormClip([t]).clip(1.0)
+        assert abs(float(t.double().norm()) - 1.0) <= 1e-6
