@@ -1,0 +1,62 @@
+"""Every build of the kernels uses the flags of tools/build_native.py, which keep packed FP32 instructions out (some of their
+forms have returned wrong values, without an error).  CPU only: the library that is
+loaded is taken apart into its gfx950 code objects and read."""
+import os
+import re
+import shutil
+import subprocess
+import sys
+from pathlib import Path
+
+import pytest
+
+ROOT = Path(__file__).resolve().parent.parent
+sys.path.insert(0, str(ROOT / "tools"))
+import build_native  # noqa: E402
+
+LIB = ROOT / "distributed_tensorflow_amd" / "_lib" / "libdtf_kernels.so"
+OBJDUMP = "/opt/rocm/llvm/bin/llvm-objdump"
+needs_rocm = pytest.mark.skipif(not os.path.exists(OBJDUMP), reason="no ROCm tools")
+
+
+def test_flags_for_scripts():
+    r = subprocess.run([sys.executable, str(ROOT / "tools" / "build_native.py"), "--flags"], capture_output=True, text=True, check=True)
+    assert r.stdout.split() == build_native.HIP_FLAGS and "-packed-fp32-ops" in build_native.HIP_FLAGS
+    assert f"--offload-arch={build_native.ARCH}" in build_native.HIP_FLAGS
+
+
+def test_no_tool_has_flags_of_its_own():
+    """A tool that compiles kernels names the shared list; nobody else spells the target out (linking needs no device flags)."""
+    own = []
+    for f in sorted((ROOT / "tools").rglob("*")):
+        if f.suffix not in (".py", ".sh", ".hip") or f.name == "build_native.py":
+            continue
+        for k, line in enumerate(f.read_text().split("\n"), 1):
+            if "--offload-arch" in line and "-shared -fPIC -o" not in line:
+                own.append(f"{f.relative_to(ROOT)}:{k}")
+    assert not own, own
+
+
+@needs_rocm
+@pytest.mark.skipif(not LIB.exists(), reason="library not built")
+def test_no_packed_fp32_instruction_is_shipped(tmp_path):
+    shutil.copy(LIB, tmp_path / "k.so")
+    subprocess.run([OBJDUMP, "--offloading", "k.so"], cwd=tmp_path, check=True, capture_output=True)
+    objects = sorted(tmp_path.glob("k.so.*gfx950"))
+    assert len(objects) >= 10
+    kernels = 0
+    for o in objects:
+        text = subprocess.run([OBJDUMP, "-d", str(o)], check=True, capture_output=True, text=True).stdout
+        kernels += text.count("s_endpgm")
+        found = re.findall(r"v_pk_(?:add|mul|fma)_f32\b.*", text)
+        assert not found, (o.name, len(found), found[0])
+    assert kernels >= 50
+
+
+@needs_rocm
+def test_the_gemm_pipelines_waits_as_shipped(tmp_path, monkeypatch):
+    """The wait-placement guard on the code that is shipped: the same check, compiled with the library's flags."""
+    import test_gemm_isa
+    run = subprocess.run
+    monkeypatch.setattr(test_gemm_isa.subprocess, "run", lambda cmd, **kw: run([cmd[0], *build_native.DEVICE_FLAGS, *cmd[1:]], **kw))
+    test_gemm_isa.test_lds_dma_pipeline_waits_are_exactly_the_pipelines_own(tmp_path)

@@ -1,5 +1,5 @@
 // Does hipExtAnyOrderLaunch (no AQL barrier bit) let kernels of ONE stream overlap on this stack?
-// Build: hipcc --offload-arch=gfx950 -O2 tools/any_order_probe.hip -o diag_build/any_order_probe
+// Build: hipcc $(python3 tools/build_native.py --flags) tools/any_order_probe.hip -o diag_build/any_order_probe
 #include <hip/hip_runtime.h>
 #include <hip/hip_ext.h>
 #include <chrono>

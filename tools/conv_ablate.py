@@ -4,6 +4,7 @@ kernel removed (-DDTF_ABLATE bits, see conv2.hip) and times each on the GPU.
   python tools/conv_ablate.py run [wgrad|fwd|dgrad] [G]
 """
 import ctypes, os, subprocess, sys, time
+from build_native import HIP_FLAGS
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 OUT = os.path.join(ROOT, "diag_build")
 WG = {0: "full", 32: "no x staging", 128: "no dY staging", 160: "no staging at all", 64: "no MFMA",
@@ -21,7 +22,7 @@ if sys.argv[1] == "buildcfg":
     os.makedirs(OUT, exist_ok=True)
     for kind, lst in CFGS.items():
         for i, c in enumerate(lst):
-            subprocess.check_call(["/opt/rocm/bin/hipcc", "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-shared",
+            subprocess.check_call(["/opt/rocm/bin/hipcc", *HIP_FLAGS, "-shared",
                                    f"-DDTF_{kind.upper()}_CFG={c}", "-DDTF_DIAG=1", "-I", ROOT + "/csrc/kernels", ROOT + "/csrc/kernels/conv2.hip",
                                    "-o", f"{OUT}/conv2_{kind}{i}.so"])
     print("built cfgs")
@@ -29,21 +30,21 @@ elif sys.argv[1] == "buildstagger":
     os.makedirs(OUT, exist_ok=True)
     mode = os.environ.get("STAGGER_MODE", "0")
     for d in STAGGER:
-        subprocess.check_call(["/opt/rocm/bin/hipcc", "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-shared",
+        subprocess.check_call(["/opt/rocm/bin/hipcc", *HIP_FLAGS, "-shared",
                                f"-DDTF_STAGGER={d}", f"-DDTF_STAGGER_MODE={mode}", "-DDTF_DIAG=1", "-I", ROOT + "/csrc/kernels", ROOT + "/csrc/kernels/conv2.hip",
                                "-o", f"{OUT}/conv2_st{d}.so"])
     print("built stagger")
 elif sys.argv[1] == "buildpc":
     os.makedirs(OUT, exist_ok=True)
     for v in sorted(WG_PC):
-        subprocess.check_call(["/opt/rocm/bin/hipcc", "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-shared",
+        subprocess.check_call(["/opt/rocm/bin/hipcc", *HIP_FLAGS, "-shared",
                                f"-DDTF_ABLATE={v}", "-DDTF_DIAG=1", "-I", ROOT + "/csrc/kernels", ROOT + "/csrc/kernels/conv2.hip",
                                "-o", f"{OUT}/conv2_ab{v}.so"])
     print("built", len(WG_PC))
 elif sys.argv[1] == "build":
     os.makedirs(OUT, exist_ok=True)
     for v in sorted(set(WG) | set(IG)):
-        subprocess.check_call(["/opt/rocm/bin/hipcc", "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-shared",
+        subprocess.check_call(["/opt/rocm/bin/hipcc", *HIP_FLAGS, "-shared",
                                f"-DDTF_ABLATE={v}", "-DDTF_DIAG=1", "-I", ROOT + "/csrc/kernels", ROOT + "/csrc/kernels/conv2.hip",
                                "-o", f"{OUT}/conv2_ab{v}.so"])
     print("built", len(set(WG) | set(IG)))

@@ -11,11 +11,12 @@ of the k-loop 42.4, with one LDS read per step instead of thirteen 40.4, with bo
 kernel gets (78.4 k cycles in 38.2 us = 2.05 GHz).  Two waves per SIMD take 40 us per image: 95 % of that floor.
 """
 import ctypes, os, subprocess, sys
+from build_native import HIP_FLAGS
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 OUT = os.path.join(ROOT, "diag_build")
 if sys.argv[1] == "build":
     os.makedirs(OUT, exist_ok=True)
-    subprocess.check_call(["/opt/rocm/bin/hipcc", "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-shared",
+    subprocess.check_call(["/opt/rocm/bin/hipcc", *HIP_FLAGS, "-shared",
                            "-DDTF_F32_TIMING=1", "-I", ROOT + "/csrc/kernels", ROOT + "/csrc/kernels/conv2_f32.hip",
                            "-o", f"{OUT}/conv2_f32_timing.so"])
     print("built")

@@ -5,17 +5,18 @@ Stamps per workgroup (100 MHz wall clock): 0 start, 1 tile staged (+sync), 2 wav
 3 all waves left the k-loop, 4 epilogue in LDS (+sync), 5 stores issued; 6/7 = shader clock at start/end.
 """
 import ctypes, os, subprocess, sys
+from build_native import HIP_FLAGS
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 OUT = os.path.join(ROOT, "diag_build")
 if sys.argv[1] == "build":
     os.makedirs(OUT, exist_ok=True)
-    subprocess.check_call(["/opt/rocm/bin/hipcc", "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-shared",
+    subprocess.check_call(["/opt/rocm/bin/hipcc", *HIP_FLAGS, "-shared",
                            "-DDTF_TIMING=1", "-DDTF_DIAG=1", "-I", ROOT + "/csrc/kernels", ROOT + "/csrc/kernels/conv2.hip",
                            "-o", f"{OUT}/conv2_timing.so"])
-    subprocess.check_call(["/opt/rocm/bin/hipcc", "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-shared",
+    subprocess.check_call(["/opt/rocm/bin/hipcc", *HIP_FLAGS, "-shared",
                            "-DDTF_TIMING=1", "-DDTF_DIAG=1", "-I", ROOT + "/csrc/kernels", ROOT + "/csrc/kernels/head.hip",
                            "-o", f"{OUT}/head_timing.so"])
-    subprocess.check_call(["/opt/rocm/bin/hipcc", "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-shared",
+    subprocess.check_call(["/opt/rocm/bin/hipcc", *HIP_FLAGS, "-shared",
                            "-DDTF_TIMING=1", "-DDTF_DIAG=1", "-I", ROOT + "/csrc/kernels", ROOT + "/csrc/kernels/gemm.hip",
                            ROOT + "/csrc/kernels/head.hip", "-o", f"{OUT}/gemm_timing.so"])
     print("built")

@@ -3,7 +3,7 @@
 // Every wave runs N v_mfma_f32_16x16x32_bf16 back to back, either on ONE accumulator (dependent chain) or on FOUR
 // (independent: the pipe's issue rate), stamps s_memtime (shader-clock counter) and s_memrealtime (100 MHz wall clock)
 // around the loop, and the host prints cycles per MFMA, ns per MFMA and the clock the two counters imply.
-//   hipcc --offload-arch=gfx950 -O3 -o mfma_rate tools/micro/mfma_rate.hip && ./mfma_rate
+//   hipcc $(python3 tools/build_native.py --flags) -o mfma_rate tools/micro/mfma_rate.hip && ./mfma_rate
 #include <hip/hip_runtime.h>
 #include <stdio.h>
 #include <stdlib.h>

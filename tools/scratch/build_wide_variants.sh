@@ -2,7 +2,7 @@
 # usage: build_wide_variants.sh name "cfg-define" [name "cfg-define" ...]
 set -e
 cd /root/repo
-FL="--offload-arch=gfx950 -O3 -std=c++17 -fPIC -I csrc/kernels"
+FL="$(python3 tools/build_native.py --flags) -I csrc/kernels"
 OBJS=$(ls build/*.o | grep -v conv2.o)
 build() { # name, extra defines
   /opt/rocm/bin/hipcc $FL "${@:2}" -c csrc/kernels/conv2.hip -o /tmp/conv2_$1.o && /opt/rocm/bin/hipcc --offload-arch=gfx950 -shared -fPIC -o diag_build/libdtf_wide_$1.so $OBJS /tmp/conv2_$1.o && echo built $1

@@ -12,9 +12,10 @@
 set -e -o pipefail
 cd "$(dirname "$0")/.."
 RT=$(ls -d /opt/rocm/lib/llvm/lib/clang/*/lib/linux | head -1)
+FLAGS=$(python3 tools/build_native.py --flags)
 mkdir -p diag_build/ubsan
 for f in csrc/kernels/*.hip csrc/runtime/*.hip; do
-  echo "/opt/rocm/bin/hipcc --offload-arch=gfx950 -O3 -g -std=c++17 -fPIC -Xarch_host -fsanitize=undefined -Xarch_host -fno-sanitize=function -Xarch_host -fno-sanitize-recover=undefined -I csrc/kernels -c $f -o diag_build/ubsan/$(basename $f .hip).o"
+  echo "/opt/rocm/bin/hipcc $FLAGS -g -Xarch_host -fsanitize=undefined -Xarch_host -fno-sanitize=function -Xarch_host -fno-sanitize-recover=undefined -I csrc/kernels -c $f -o diag_build/ubsan/$(basename $f .hip).o"
 done | xargs -P 8 -I{} sh -c "{}"
 /opt/rocm/bin/hipcc --offload-arch=gfx950 -shared -fPIC -o diag_build/libdtf_kernels_ubsan.so diag_build/ubsan/*.o \
   -Wl,--whole-archive $RT/libclang_rt.ubsan_standalone-x86_64.a $RT/libclang_rt.ubsan_standalone_cxx-x86_64.a -Wl,--no-whole-archive -lpthread -ldl
