@@ -1,5 +1,5 @@
 """Every build of the kernels uses the flags of tools/build_native.py, which keep packed FP32 instructions out (some of their
-forms have returned wrong values, without an error).  CPU only: the library that is
+forms have returned wrong values, without an error), and a change of them rebuilds what is there.  CPU only: the library that is
 loaded is taken apart into its gfx950 code objects and read."""
 import os
 import re
@@ -60,3 +60,53 @@ def test_the_gemm_pipelines_waits_as_shipped(tmp_path, monkeypatch):
     run = subprocess.run
     monkeypatch.setattr(test_gemm_isa.subprocess, "run", lambda cmd, **kw: run([cmd[0], *build_native.DEVICE_FLAGS, *cmd[1:]], **kw))
     test_gemm_isa.test_lds_dma_pipeline_waits_are_exactly_the_pipelines_own(tmp_path)
+
+
+# ------------------------------------------------------------------------------------------------ what is rebuilt
+@pytest.fixture
+def tree(tmp_path, monkeypatch):
+    """A source tree of two kernels; commands are noted and make their output file."""
+    for d in ("csrc/kernels", "csrc/runtime"):
+        (tmp_path / d).mkdir(parents=True)
+    for name in ("a", "b"):
+        (tmp_path / "csrc" / "kernels" / f"{name}.hip").write_text("//")
+    commands = []
+
+    def run(cmd):
+        commands.append(cmd)
+        Path(cmd[cmd.index("-o") + 1]).write_text("built")
+
+    monkeypatch.setattr(build_native, "CSRC", tmp_path / "csrc")
+    monkeypatch.setattr(build_native, "OUT", tmp_path / "lib")
+    monkeypatch.setattr(build_native, "BUILD", tmp_path / "build")
+    monkeypatch.setattr(build_native, "_hipcc", lambda: "hipcc")
+    monkeypatch.setattr(build_native, "_run", run)
+    return commands
+
+
+def compiled(commands):
+    return sorted(Path(c[c.index("-c") + 1]).stem for c in commands if "-c" in c)
+
+
+def test_a_change_of_flags_rebuilds_every_object(tree, monkeypatch):
+    build_native.build_kernels(verbose=False)
+    assert compiled(tree) == ["a", "b"] and "-shared" in tree[-1]
+    del tree[:]
+    build_native.build_kernels(verbose=False)
+    assert tree == []                                        # nothing to do
+    monkeypatch.setattr(build_native, "HIP_FLAGS", build_native.HIP_FLAGS + ["-DX=1"])
+    build_native.build_kernels(verbose=False)
+    assert compiled(tree) == ["a", "b"] and "-shared" in tree[-1] and all("-DX=1" in c for c in tree if "-c" in c)
+    del tree[:]
+    build_native.build_kernels(verbose=False)
+    assert tree == []
+
+
+def test_an_object_whose_flags_are_unknown_is_rebuilt(tree):
+    build_native.build_kernels(verbose=False)
+    for f in build_native.BUILD.glob("a*"):
+        if f.suffix != ".o":
+            f.unlink()
+    del tree[:]
+    build_native.build_kernels(verbose=False)
+    assert compiled(tree) == ["a"]

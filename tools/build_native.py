@@ -6,7 +6,7 @@
 
 hipcc cross-compiles without a GPU, so this runs on the CPU-only build box.  The
 .so files land in distributed_tensorflow_amd/_lib/ (git-ignored, but shipped to
-the GPU box by gpurun).  Objects are cached under build/ keyed by source mtime.
+the GPU box by gpurun).  Objects are cached under build/ by their sources' times and the command that made them.
 ``--flags`` prints the compile flags for scripts that build kernels themselves.
 """
 from __future__ import annotations
@@ -63,10 +63,19 @@ def build_kernels(force: bool = False, verbose: bool = True) -> Path:
     for s in srcs:
         o = BUILD / (s.stem + ".o")
         objs.append(o)
-        if force or _newer([s] + headers, o):
-            jobs.append([hipcc, *HIP_FLAGS, "-Wall", "-Wextra", "-Werror", "-I", str(CSRC / "kernels"), "-c", str(s), "-o", str(o)])
+        cmd = [hipcc, *HIP_FLAGS, "-Wall", "-Wextra", "-Werror", "-I", str(CSRC / "kernels"), "-c", str(s), "-o", str(o)]
+        made_by = o.with_suffix(".cmd")        # beside the object: the command that made it
+        if force or _newer([s] + headers, o) or not made_by.exists() or made_by.read_text() != " ".join(cmd):
+            jobs.append((cmd, made_by))
+
+    def compile_one(job):
+        cmd, made_by = job
+        made_by.unlink(missing_ok=True)
+        _run(cmd)
+        made_by.write_text(" ".join(cmd))
+
     with cf.ThreadPoolExecutor(max_workers=min(8, max(1, len(jobs)))) as ex:
-        list(ex.map(_run, jobs))
+        list(ex.map(compile_one, jobs))
     lib = OUT / "libdtf_kernels.so"
     if force or jobs or _newer(objs, lib):
         _run([hipcc, f"--offload-arch={ARCH}", "-shared", "-fPIC", "-o", str(lib)] + [str(o) for o in objs])
