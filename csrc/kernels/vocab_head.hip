@@ -27,6 +27,9 @@ __device__ __forceinline__ f32x4 vh_mma(const u32x4& a, const u32x4& b, f32x4 c)
 // the ones before it leave (together all 24), products of two bf16 values are exact in the fp32 accumulators, and of the nine the
 // three smallest are left out:
 //   a b = a1 b1 + (a1 b2 + a2 b1) + (a1 b3 + a2 b2 + a3 b1) + at most 2^-21 |a b| (2^-23 on average)
+// for values from about 2e-34 on; below, the third part ends at 2^-133, bf16's smallest step, and up to 2^-133 (|a| + |b|) is lost
+// as well (of 1e-35 1e-5, of 1e-37 1e-3: an upstream gradient of a row, which is multiplied into d, may be as small; the common
+// grad_scale is not).
 // Six bf16 instructions do 16 x 16 x 32 in 96 cycles, the fp32 ones (16 x 16 x 4) take 256.  An infinite value gives NaN (its
 // second part is inf - inf).  The leading bits are cut off, not rounded: the conversion instruction is several times slower than a
 // mask and a byte permutation (4096 x 1024 x 16000 forward 605 and 567 us; with the fp32 instructions 971, 138 TFLOP/s of their

@@ -7,7 +7,8 @@ The ten-class head of the engine keeps a row's logits in registers; here the cla
 the engine's: rows of hidden units ``h`` [n, hidden], the weight transposed ``wT`` [classes, hidden], int32 labels, the
 per-row loss and everything that is summed in fp32; both operands bf16 (gradients of them bf16 as well, ``dwT`` on request
 fp32) or both fp32 (every product to within 2^-21, on average 2^-23, from three bf16 parts of each value on the bf16 matrix
-cores; infinite values make NaN).  Rows of ``h`` and ``wT`` may be further apart than they are long.  Copied once per call are
+cores, where neither factor is below 2e-34 -- products of smaller ones lose up to 2^-133 of the other besides --; infinite
+values make NaN).  Rows of ``h`` and ``wT`` may be further apart than they are long.  Copied once per call are
 rows of ``h`` that do not start on 16 bytes, and rows of ``wT`` that do not start on 4 bytes or leave a gap behind a broken 16
 bytes (bf16: an odd number of hidden units).
 

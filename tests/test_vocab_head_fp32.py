@@ -6,7 +6,10 @@ elsewhere.  Then every element of dh is ONE product, row_scale_i * w[y_i][k], an
 
 Bound, u = 2^-24: 8 u of a product for the parts that are left out (2^-21), and of the running sum 2 u for each of the six
 instructions that add to it (rounding or truncation), 2 u for the last factor and the store.  Instructions that add zeros round
-nothing.  Two parts only would leave out up to 2^-14 of a product, typically 2^-16 = 256 u."""
+nothing.  Two parts only would leave out up to 2^-14 of a product, typically 2^-16 = 256 u.
+
+The smallest step of a bf16 value is 2^-133: what a value's three parts leave is below 2^-24 of it or below 2^-133, whichever is
+more, and a product a b is off by up to 2^-133 (|a| + |b|) besides.  That counts where an operand is below about 2^-112, 2e-34."""
 import numpy as np
 import pytest
 import torch
@@ -15,6 +18,9 @@ from distributed_tensorflow_amd.ops import vocab_head_bwd, vocab_head_fwd
 
 gpu = pytest.mark.gpu
 U = 2.0 ** -24
+
+
+LEAST = 2.0 ** -133
 
 
 def bound(terms, sums):
@@ -56,6 +62,20 @@ def test_three_parts_are_within_the_bound_and_less_is_not(rounded):
     for lost in ((1, 1), (0, 2), (2, 0)):
         less = err(product(a, b, rounded=rounded, terms=[t for t in TERMS if t != lost]))
         assert (less > bound(1, 1.0)).mean() > 0.3, lost
+
+
+@pytest.mark.parametrize("rounded", [False, True])
+@pytest.mark.parametrize("exp", [-112, -120, -126, -132])
+def test_small_values_keep_what_bf16_holds(exp, rounded):
+    g = np.random.default_rng(2)
+    a = (g.standard_normal(100000) * 2.0 ** exp).astype(np.float32)
+    b = g.standard_normal(100000).astype(np.float32)
+    want = a.astype(np.float64) * b
+    d = np.abs(product(a, b, rounded=rounded) - want)
+    assert (d <= 8 * U * np.abs(want) + LEAST * (np.abs(a.astype(np.float64)) + np.abs(b))).all()
+    # only small values (a normal distribution has some of any size) lose more than others do
+    more = d > 8 * U * np.abs(want)
+    assert (np.abs(a[more].astype(np.float64)) < 2.0 ** -110).all() and (more.any() or exp == -112)
 
 
 # --------------------------------------------------------------------------------------------------------- kernels
@@ -110,3 +130,21 @@ def test_logits_of_single_products(gpu_lib, n, hidden, classes):
         want = v.double() * w[c].double()[k]
         within(lse, want, bound(1, want.abs()) + 4 * U * (1 + want.abs()), f"lse of class {c}")
         assert float(loss.abs().max()) <= 4 * U * (1 + float(want.abs().max()))
+
+
+@gpu
+@pytest.mark.parametrize("exp", [-100, -112, -120, -126])
+@pytest.mark.parametrize("n,hidden,classes", [(5, 200, 777), (100, 200, 777), (300, 200, 777)])
+def test_small_upstream_gradients(gpu_lib, n, hidden, classes, exp):
+    """row_scale is multiplied into d before d is cut into parts; grad_scale is not."""
+    g = torch.Generator(device="cuda").manual_seed(n)
+    h, w = (torch.randn((r, hidden), device="cuda", generator=g) for r in (n, classes))
+    y = torch.randperm(classes, device="cuda", generator=g)[:n]
+    lse = torch.full((n,), 1000.0, device="cuda")
+    base = torch.rand(n, device="cuda", generator=g) + 0.5
+    for s, grad_scale, least in ((base * 2.0 ** exp, 1.0, LEAST), (base, 2.0 ** exp, 0.0)):
+        dh, dw, _ = vocab_head_bwd(h, w, y.to(torch.int32), lse, row_scale=s, grad_scale=grad_scale)
+        sd = (s.double() * grad_scale)[:, None]
+        for got, x, what in ((dh, w.double()[y], "dh"), (dw[y], h.double(), "dw")):
+            want = -sd * x
+            within(got, want, bound(1, want.abs()) + least * (sd + x.abs()) + 2.0 ** -149, what)
