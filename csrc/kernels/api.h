@@ -171,8 +171,8 @@ long dtf_vocab_head_workspace(int dtype, int backward_pass, const void* h, long 
 int dtf_vocab_head_fwd(int dtype, const void* h, long ldh, const void* w, long ldw, const void* bias, const void* labels, int n,
                        int H, int V, int ignore, void* loss, void* lse, void* ws, long ws_bytes, hipStream_t s);
 int dtf_vocab_head_bwd(int dtype, const void* h, long ldh, const void* w, long ldw, const void* bias, const void* labels,
-                       const void* lse, const void* row_scale, float grad_scale, int n, int H, int V, int ignore, int piece, void* dh,
-                       void* dw, int dw_f32, void* db, void* ws, long ws_bytes, hipStream_t s);
+                       const void* lse, const void* row_scale, float grad_scale, int n, int H, int V, int ignore, int piece, int keep,
+                       void* dh, void* dw, int dw_f32, void* db, void* ws, long ws_bytes, hipStream_t s);
 // ---- global norm of a list of gradient tensors and clipping by it (clip.hip); mirrored in ops/clip.py ----
 struct DtfClipSpan {
   const void* in;

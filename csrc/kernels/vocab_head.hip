@@ -11,6 +11,7 @@
 //
 // All products run through one kernel template, vh_gemm: out[j][i] = sum_k A(i, k) B(j, k), where an operand lies in memory
 // with k contiguous (fast) or with its rows contiguous (slow); nothing is transposed in memory.
+#include <type_traits>
 #include "common.hpp"
 #include "api.h"
 
@@ -679,7 +680,10 @@ struct VhForward {
 // a tile of them, the rounding errors themselves are kept as rows 32 to 63, next to nothing in time: one row's gradient is then as
 // exact as if d had stayed in fp32 (one row: 0.17 % rms, the operand type's own rounding, instead of up to 0.4; 16 rows, 4096 x
 // 32000, backward 161 -> 166 us.  For 64 rows, a second tile, it would be 168 -> 211 us, and errors of many rows even out.)
-struct VhGradLogits {
+// KEEP: more rows keep them, too, behind d, and dh and dw are products of both, for a caller who asks for it (4096 x 1024 x 65536:
+// backward 1547 -> 2694 us, dw in fp32 off by 1.4e-6 rms instead of 8.7e-4).
+template <bool KEEP>
+struct VhGradLogitsT {
   static constexpr bool kCopies = true;
   VhCopy copy;              // h for dw: does not depend on d and needs no launch of its own
   const float* bias;        // of the piece
@@ -688,7 +692,8 @@ struct VhGradLogits {
   const float* row_scale;   // or nullptr
   int v0, classes, ignore;  // the product's first class, all classes
   void* d;
-  long ldd, rest;           // elements from a row to the row of its rounding errors (0: not kept; else rows up to 32 are written)
+  long ldd, rest;           // elements from a row to the row of its rounding errors (0: not kept; else, without KEEP, rows up to 32
+                            // are written)
   int places;               // of this product's classes: up to there d is written
   float* dbpart;            // [row tile][ldd] or nullptr
   int dbplaces;             // up to there it is written
@@ -704,7 +709,7 @@ struct VhGradLogits {
   }
   template <int BM, int BN, int NT>
   __device__ __forceinline__ VhEarly<BM, BN, NT> request(const VhOperands& p, int m0, int n0, int tid) const {
-    return vh_request<VhGradLogits, BM, BN, NT>(*this, p, m0, n0, tid);
+    return vh_request<VhGradLogitsT, BM, BN, NT>(*this, p, m0, n0, tid);
   }
   template <int BM, int BN, int NT>
   __device__ __forceinline__ void keep(const VhEarly<BM, BN, NT>& x, VhLogitsInputs<BM, BN>* in, int tid) const {
@@ -721,7 +726,7 @@ struct VhGradLogits {
 #pragma unroll
     for (int j = 0; j < NTL; ++j) {
       const int jl = c.wn0 + 16 * j + i16, row = c.n0 + jl;
-      const bool live = row < (REST && rest ? 32 : p.N);
+      const bool live = row < (!KEEP && REST && rest ? 32 : p.N);
       const VhRowInputs x = in.row[jl];
       const int y = x.label - (c.wm0 + 4 * g);
       const bool hit = y >= 0 && y < Tile::WM, dead = x.sc == 0.f;
@@ -749,7 +754,18 @@ struct VhGradLogits {
             const int m = mw + 16 * i;
             const f32x4 v = c.acc[i][j], x = c.acc[i + 1][j];
             const bf16x8 y = {(T)v[0], (T)v[1], (T)v[2], (T)v[3], (T)x[0], (T)x[1], (T)x[2], (T)x[3]};
-            if (m < places) *reinterpret_cast<bf16x8*>(o + vh_place(m)) = y;
+            if (m < places) {
+              *reinterpret_cast<bf16x8*>(o + vh_place(m)) = y;
+              if constexpr (KEEP) {
+                bf16x8 left;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                  left[r] = (T)(v[r] - (float)y[r]);
+                  left[4 + r] = (T)(x[r] - (float)y[4 + r]);
+                }
+                *reinterpret_cast<bf16x8*>(o + vh_place(m) + rest) = left;
+              }
+            }
           }
         } else {
           typedef __attribute__((ext_vector_type(4))) T T4;
@@ -1179,7 +1195,9 @@ struct Plan {
   long total;
   long ldk, ldv;            // padded hidden units, classes of a piece
   int cfg, piece, pieces, splits_h, splits_w;
-  int parts, drows;         // parts == 2: d has 64 rows, its rounding errors from row 32 on
+  int few;                  // d has 64 rows, its rounding errors from row 32 on
+  int keep;                 // d has 2 n rows, its rounding errors from row n on
+  int drows, rest;          // rows of d; from a row to that of its rounding errors (0: not kept)
   GradTile tile_h, tile_w;
 };
 
@@ -1194,6 +1212,7 @@ int piece_for(long n, int classes) {
   return v >= classes ? classes : (int)v;
 }
 
+// backward: 1, or 2 with the rounding errors of d kept for any number of rows
 Plan plan_for(int dtype, int backward, long n, int H, int V, bool h_ok, bool w_ok, bool bias, int piece) {
   Plan q{};
   const int E = esize(dtype);
@@ -1205,11 +1224,13 @@ Plan plan_for(int dtype, int backward, long n, int H, int V, bool h_ok, bool w_o
   };
   q.cfg = config_for(n);
   q.ldk = up(H, 16 / E);
-  q.parts = backward && E == 2 && n <= 32 ? 2 : 1;
-  q.drows = q.parts == 2 ? 64 : (int)n;
+  q.few = backward && E == 2 && n <= 32;
+  q.keep = backward == 2 && E == 2 && !q.few;
+  q.rest = q.few ? 32 : (q.keep ? (int)n : 0);
+  q.drows = q.few ? 64 : (int)(n + q.rest);
   const long dn = q.drows;
   if (!h_ok || backward) q.h_copy = take(dn * q.ldk * E);
-  q.piece = backward ? (piece > 0 ? (int)up(piece, kPiece) : piece_for(n, V)) : V;
+  q.piece = backward ? (piece > 0 ? (int)up(piece, kPiece) : piece_for(n + (q.keep ? n : 0), V)) : V;
   if (q.piece > V) q.piece = V;
   q.pieces = cdiv(V, q.piece);
   if (!w_ok) q.w_copy = take((long)q.piece * q.ldk * E);
@@ -1223,9 +1244,9 @@ Plan plan_for(int dtype, int backward, long n, int H, int V, bool h_ok, bool w_o
     q.d = take(dn * q.ldv * E);
     q.tile_h = dh_tile(E, q.cfg, n, H);
     q.tile_w = dw_tile(E, q.cfg, H, q.piece);
-    q.splits_h = splits_for((long)cdiv(H, q.tile_h.bm) * cdiv(dn, q.tile_h.bn), cdiv(q.ldv, KT), q.tile_h.want);
+    q.splits_h = splits_for((long)cdiv(H, q.tile_h.bm) * cdiv(q.few ? dn : n, q.tile_h.bn), cdiv(q.ldv, KT), q.tile_h.want);
     q.splits_w = splits_for((long)cdiv(H, q.tile_w.bm) * cdiv(q.piece, q.tile_w.bn), cdiv(dn, KT), q.tile_w.want);
-    if (q.pieces > 1 || q.splits_h > 1) q.sum_h = take(q.splits_h * n * H * 4);
+    if (q.pieces > 1 || q.splits_h > 1 || q.keep) q.sum_h = take(q.splits_h * n * H * 4);
     if (q.splits_w > 1) q.sum_w = take(q.splits_w * (long)q.piece * H * 4);
     if (bias) q.dbpart = take((long)cdiv(n, 32) * q.ldv * 4);      // at most that many row tiles
   }
@@ -1292,14 +1313,14 @@ int forward(const void* h, long ldh, const void* w, long ldw, const float* bias,
 
 template <typename T>
 int backward(const void* h, long ldh, const void* w, long ldw, const float* bias, const int* labels, const float* lse,
-             const float* row_scale, float grad_scale, int n, int H, int V, int ignore, int piece, void* dh, void* dw, int dw_f32,
-             void* db, void* ws, hipStream_t s) {
+             const float* row_scale, float grad_scale, int n, int H, int V, int ignore, int piece, int keep, void* dh, void* dw,
+             int dw_f32, void* db, void* ws, hipStream_t s) {
   const int E = sizeof(T), KT = 128 / E;
   const bool h_ok = rows_ok(h, ldh, H, E);
-  const Plan q = plan_for(E == 2 ? 1 : 0, 1, n, H, V, h_ok, w_rows_ok(w, ldw, H, E), db != nullptr, piece);
+  const Plan q = plan_for(E == 2 ? 1 : 0, keep ? 2 : 1, n, H, V, h_ok, w_rows_ok(w, ldw, H, E), db != nullptr, piece);
   const T* hp = at<T>(ws, q.h_copy);
   const int dn = q.drows;
-  VhCopy copy{h, ldh, q.parts == 2 ? 32 : n, n, H, at<T>(ws, q.h_copy), q.ldk, labels, ignore, q.parts == 2 ? 32 * q.ldk : 0, 0};
+  VhCopy copy{h, ldh, q.few ? 32 : n, n, H, at<T>(ws, q.h_copy), q.ldk, labels, ignore, q.rest * q.ldk, 0};
   // Only dw needs the copy where h is aligned: few rows are copied next to the first product (16 rows, 4096 x 32000: 4.5 us less);
   // among large tiles, which hold a CU each, the copy is a launch of its own.
   const bool beside = h_ok && q.cfg != kLarge;
@@ -1319,16 +1340,21 @@ int backward(const void* h, long ldh, const void* w, long ldw, const float* bias
     }
     T* d = at<T>(ws, q.d);
     const LogitsTiling t = logits_tiling(E, q.cfg, n, vn);
-    VH_TRY(logits_all<T>(t, VhOperands{wp, hl, ldwp, ldl, vn, n, q.w_copy ? (int)q.ldk : H, (int)q.ldk, 0, 0, 0, 0}, [&](int part, int c0, int) {
-      VhCopy now = copy;
-      if (k || part) now.blocks = 0;
-      // one tile of rows: its sums are the whole ones
-      const bool whole = n <= t.kind[part].bn;
-      float* dbp = !db ? nullptr : whole ? (float*)db + v0 + c0 : at<float>(ws, q.dbpart) + c0;
-      return VhGradLogits{now, bias ? bias + v0 + c0 : nullptr, labels, lse, row_scale, v0 + c0, V, ignore, d + c0, ldv,
-                          q.parts == 2 ? 32 * ldv : 0, (int)ldv - c0, dbp, whole ? (part ? vn - t.first : t.first) : (int)ldv - c0,
-                          whole ? grad_scale : 1.f};
-    }, s));
+    const VhOperands z{wp, hl, ldwp, ldl, vn, n, q.w_copy ? (int)q.ldk : H, (int)q.ldk, 0, 0, 0, 0};
+    auto logits_with = [&](auto keep_d) {
+      return logits_all<T>(t, z, [&](int part, int c0, int) {
+        VhCopy now = copy;
+        if (k || part) now.blocks = 0;
+        // one tile of rows: its sums are the whole ones
+        const bool whole = n <= t.kind[part].bn;
+        float* dbp = !db ? nullptr : whole ? (float*)db + v0 + c0 : at<float>(ws, q.dbpart) + c0;
+        return VhGradLogitsT<decltype(keep_d)::value>{
+            now, bias ? bias + v0 + c0 : nullptr, labels, lse, row_scale, v0 + c0, V, ignore, d + c0, ldv, q.rest * ldv, (int)ldv - c0, dbp,
+            whole ? (part ? vn - t.first : t.first) : (int)ldv - c0, whole ? grad_scale : 1.f};
+      }, s);
+    };
+    if constexpr (sizeof(T) == 2) VH_TRY(q.keep ? logits_with(std::true_type{}) : logits_with(std::false_type{}));
+    else VH_TRY(logits_with(std::false_type{}));
     for (int part = 0; db && part < 2; ++part) {
       const int c0 = part ? t.first : 0, cn = part ? vn - t.first : t.first;
       if (!cn || n <= t.kind[part].bn) continue;
@@ -1352,8 +1378,15 @@ int backward(const void* h, long ldh, const void* w, long ldw, const float* bias
     }
     if (dh) {
       const bool last = k == q.pieces - 1, split = q.splits_h > 1;
-      VhStore st{dh, H, 0, 0, n, q.sum_h ? at<float>(ws, q.sum_h) : nullptr, k == 0, last && !split, grad_scale, q.parts == 2};
-      VH_TRY((product_dh<T>(q.cfg, q.tile_h, VhOperands{wp, d, ldwp, ldv, H, dn, vn, (int)ldv, 0, 0, 0, 0}, q.splits_h, st, s)));
+      VhStore st{dh, H, 0, 0, n, q.sum_h ? at<float>(ws, q.sum_h) : nullptr, k == 0, last && !split && !q.keep, grad_scale, q.few};
+      VhOperands o{wp, d, ldwp, ldv, H, q.few ? dn : n, vn, (int)ldv, 0, 0, 0, 0};
+      VH_TRY((product_dh<T>(q.cfg, q.tile_h, o, q.splits_h, st, s)));
+      if (q.keep) {             // the errors' product on top
+        o.B = d + q.rest * ldv;
+        st.first = 0;
+        st.last = last && !split;
+        VH_TRY((product_dh<T>(q.cfg, q.tile_h, o, q.splits_h, st, s)));
+      }
       if (last && split) VH_TRY(launch_sum(at<float>(ws, q.sum_h), (long)n * H, q.splits_h, (T*)dh, grad_scale, s));
     }
   }
@@ -1369,10 +1402,11 @@ bool sizes_ok(int dtype, long n, int H, int V, long ldh, long ldw) {
 
 extern "C" {
 
-// dtype: 0 fp32, 1 bf16.  piece: classes per piece of the backward pass (0: the default).  Returns < 0 for bad arguments.
+// dtype: 0 fp32, 1 bf16.  backward_pass: 1, or 2 for one with keep.  piece: classes per piece of the backward pass (0: the
+// default).  Returns < 0 for bad arguments.
 long dtf_vocab_head_workspace(int dtype, int backward_pass, const void* h, long ldh, const void* w, long ldw, int n, int H, int V,
                               int bias, int piece) {
-  if (!sizes_ok(dtype, n, H, V, ldh, ldw) || piece < 0 || piece > kMaxRow) return -3;
+  if (!sizes_ok(dtype, n, H, V, ldh, ldw) || backward_pass < 0 || backward_pass > 2 || piece < 0 || piece > kMaxRow) return -3;
   const int E = esize(dtype);
   return plan_for(dtype, backward_pass, n, H, V, rows_ok(h, ldh, H, E), w_rows_ok(w, ldw, H, E), bias != 0, piece).total;
 }
@@ -1388,17 +1422,17 @@ int dtf_vocab_head_fwd(int dtype, const void* h, long ldh, const void* w, long l
 }
 
 // dh [n][H] in the operand type, dw [V][H] in the operand type or fp32 (dw_f32), db [V] fp32; each may be NULL (not wanted).
-// d loss / d loss_i = grad_scale * row_scale[i] (row_scale fp32 [n] or NULL: 1)
+// d loss / d loss_i = grad_scale * row_scale[i] (row_scale fp32 [n] or NULL: 1).  keep: bf16 operands keep what rounding drops of d
 int dtf_vocab_head_bwd(int dtype, const void* h, long ldh, const void* w, long ldw, const void* bias, const void* labels,
-                       const void* lse, const void* row_scale, float grad_scale, int n, int H, int V, int ignore, int piece, void* dh,
-                       void* dw, int dw_f32, void* db, void* ws, long ws_bytes, hipStream_t s) {
+                       const void* lse, const void* row_scale, float grad_scale, int n, int H, int V, int ignore, int piece, int keep,
+                       void* dh, void* dw, int dw_f32, void* db, void* ws, long ws_bytes, hipStream_t s) {
   if (!sizes_ok(dtype, n, H, V, ldh, ldw) || !h || !w || !labels || !lse || !ws || ((uintptr_t)ws & 255) || piece < 0 || piece > kMaxRow) return -3;
   if ((uintptr_t)h & (esize(dtype) - 1) || (uintptr_t)w & (esize(dtype) - 1) || ((uintptr_t)dh & 15) || ((uintptr_t)dw & 15)) return -3;
-  if (ws_bytes < dtf_vocab_head_workspace(dtype, 1, h, ldh, w, ldw, n, H, V, db != nullptr, piece)) return -2;
+  if (ws_bytes < dtf_vocab_head_workspace(dtype, keep ? 2 : 1, h, ldh, w, ldw, n, H, V, db != nullptr, piece)) return -2;
   return dtype == 1 ? backward<bf16>(h, ldh, w, ldw, (const float*)bias, (const int*)labels, (const float*)lse, (const float*)row_scale,
-                                     grad_scale, n, H, V, ignore, piece, dh, dw, dw_f32, db, ws, s)
+                                     grad_scale, n, H, V, ignore, piece, keep, dh, dw, dw_f32, db, ws, s)
                     : backward<float>(h, ldh, w, ldw, (const float*)bias, (const int*)labels, (const float*)lse, (const float*)row_scale,
-                                      grad_scale, n, H, V, ignore, piece, dh, dw, dw_f32, db, ws, s);
+                                      grad_scale, n, H, V, ignore, piece, keep, dh, dw, dw_f32, db, ws, s);
 }
 
 }  // extern "C"

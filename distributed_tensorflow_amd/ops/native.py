@@ -146,7 +146,7 @@ _SIGS = {
     "dtf_vocab_head_fwd": [c_int, c_void_p, c_long, c_void_p, c_long, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_void_p,
                            c_void_p, c_void_p, c_long, c_void_p],
     "dtf_vocab_head_bwd": [c_int, c_void_p, c_long, c_void_p, c_long, c_void_p, c_void_p, c_void_p, c_void_p, c_float, c_int, c_int,
-                           c_int, c_int, c_int, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_long, c_void_p],
+                           c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_long, c_void_p],
     # ---- global norm and clipping (csrc/kernels/clip.hip; spans: ops/clip.py ClipSpan) ----
     "dtf_clip_table": [c_int, c_void_p, c_void_p, c_long, ctypes.POINTER(c_int)],
     "dtf_clip_partials": [c_long],

@@ -7,8 +7,7 @@ The ten-class head of the engine keeps a row's logits in registers; here the cla
 the engine's: rows of hidden units ``h`` [n, hidden], the weight transposed ``wT`` [classes, hidden], int32 labels, the
 per-row loss and everything that is summed in fp32; both operands bf16 (gradients of them bf16 as well, ``dwT`` on request
 fp32) or both fp32 (every product to within 2^-21, on average 2^-23, from three bf16 parts of each value on the bf16 matrix
-cores, where neither factor is below 2e-34 -- products of smaller ones lose up to 2^-133 of the other besides --; infinite
-values make NaN).  Rows of ``h`` and ``wT`` may be further apart than they are long.  Copied once per call are
+cores; where a factor is below 2e-34, up to 2^-133 of the other is lost as well; infinite values make NaN).  Rows of ``h`` and ``wT`` may be further apart than they are long.  Copied once per call are
 rows of ``h`` that do not start on 16 bytes, and rows of ``wT`` that do not start on 4 bytes or leave a gap behind a broken 16
 bytes (bf16: an odd number of hidden units).
 
@@ -18,8 +17,8 @@ A row whose label is ``ignore_label`` has loss 0 and takes no part in any gradie
 weight makes NaN, of its own class or of the one before it.
 
 The backward pass computes the logits again, one piece of the classes at a time: its workspace holds the gradient of the
-piece's logits in the operands' type (at most 2^27 values, or 1024 classes of very many rows), a copy of ``h`` without its
-ignored rows, fp32 sums of ``dh`` where there are several pieces or the classes are cut among workgroups, and the copies
+piece's logits in the operands' type (at most 2^27 values, or 1024 classes of very many rows; bf16 drops up to 2^-9 of a value
+there, unless ``keep_rounding`` asks for two bf16 values), a copy of ``h`` without its ignored rows, fp32 sums of ``dh`` where there are several pieces or the classes are cut among workgroups, and the copies
 above.  Calls launch on the current stream of the operands' device, take their workspace from PyTorch's allocator on that
 stream and keep nothing, so they can be captured into HIP graphs and run on several streams at once.  Autograd does not record
 them: operands that require gradients are taken under ``torch.no_grad()`` only.
@@ -114,11 +113,14 @@ def _span(t: torch.Tensor) -> Tuple[int, int]:
 def vocab_head_bwd(h: torch.Tensor, wT: torch.Tensor, labels: torch.Tensor, lse: torch.Tensor,
                    bias: Optional[torch.Tensor] = None, *, grad_scale: float = 1.0, row_scale: Optional[torch.Tensor] = None,
                    ignore_label: int = -1, need_dh: bool = True, need_dwT: bool = True, dh: Optional[torch.Tensor] = None,
-                   dwT: Optional[torch.Tensor] = None, dbias: Optional[torch.Tensor] = None, piece: int = 0):
+                   dwT: Optional[torch.Tensor] = None, dbias: Optional[torch.Tensor] = None, piece: int = 0,
+                   keep_rounding: bool = False):
     """(dh, dwT, dbias) of sum_i grad_scale * row_scale[i] * loss_rows[i]; dbias is None without a bias, dh / dwT where they
     are not wanted.  ``row_scale``: fp32 [n], the upstream gradient of the loss rows (default: ones).  ``dh`` / ``dwT`` /
     ``dbias``: where to write (contiguous, 16-byte aligned; ``dwT`` in the operands' type or fp32), e.g. views of a gradient
-    arena.  ``piece``: classes per piece (rounded up to 256; 0: chosen from n)."""
+    arena.  ``piece``: classes per piece (rounded up to 256; 0: chosen from n).  ``keep_rounding``: bf16 operands keep what
+    rounding drops of the logits' gradient for any number of rows, not up to 32 only; dh and dwT then take two products each (1.6
+    to 1.75 times the time of a large backward pass) and are as exact as if it had stayed in fp32."""
     n, hidden, classes, ldh, ldw = _check(h, wT, labels, bias, ignore_label, lse, row_scale, dh, dwT, dbias)
     _vector(lse, "lse", n, torch.float32, h.device)
     _vector(row_scale, "row_scale", n, torch.float32, h.device)
@@ -159,11 +161,12 @@ def vocab_head_bwd(h: torch.Tensor, wT: torch.Tensor, labels: torch.Tensor, lse:
         torch.autograd.graph.increment_version(given)       # written in place
     lib, dt = native.load(), _DTYPES[h.dtype]
     with on_device(dev) as stream:
-        need = lib.dtf_vocab_head_workspace(dt, 1, ptr(h), ldh, ptr(wT), ldw, n, hidden, classes, int(dbias is not None), piece)
+        need = lib.dtf_vocab_head_workspace(dt, 2 if keep_rounding else 1, ptr(h), ldh, ptr(wT), ldw, n, hidden, classes, int(dbias is not None), piece)
         check(min(need, 0), "vocab_head_workspace")
         ws = torch.empty(need, dtype=torch.uint8, device=dev)
         check(lib.dtf_vocab_head_bwd(dt, ptr(h), ldh, ptr(wT), ldw, ptr(bias), ptr(labels), ptr(lse), ptr(row_scale),
-                                     float(grad_scale), n, hidden, classes, ignore_label, piece, ptr(dh), ptr(dwT),
-                                     int(dwT is not None and dwT.dtype == torch.float32), ptr(dbias), ptr(ws), need, stream),
+                                     float(grad_scale), n, hidden, classes, ignore_label, piece, int(keep_rounding), ptr(dh),
+                                     ptr(dwT), int(dwT is not None and dwT.dtype == torch.float32), ptr(dbias), ptr(ws), need,
+                                     stream),
               "vocab_head_bwd")
     return dh, dwT, dbias
