@@ -1056,10 +1056,9 @@ GradTile dw_tile(int E, int cfg, int H, int classes) {
 
 // How the logits product of some classes is tiled: the classes below `first` in tiles of one kind, the others in a second one.
 // The large kinds run one workgroup per CU, so what counts is the number of rounds over the 256 CUs times the length of a round
-// (measured at H = 4096, against 256 x 256: 0.82 for 192 x 256, 0.68 for 256 x 128), and a last round for a few tiles is as long
-// as any other: its classes go to small tiles instead.  777 rows x 50001 classes: 784 tiles are four rounds, 362 us; three
-// rounds and 91 small tiles 330 us.  Logits of few tiles are cut as small as the
-// CUs hold them at once, because a workgroup alone on its CU takes long over its K (300 rows, 2048 x 5000 bf16: 30 us in large
+// (measured at H = 4096, against 256 x 256, and used at every width: 0.82 for 192 x 256, 0.68 for 256 x 128), and a last round
+// for a few tiles is as long as any other: its classes go to small tiles instead.  777 rows x 50001 classes: 784 tiles are four
+// rounds, 362 us; three rounds and 91 small tiles 330 us.  Logits of few tiles are cut as small as the CUs hold them at once, because a workgroup alone on its CU takes long over its K (300 rows, 2048 x 5000 bf16: 30 us in large
 // tiles, 20 in 200 of 128 x 64; 526 rows, 2944 x 537 fp32: 101 us in 45 tiles of 128 x 64, 52 in 153 of 64 x 32).  Room for
 // 512 tiles in bf16 (500 rows, 1000 x 12000: 24 us large, 30 in 752 small ones), 768 in fp32, whose tiles take longer (600 rows,
 // 2048 x 8000: 180 us large, 170 in 630 small ones).

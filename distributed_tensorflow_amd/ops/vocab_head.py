@@ -7,9 +7,9 @@ The ten-class head of the engine keeps a row's logits in registers; here the cla
 the engine's: rows of hidden units ``h`` [n, hidden], the weight transposed ``wT`` [classes, hidden], int32 labels, the
 per-row loss and everything that is summed in fp32; both operands bf16 (gradients of them bf16 as well, ``dwT`` on request
 fp32) or both fp32 (every product to within 2^-21, on average 2^-23, from three bf16 parts of each value on the bf16 matrix
-cores; where a factor is below 2e-34, up to 2^-133 of the other is lost as well; infinite values make NaN).  Rows of ``h`` and ``wT`` may be further apart than they are long.  Copied once per call are
-rows of ``h`` that do not start on 16 bytes, and rows of ``wT`` that do not start on 4 bytes or leave a gap behind a broken 16
-bytes (bf16: an odd number of hidden units).
+cores; where a factor is below 2e-34, up to 2^-133 of the other is lost as well; infinite values make NaN).  Rows of ``h``
+and ``wT`` may be further apart than they are long.  Copied once per call are rows of ``h`` that do not start on 16 bytes, and
+rows of ``wT`` that do not start on 4 bytes or leave a gap behind a broken 16 bytes (bf16: an odd number of hidden units).
 
 A row whose label is ``ignore_label`` has loss 0 and takes no part in any gradient, whatever its hidden units hold
 (padding); any other label outside the classes makes its loss, and with it every gradient it enters, NaN, as
@@ -18,8 +18,8 @@ weight makes NaN, of its own class or of the one before it.
 
 The backward pass computes the logits again, one piece of the classes at a time: its workspace holds the gradient of the
 piece's logits in the operands' type (at most 2^27 values, or 1024 classes of very many rows; bf16 drops up to 2^-9 of a value
-there, unless ``keep_rounding`` asks for two bf16 values), a copy of ``h`` without its ignored rows, fp32 sums of ``dh`` where there are several pieces or the classes are cut among workgroups, and the copies
-above.  Calls launch on the current stream of the operands' device, take their workspace from PyTorch's allocator on that
+there, unless ``keep_rounding`` asks for two bf16 values), a copy of ``h`` without its ignored rows, fp32 sums of ``dh`` where
+there are several pieces or the classes are cut among workgroups, and the copies above.  Calls launch on the current stream of the operands' device, take their workspace from PyTorch's allocator on that
 stream and keep nothing, so they can be captured into HIP graphs and run on several streams at once.  Autograd does not record
 them: operands that require gradients are taken under ``torch.no_grad()`` only.
 Kernels: csrc/kernels/vocab_head.hip.
