@@ -17,11 +17,12 @@ A row whose label is ``ignore_label`` has loss 0 and takes no part in any gradie
 weight makes NaN, of its own class or of the one before it.
 
 The backward pass computes the logits again, one piece of the classes at a time: its workspace holds the gradient of the
-piece's logits in the operands' type (at most 2^27 values, or 1024 classes of very many rows; bf16 drops up to 2^-9 of a value
+piece's logits in the operands' type (at most 2^27 values, or 1024 classes of very many rows; bf16 drops up to 2^-8 of a value
 there, unless ``keep_rounding`` asks for two bf16 values), a copy of ``h`` without its ignored rows, fp32 sums of ``dh`` where
-there are several pieces or the classes are cut among workgroups, and the copies above.  Calls launch on the current stream of the operands' device, take their workspace from PyTorch's allocator on that
-stream and keep nothing, so they can be captured into HIP graphs and run on several streams at once.  Autograd does not record
-them: operands that require gradients are taken under ``torch.no_grad()`` only.
+there are several pieces or the classes are cut among workgroups, and the copies above.  Calls launch on the current stream of
+the operands' device, take their workspace from PyTorch's allocator on that stream and keep nothing, so they can be captured
+into HIP graphs and run on several streams at once.  Autograd does not record them: operands that require gradients are taken
+under ``torch.no_grad()`` only.
 Kernels: csrc/kernels/vocab_head.hip.
 """
 from __future__ import annotations

@@ -49,7 +49,7 @@ def test_against_the_formula(gpu_lib, n, hidden, classes, piece):
 @gpu
 @pytest.mark.parametrize("n", [50, 300])
 def test_what_it_is_for(gpu_lib, n):
-    """Ordinary rows and an fp32 gradient of the weight: 2^-9 of d shows in it, and is gone."""
+    """Ordinary rows and an fp32 gradient of the weight: d's rounding, up to 2^-8 of a value, shows in it, and is gone."""
     h, w, y, _ = make(n, 64, 3000, "bf16", seed=n)
     x = Exact(h, w, y)
     _, lse = vocab_head_fwd(h, w, y)
