@@ -210,7 +210,7 @@ class GlobalNormClip:
             check(self.lib.dtf_clip_by_global_norm(ptr(self.table), self.chunks, self._in_place, ptr(part), self.slots, scale,
                                                    clip_norm, ptr(norm), stream), "clip_by_global_norm")
         torch.autograd.graph.increment_version(self._written)
-        return self.out, norm
+        return list(self.out), norm
 
 
 def _scale(scale: float) -> float:

@@ -86,6 +86,17 @@ def test_a_captured_call_is_not_recorded(plan):
     assert all(m.streams == [9] for m in p._memory)
 
 
+def test_the_list_of_outputs_is_the_callers(plan):
+    """What a caller does to the list that a call returned must not change the next call's."""
+    p, _ = plan
+    a, b = torch.zeros(1), torch.zeros(1)
+    p.out = [a, b]
+    got, _ = p.clip(1.0)
+    assert got[0] is a and got[1] is b
+    got.clear()
+    assert len(p.clip(1.0)[0]) == 2
+
+
 @gpu
 def test_memory_of_a_dropped_plan_is_not_handed_out_while_it_is_read(gpu_lib):
     """The call waits on its stream behind other work; the plan and its tensors are gone before it runs."""
