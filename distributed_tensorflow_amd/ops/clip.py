@@ -187,7 +187,8 @@ class GlobalNormClip:
     def norm(self, scale: float = 1.0) -> torch.Tensor:
         """``scale`` * norm of all tensors, an fp32 scalar on the device (infinity from 3.4e38 on)."""
         scale = _scale(scale)
-        no_autograd(self._requires)
+        if self._requires:
+            no_autograd(self._requires)
         with on_device(self.device) as stream:
             self._used_on(stream)
             part, norm = self._buffers()
@@ -203,7 +204,8 @@ class GlobalNormClip:
             raise ValueError(f"clip_norm must be positive and finite, got {clip_norm}")
         if self._clip_error:
             raise ValueError(self._clip_error)
-        no_autograd(self._requires)
+        if self._requires:
+            no_autograd(self._requires)
         with on_device(self.device) as stream:
             self._used_on(stream)
             part, norm = self._buffers()
