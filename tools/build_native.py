@@ -4,9 +4,9 @@
   libdtf_kernels.so  hand-written HIP kernels + step runtime (hipcc --offload-arch=gfx950)
   libdtf_ckpt.so     TF tensor-bundle (Saver V2) checkpoint codec (host C++)
 
-hipcc cross-compiles without a GPU, so this runs on the CPU-only build box.  The
-.so files land in distributed_tensorflow_amd/_lib/ (git-ignored, but shipped to
-the GPU box by gpurun).  Objects are cached under build/ by their sources' times and the command that made them.
+hipcc cross-compiles without a GPU, so this runs anywhere.  The .so files land in
+distributed_tensorflow_amd/_lib/ (git-ignored).  Objects are cached under build/ by
+their sources' times and the command that made them.
 ``--flags`` prints the compile flags for scripts that build kernels themselves.
 """
 from __future__ import annotations
